@@ -8,6 +8,13 @@ Python mirror of the op interface (aubier_amd.ops) and the seeded synthetic inpu
 from .ops import (  # noqa: F401
     MlaM4Error,
     Q8_0,
+    ggml_m4_kqkv_paged,
+    ggml_m4_kvrows,
+    ggml_m4_pages,
+    kqkv_paged_workspace_bytes,
+    supports_kqkv_paged,
+    supports_kvrows,
+    supports_pages,
     ggml_m4_phase_kvwrite,
     ggml_m4_phase_wvb,
     rope_params,

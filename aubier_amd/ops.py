@@ -101,6 +101,18 @@ _EXPORTS = {
                                                                               ctypes.POINTER(MlaTensor), ctypes.c_void_p]),
     "mla_m4_supports_phase_kvwrite": (ctypes.c_int, [ctypes.POINTER(MlaTensor)] * 6 + [ctypes.POINTER(RopeParams),
                                                                                        ctypes.POINTER(MlaTensor)]),
+    "mla_m4_pages": (ctypes.c_int, [ctypes.POINTER(MlaTensor)] * 4 + [ctypes.c_int32] + [ctypes.POINTER(MlaTensor)] * 3 +
+                     [ctypes.c_void_p]),
+    "mla_m4_supports_pages": (ctypes.c_int, [ctypes.POINTER(MlaTensor)] * 4 + [ctypes.c_int32] + [ctypes.POINTER(MlaTensor)] * 3),
+    "mla_m4_kvrows": (ctypes.c_int, [ctypes.POINTER(MlaTensor)] * 5 + [ctypes.POINTER(RopeParams), ctypes.POINTER(MlaTensor),
+                                                                       ctypes.c_void_p]),
+    "mla_m4_supports_kvrows": (ctypes.c_int, [ctypes.POINTER(MlaTensor)] * 5 + [ctypes.POINTER(RopeParams),
+                                                                                ctypes.POINTER(MlaTensor)]),
+    "mla_m4_kqkv_paged": (ctypes.c_int, [ctypes.POINTER(MlaTensor)] * 5 + [ctypes.c_int32, ctypes.POINTER(MlaTensor), ctypes.c_float,
+                                                                           ctypes.POINTER(MlaTensor), ctypes.c_void_p,
+                                                                           ctypes.c_size_t, ctypes.c_void_p]),
+    "mla_m4_kqkv_paged_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(MlaTensor)] * 4),
+    "mla_m4_supports_kqkv_paged": (ctypes.c_int, [ctypes.POINTER(MlaTensor)] * 5 + [ctypes.c_int32] + [ctypes.POINTER(MlaTensor)] * 2),
 }
 
 
@@ -200,6 +212,14 @@ def _stream(t: torch.Tensor) -> int:
 def _check(op: str, rc: int) -> None:
     if rc != 0:
         raise MlaM4Error(op, rc)
+
+
+def _on(op: str, *tensors):
+    """The device of the tensors as the current one for a launch (the ops of a paged batch): they lie on one GPU."""
+    devs = {t.device for t in tensors if t is not None}
+    if len(devs) != 1 or next(iter(devs)).type != "cuda":
+        raise MlaM4Error(op, -1)
+    return torch.cuda.device(next(iter(devs)))
 
 
 # ------------------------------------------------------------------------------------ ops
@@ -394,3 +414,77 @@ def supports_phase_kvwrite(cur, wkv_a, kv_norm, kcache, kidx, pos, rope: RopePar
     return bool(load_library().mla_m4_supports_phase_kvwrite(_ptr(view(cur)), _ptr(view(wkv_a)), _ptr(view(kv_norm)),
                                                              _ptr(view(kcache)), _ptr(view(kidx)), _ptr(view(pos)),
                                                              ctypes.byref(rope), _ptr(view(out))))
+
+
+# ------------------------------------------------------------------------------------ paged batches
+def ggml_m4_pages(past: torch.Tensor, n_new: torch.Tensor, free: torch.Tensor, table: torch.Tensor, page_size: int, n_rows: int,
+                  slot: Optional[torch.Tensor] = None, pos: Optional[torch.Tensor] = None, used: Optional[torch.Tensor] = None):
+    """Block tables and slot maps from request lengths (include/mla_m4.h mla_m4_pages): past, n_new int32 [n_seq];
+    free int32 [n_free], the ids that may be taken; table int32 [n_seq, max_pages], the new pages entered in place.
+    Returns slot int64 [n_rows] (-1: no cell), pos int32 [n_rows] and used int32 [2] (pages taken, rows of the batch)."""
+    lib = load_library()
+    dev = table.device
+    slot = torch.empty(n_rows, dtype=torch.int64, device=dev) if slot is None else slot
+    pos = torch.empty(n_rows, dtype=torch.int32, device=dev) if pos is None else pos
+    used = torch.empty(2, dtype=torch.int32, device=dev) if used is None else used
+    with _on("ggml_m4_pages", past, n_new, free, table, slot, pos, used):
+        _check("ggml_m4_pages", lib.mla_m4_pages(_ptr(view(past)), _ptr(view(n_new)), _ptr(view(free)), _ptr(view(table)), int(page_size),
+                                                 _ptr(view(slot)), _ptr(view(pos)), _ptr(view(used)), _stream(table)))
+    return slot, pos, used
+
+
+def ggml_m4_kvrows(x: torch.Tensor, kv_norm: torch.Tensor, kcache, slot: torch.Tensor, pos: torch.Tensor, rope: RopeParams,
+                   out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """A batch's latent rows into the cache (include/mla_m4.h mla_m4_kvrows): x f32 or f16 [n_rows, d_lat + n_dims], the
+    wkv_a product; kv_norm f32 [d_lat]; kcache f16 [n_cells, d_lat + n_dims] or Q8_0, row slot[r] written in place (none for
+    a slot outside the cache); slot int64 [n_rows], pos int32 [n_rows] -> Kcur f32 [n_rows, d_lat + n_dims]."""
+    lib = load_library()
+    if out is None:
+        out = torch.empty(x.shape, dtype=torch.float32, device=x.device)
+    with _on("ggml_m4_kvrows", x, kv_norm, kcache, slot, pos, out):
+        _check("ggml_m4_kvrows", lib.mla_m4_kvrows(_ptr(view(x)), _ptr(view(kv_norm)), _ptr(view(kcache)), _ptr(view(slot)),
+                                                   _ptr(view(pos)), ctypes.byref(rope), _ptr(view(out)), _stream(x)))
+    return out
+
+
+def kqkv_paged_workspace_bytes(kcache, q: torch.Tensor, past: torch.Tensor, out: torch.Tensor) -> int:
+    return int(load_library().mla_m4_kqkv_paged_workspace_bytes(_ptr(view(kcache)), _ptr(view(q)), _ptr(view(past)), _ptr(view(out))))
+
+
+def ggml_m4_kqkv_paged(kcache, q: torch.Tensor, past: torch.Tensor, n_new: torch.Tensor, table: torch.Tensor, page_size: int,
+                       kq_scale: float, prefix: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
+                       workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """KQKV over the pages of a batch (include/mla_m4.h mla_m4_kqkv_paged): token i of request b sees the first
+    past[b] + i + 1 cells of table[b].  kcache [n_cells, D_k] f16 or Q8_0; q [nt, H, D_k] f32 or f16; past, n_new int32
+    [n_seq]; table int32 [n_seq, max_pages]; prefix int32 [2] (cells, requests) or None: the first requests' tables begin
+    with the same pages, whose cells are then read once for all of them.  out [H, nt, D_v], of q's type unless given; rows
+    behind the last request are left as they are (in a new `out`: not set).  workspace: optional uint8 device buffer."""
+    lib = load_library()
+    if out is None:
+        out = torch.empty((q.shape[1], q.shape[0], _dv_of(kcache)), dtype=q.dtype, device=q.device)
+    with _on("ggml_m4_kqkv_paged", kcache, q, past, n_new, table, prefix, out, workspace):
+        vk, vq, vp, vo = view(kcache), view(q), view(past), view(out)
+        if workspace is None:
+            need = int(lib.mla_m4_kqkv_paged_workspace_bytes(_ptr(vk), _ptr(vq), _ptr(vp), _ptr(vo)))
+            workspace = torch.empty(need, dtype=torch.uint8, device=q.device) if need > 0 else None
+        ws_ptr = workspace.data_ptr() if workspace is not None else None
+        ws_bytes = workspace.numel() * workspace.element_size() if workspace is not None else 0
+        _check("ggml_m4_kqkv_paged", lib.mla_m4_kqkv_paged(_ptr(vk), _ptr(vq), _ptr(vp), _ptr(view(n_new)), _ptr(view(table)),
+                                                           int(page_size), _ptr(view(prefix)), ctypes.c_float(kq_scale), _ptr(vo),
+                                                           ws_ptr, ws_bytes, _stream(q)))
+    return out
+
+
+def supports_pages(past, n_new, free, table, page_size: int, slot, pos, used) -> bool:
+    return bool(load_library().mla_m4_supports_pages(_ptr(view(past)), _ptr(view(n_new)), _ptr(view(free)), _ptr(view(table)),
+                                                     int(page_size), _ptr(view(slot)), _ptr(view(pos)), _ptr(view(used))))
+
+
+def supports_kvrows(x, kv_norm, kcache, slot, pos, rope: RopeParams, out) -> bool:
+    return bool(load_library().mla_m4_supports_kvrows(_ptr(view(x)), _ptr(view(kv_norm)), _ptr(view(kcache)), _ptr(view(slot)),
+                                                      _ptr(view(pos)), ctypes.byref(rope), _ptr(view(out))))
+
+
+def supports_kqkv_paged(kcache, q, past, n_new, table, page_size: int, prefix, out) -> bool:
+    return bool(load_library().mla_m4_supports_kqkv_paged(_ptr(view(kcache)), _ptr(view(q)), _ptr(view(past)), _ptr(view(n_new)),
+                                                          _ptr(view(table)), int(page_size), _ptr(view(prefix)), _ptr(view(out))))

@@ -263,6 +263,88 @@ int mla_m4_phase_kvwrite(const mla_m4_tensor * cur, const mla_m4_tensor * wkv_a,
                          const mla_m4_rope_params * rope, const mla_m4_tensor * dst, void * stream);
 
 /* -------------------------------------------------------------------------------------------
+ * Paged batches -- no counterpart in the reference, whose batch-of-N session keeps every sequence in a
+ * fixed region of one window.  Here the cache is a pool of pages of page_size cells (rows of D_k), a
+ * power of two in 16 .. 65536, and a request's cells are listed page by page in its block table: cell j
+ * of request b is row table[b][j / page_size] * page_size + j % page_size of the cache.  A call serves
+ * n_seq requests (at most 4096); request b holds past[b] cells and adds n_new[b] tokens (0: none), and
+ * the tokens' rows follow one another in request order, at most 65535 of them.
+ *   past, n_new  I32 ne [n_seq]               read on the device; negative values count as 0
+ *   table        I32 ne [max_pages, n_seq]    nb[0] = 4, any 4-byte multiple between requests
+ * A step: mla_m4_pages (the new tokens' pages, slots and positions), mla_m4_kvrows (their rows into the
+ * cache), mla_m4_wkb, mla_m4_kqkv_paged, mla_m4_phase_wvb.  All lengths stay on the device, so a captured
+ * step replays with new ones.
+ * ------------------------------------------------------------------------------------------- */
+
+/* Block tables and slot maps from request lengths, one launch.  Request b starts the pages
+ * ceil(past / page_size) .. ceil((past + n_new) / page_size) - 1 of its table; they are taken from the
+ * free list in request order and entered in the table.  For the row of a token at position p
+ *   slot = its cell (page * page_size + p % page_size), pos = p,
+ * and slot = -1 where there is no page: past the free list's end (the table gets -1 there too), past the
+ * table's width, or where the table holds a negative id.  Rows behind the last request get slot -1 and
+ * pos 0.  Nothing else of the table is written, and the lengths and the list are not changed: the caller
+ * moves on by used.
+ *   free  I32 ne [n_free]   page ids, distinct; may be empty
+ *   slot  I64 ne [n_rows], pos I32 ne [n_rows]   n_rows: the rows there is room for; tokens past it are
+ *                                                no part of the batch
+ *   used  I32 ne [2]        pages taken from the list, rows of the batch */
+int mla_m4_pages(const mla_m4_tensor * past, const mla_m4_tensor * n_new, const mla_m4_tensor * free_ids,
+                 const mla_m4_tensor * table, int32_t page_size, const mla_m4_tensor * slot,
+                 const mla_m4_tensor * pos, const mla_m4_tensor * used, void * stream);
+
+/* The rows of a batch into the cache: what KV-write does behind its product, for n_rows tokens.
+ *   x        F32|F16 ne [d_lat + n_dims, n_rows]  the wkv_a product; rows 4 elements aligned
+ *   kv_norm  F32 ne [d_lat]                       16-byte aligned
+ *   kcache   F16 ne [d_lat + n_dims, n_cells]     rows 8-byte aligned; or Q8_0, rows 2-byte aligned
+ *   slot     I64 ne [n_rows], pos I32 ne [n_rows]
+ *   dst      F32 ne [d_lat + n_dims, n_rows]      Kcur, 16-byte aligned rows; or NULL
+ * Columns [0, d_lat): x / sqrt(mean of squares + eps) * kv_norm; [d_lat, d_lat + n_dims): rope, NORMAL
+ * mode with YaRN, as phase 0, the angles taken in 64 bits.  The row goes to cache row slot, rounded as
+ * phase 0 does (f16, or ggml's f32 -> q8_0); a slot outside [0, n_cells) stores nothing.  Kcur is
+ * written for every row.  Slots are distinct: of two rows with one slot, either's values may end up
+ * there.  d_lat and n_dims multiples of 32, n_dims <= 256, d_lat + n_dims <= 1024. */
+int mla_m4_kvrows(const mla_m4_tensor * x, const mla_m4_tensor * kv_norm, const mla_m4_tensor * kcache,
+                  const mla_m4_tensor * slot, const mla_m4_tensor * pos, const mla_m4_rope_params * rope,
+                  const mla_m4_tensor * dst, void * stream);
+
+/* KQKV over the pages of a batch: token i of request b sees the first past[b] + i + 1 cells of its table,
+ *   dst[h][t][:] = softmax_j(kq_scale * q[t][h] . K[j]) . V[j][:]
+ * with V the first D_v columns of K.
+ *   kcache  F16 ne [D_k, n_cells]   nb[1] a multiple of 16; or Q8_0, contiguous rows; 16-byte aligned.  Of
+ *                                   any size: there is no 4 GiB bound
+ *   q       F32|F16 ne [D_k, H, nt] nb[0] = element size, 16-byte aligned strides, H <= 1024
+ *   prefix  I32 ne [2], or NULL     (cells, requests): the tables of the first `requests` requests begin
+ *                                   with the same pages, for at least `cells` cells.  Those cells are
+ *                                   then read and multiplied once for all of them, through request 0's
+ *                                   table.  Without it, or where fewer cells are held by one of them,
+ *                                   the result is the same up to rounding
+ *   dst     F32|F16 ne [D_v, nt, H] contiguous; rows of tokens behind the last request are not written
+ * (D_k, D_v) = (576, 512) or (320, 256).  A page id outside the pool has no cells: the keys there are not
+ * seen.  A token that sees no key gets zeros.  What lies in cells that no token of a request sees (the
+ * rest of its last page) does not matter, NaN and infinities included.
+ * q and the weights of the softmax enter the products as f16, the sums are f32 (as mla_m4_kqkv over an F16
+ * cache); a Q8_0 cache is computed as f16(q d).
+ * workspace: device memory, >= mla_m4_kqkv_paged_workspace_bytes(), 16-byte aligned, not shared by calls
+ * that may overlap. */
+int mla_m4_kqkv_paged(const mla_m4_tensor * kcache, const mla_m4_tensor * q, const mla_m4_tensor * past,
+                      const mla_m4_tensor * n_new, const mla_m4_tensor * table, int32_t page_size,
+                      const mla_m4_tensor * prefix, float kq_scale, const mla_m4_tensor * dst,
+                      void * workspace, size_t workspace_bytes, void * stream);
+size_t mla_m4_kqkv_paged_workspace_bytes(const mla_m4_tensor * kcache, const mla_m4_tensor * q,
+                                         const mla_m4_tensor * past, const mla_m4_tensor * dst);
+
+/* their supports_op mirrors, as below */
+int mla_m4_supports_pages(const mla_m4_tensor * past, const mla_m4_tensor * n_new, const mla_m4_tensor * free_ids,
+                          const mla_m4_tensor * table, int32_t page_size, const mla_m4_tensor * slot,
+                          const mla_m4_tensor * pos, const mla_m4_tensor * used);
+int mla_m4_supports_kvrows(const mla_m4_tensor * x, const mla_m4_tensor * kv_norm, const mla_m4_tensor * kcache,
+                           const mla_m4_tensor * slot, const mla_m4_tensor * pos,
+                           const mla_m4_rope_params * rope, const mla_m4_tensor * dst);
+int mla_m4_supports_kqkv_paged(const mla_m4_tensor * kcache, const mla_m4_tensor * q, const mla_m4_tensor * past,
+                               const mla_m4_tensor * n_new, const mla_m4_tensor * table, int32_t page_size,
+                               const mla_m4_tensor * prefix, const mla_m4_tensor * dst);
+
+/* -------------------------------------------------------------------------------------------
  * supports_op mirrors (ggml-cuda.cu:5848-5885): 1 if the entry point above accepts these
  * tensors, 0 otherwise.  They run the same host-side contract checks as the launch, without
  * launching, so the backend's supports_op and the launcher cannot disagree.  Data pointers may
