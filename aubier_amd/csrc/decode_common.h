@@ -110,6 +110,8 @@ struct SliceDma { i32x4 krs, mrs; uint32_t sb; };
 template <int DK>
 struct SliceStream {
     using G = SliceGeom<DK>;
+    using Dma = SliceDma;
+    static constexpr int MASK = 1;      // mask DMA instructions per slice
     const char * kc;
     int64_t kc_nb1;
     const float * mrow;     // this token's mask row (or any valid pointer when there is none)
@@ -349,15 +351,15 @@ __device__ __forceinline__ void mfma16(f32x4 & acc, const half8 & a, const half8
 
 // S^T = K . Q^T for the wave's 16 keys of the slice at sb (C rows = keys 4 g + r, C cols = heads
 // j16 (acc0) and 16 + j16 (acc1)).  DMA accounting (instructions complete in issue order): the
-// slice is DMA_N blocks then the mask, step s reading blocks 2 (s >> 1) and 2 (s >> 1) + 1; before
+// slice is DMA_N blocks then the mask (SS::MASK = 0: a stream without one), step s reading blocks 2 (s >> 1) and 2 (s >> 1) + 1; before
 // that read, the blocks after them, the mask and the next slice's instructions issued so far (one
 // per completed step) may still be in flight.
 // With DMA, the next slice's DMA (dn, streaming cache policy) is spread over the steps.  Operand
 // reads run QPF steps ahead of their MFMAs; the scheduling barriers keep the compiler from sinking
 // them back next to their use.  Two accumulator chains per head tile (even / odd steps) keep
 // consecutive MFMAs independent.  Returns with the slice's mask slot landed.
-template <int DK, bool DMA>
-__device__ __forceinline__ void qk_slice(const SliceStream<DK> & ss, const SliceDma & dn, const char * sb, int lane,
+template <int DK, bool DMA, typename SS = SliceStream<DK>>
+__device__ __forceinline__ void qk_slice(const SS & ss, const typename SS::Dma & dn, const char * sb, int lane,
                                          const half8 (&qreg)[2][SliceGeom<DK>::QSTEPS], f32x4 & s0, f32x4 & s1) {
     using G = SliceGeom<DK>;
     constexpr int QPF = 4;
@@ -368,7 +370,7 @@ __device__ __forceinline__ void qk_slice(const SliceStream<DK> & ss, const Slice
     const int a0 = slot_byte(j16, g);
     auto arow = [&](int st) { return reinterpret_cast<const half8 *>(sb + (a0 ^ (64 * (st & 1))) + 2048 * (st >> 1)); };
     half8 abuf[QPF];
-    wait_vm<G::DMA_N + 1 - QPF>();      // blocks 0 .. QPF - 1
+    wait_vm<G::DMA_N + SS::MASK - QPF>();      // blocks 0 .. QPF - 1
 #pragma unroll
     for (int s = 0; s < QPF; ++s) abuf[s] = *arow(s);
 #pragma unroll
@@ -376,7 +378,7 @@ __device__ __forceinline__ void qk_slice(const SliceStream<DK> & ss, const Slice
         const half8 av = abuf[s % QPF];
         if (s + QPF < G::QSTEPS) {
             // blocks 0 .. 2 ((s + QPF) >> 1) + 1 landed; s instructions of the next slice issued
-            const int later = G::DMA_N - 1 - 2 * ((s + QPF) >> 1);
+            const int later = G::DMA_N - 2 + SS::MASK - 2 * ((s + QPF) >> 1);
             if constexpr (DMA) wait_vm_le(later + s);
             else wait_vm_le(later);
             abuf[s % QPF] = *arow(s + QPF);
@@ -391,11 +393,11 @@ __device__ __forceinline__ void qk_slice(const SliceStream<DK> & ss, const Slice
         if constexpr (DMA) ss.put(dn, s);
         __builtin_amdgcn_sched_barrier(0);
     }
-    if constexpr (DMA) {
+    if constexpr (!DMA) {
+        wait_vm<0>();
+    } else if constexpr (SS::MASK != 0) {
         ss.put(dn, G::DMA_N);
         wait_vm<G::DMA_N + 1>();             // the mask slot (the next slice's DMA_N + 1 may be in flight)
-    } else {
-        wait_vm<0>();
     }
     s0 = acc0 + acc2;
     s1 = acc1 + acc3;

@@ -54,7 +54,6 @@ hipError_t launch_kvrows(const KvRowsArgs & a, hipStream_t stream);
 struct AttnArgs {
     const char * kc;
     int64_t kc_nb1;
-    int64_t n_pages;
     const char * q;         // rows' heads: q + token * q_nb2 + head * q_nb1
     int64_t q_nb1, q_nb2;
     const int32_t * past;
@@ -65,11 +64,12 @@ struct AttnArgs {
     char * dst;             // [H][nt][D_v]
     char * work;
     float scale_log2;
-    int n_seq, max_pages, page_shift, n_head, nt;
+    int n_seq, max_pages, n_pages, page_shift, n_head, nt;
     int q_f16, dst_f16;
 };
 bool attn_supported(int dk, int dv);
 size_t attn_workspace_bytes(int dk, int dv, int n_seq, int n_head, int nt);
+constexpr int64_t MAX_STRIDE = 1 << 25;   // bytes between rows of the cache, heads and tokens of q: 32-bit offsets inside a tile
 hipError_t launch_attn(int dk, int dv, bool q8, const AttnArgs & a, hipStream_t stream);
 
 }  // namespace paged

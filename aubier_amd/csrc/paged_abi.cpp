@@ -146,6 +146,7 @@ int check_attn(const mla_m4_tensor * kc, const mla_m4_tensor * q, const mla_m4_t
     if (rc != MLA_M4_OK) return rc;
     if (kc->ne[1] < page_size) return MLA_M4_ERR_SHAPE;         // not one page
     if (!pg::attn_supported((int)(kc->ne[0] > 4096 ? 0 : kc->ne[0]), (int)(dst->ne[0] > 4096 ? 0 : dst->ne[0]))) return MLA_M4_ERR_UNSUPPORTED;
+    if (kc->nb[1] > pg::MAX_STRIDE || q->nb[1] > pg::MAX_STRIDE || q->nb[2] > pg::MAX_STRIDE) return MLA_M4_ERR_UNSUPPORTED;
     if (q->ne[1] > 1024 || q->ne[2] > pg::MAX_ROWS || kc->ne[1] / page_size > INT32_MAX) return MLA_M4_ERR_UNSUPPORTED;
     return MLA_M4_OK;
 }
@@ -237,7 +238,7 @@ int mla_m4_kqkv_paged(const mla_m4_tensor * kcache, const mla_m4_tensor * q, con
     pg::AttnArgs a{};
     a.kc = static_cast<const char *>(kcache->data);
     a.kc_nb1 = (int64_t)kcache->nb[1];
-    a.n_pages = kcache->ne[1] / page_size;
+    a.n_pages = (int)(kcache->ne[1] / page_size);
     a.q = static_cast<const char *>(q->data);
     a.q_nb1 = (int64_t)q->nb[1];
     a.q_nb2 = (int64_t)q->nb[2];

@@ -1,0 +1,674 @@
+// paged_pass.h -- one piece of the attention over pages (kqkv_paged.hip): up to 128 rows against a run of 64-key
+// tiles whose cells are found through a block table.  Two forms, on the decode and the prefill kernels' products:
+// up to 32 rows (the four waves share the keys of Q.K^T and the columns of P.V) and up to 128 (a wave per 32 rows).
+//
+// A row is a (token, head) pair of the piece's rows, numbered token * H + head, so any head count and any number of
+// tokens fill the matrix instructions' 32 columns.  Pages are multiples of 16 cells, so a wave's 16-key slice of a
+// tile lies in one page: its address is one scalar load of the table and a buffer resource at the page's own 64-bit
+// base, whose record count ends with the last cell that is seen.  Cells past it read as zeros, whatever they hold.
+#pragma once
+
+#include "paged_common.h"
+#include "q8_slice.h"
+
+namespace mla {
+namespace paged {
+
+using namespace decode;
+
+// LDS DMA as mla_common.h's dma16, with the five wait states that a vector-memory instruction needs behind a vector
+// instruction that writes one of its scalar registers (a v_readlane that brings back a spilled resource, a
+// v_readfirstlane): the compiler does not see that this text holds one, and without them the load has gone to the
+// address that the registers held before.
+template <bool NT>
+__device__ __forceinline__ void page_dma16(i32x4 rsrc, uint32_t voff, uint32_t soff, uint32_t lds_base) {
+    if constexpr (NT)
+        asm volatile("s_nop 4\n\tbuffer_load_dwordx4 %0, %1, %2 offen nt lds" :: "v"(voff), "s"(rsrc), "s"(soff), "{m0}"(lds_base) : "memory");
+    else
+        asm volatile("s_nop 4\n\tbuffer_load_dwordx4 %0, %1, %2 offen lds" :: "v"(voff), "s"(rsrc), "s"(soff), "{m0}"(lds_base) : "memory");
+}
+
+constexpr int BLOCK_ROWS = 128;             // rows of the wide form
+
+// Where the keys of a piece are and which of its rows sees which (uniform over the workgroup)
+struct Piece {
+    int row0, rows;         // its rows: flat rows row0 .. row0 + rows - 1 of the tokens from tok0 on
+    int tok0;               // batch row of that first token
+    int past;               // flat row r sees the keys before min(past + r / H + 1, key1)
+    int key0, key1;         // the keys: tile k holds key0 + 64 k .. + 63, those before key1
+    int ta, tb;             // its tiles
+    int lim_min;            // the fewest keys that a row sees
+    const int32_t * table;  // the block table
+    int slot;               // the record that takes the result, or -1: it is complete and goes to dst
+};
+
+// Records: (m, l) of the block's 128 rows, m in log2 units (a reference for the scores, at most 15 below their
+// maximum; -inf: no key), then o / l in f16, D_v per row.
+template <int DV>
+constexpr size_t record_bytes() { return BLOCK_ROWS * 8 + (size_t)BLOCK_ROWS * DV * 2; }
+
+template <int DK, int DV, bool Q8>
+struct PieceLds {
+    using G = SliceGeom<DK>;
+    static constexpr int SLOT8 = Q8 ? Q8Geom<DK>::ROWS_BYTES : 0;       // an int8 slice
+    static constexpr int TILE = 2 * NWAVE * SLOT8;                      // the f16 tile behind the int8 ring
+    static constexpr int RING = Q8 ? TILE + NWAVE * G::STAGE : G::RING;
+    __attribute__((aligned(16))) char ring[RING];
+    __attribute__((aligned(16))) half_t px[Q8 ? 1 : 2][HG * DecodeCfg<DK, DV>::PROW];
+    __attribute__((aligned(16))) float red[2][HG][NWAVE];
+    __attribute__((aligned(16))) int64_t qoff[BLOCK_ROWS];              // byte offset of a row's q from the first token's
+    int drow[BLOCK_ROWS];                                               // its row of dst (head * nt + token), -1: none
+    int lim[BLOCK_ROWS];                                                // keys it sees
+    // cells of a slice that are seen (by tile modulo 4: tile k + 2's are written while others read tile k's), and
+    // the rows of a slice that hold a NaN or an infinity (by tile parity)
+    __attribute__((aligned(16))) int vc[4][NWAVE];
+    uint64_t bad[2][NWAVE][2];
+};
+
+// the thread index by way of an opaque move, so that what follows from it is computed where it is used, rather than
+// before the loop over pieces and kept (or spilled) through it
+__device__ __forceinline__ int opaque_tid() {
+    int t;
+    asm volatile("v_mov_b32 %0, %1" : "=v"(t) : "v"(threadIdx.x));
+    return t;
+}
+
+__device__ __forceinline__ void piece_rows(const AttnArgs & a, const Piece & p, int64_t * qoff, int * drow, int * lim) {
+    const int tid = threadIdx.x;
+    if (tid >= BLOCK_ROWS) return;
+    const int r = p.row0 + tid;
+    const int t = r / a.n_head, h = r - t * a.n_head;
+    const bool live = tid < p.rows;
+    qoff[tid] = live ? (int64_t)t * a.q_nb2 + (int64_t)h * a.q_nb1 : 0;
+    drow[tid] = live ? h * a.nt + p.tok0 + t : -1;
+    lim[tid] = live ? min(p.past + t + 1, p.key1) : 0;
+}
+
+// A wave's view of a piece's keys
+template <int DK>
+struct PageStream {
+    using G = SliceGeom<DK>;
+    struct Dma { i32x4 krs; uint32_t sb; int n; };      // n: cells of the slice that are seen
+    static constexpr int MASK = 0;
+    const char * kc;
+    int64_t kc_nb1;
+    const int32_t * table;
+    int n_pages, shift, key0, key1, w;
+    uint32_t ring_lds, kvoff0, kvoff1;
+
+    __device__ __forceinline__ PageStream(const AttnArgs & a, const Piece & p, int w_, uint32_t ring_lds_, int lane) {
+        kc = a.kc;
+        kc_nb1 = a.kc_nb1;
+        table = p.table;
+        n_pages = a.n_pages;
+        shift = a.page_shift;
+        key0 = p.key0;
+        key1 = p.key1;
+        w = w_;
+        ring_lds = ring_lds_;
+        const int r0 = 2 * (lane >> 4) + ((lane >> 3) & 1);
+        kvoff0 = (uint32_t)(r0 * (uint32_t)kc_nb1) + 16u * (uint32_t)((lane & 7) ^ row_sw(r0));
+        kvoff1 = (uint32_t)((r0 + 8) * (uint32_t)kc_nb1) + 16u * (uint32_t)((lane & 7) ^ row_sw(r0 + 8));
+    }
+    // the wave's slice of tile k: its first cell and how many cells of it are seen
+    __device__ __forceinline__ int slice(int k, int64_t & cell) const {
+        const int key = key0 + k * TK + WK * w;
+        cell = 0;
+        if (key >= key1) return 0;
+        const int id = __builtin_amdgcn_readfirstlane(*(const __attribute__((address_space(4))) int32_t *)(uintptr_t)(table + (key >> shift)));
+        if (id < 0 || id >= n_pages) return 0;
+        cell = ((int64_t)id << shift) + (key & ((1 << shift) - 1));
+        return min(WK, key1 - key);
+    }
+    __device__ __forceinline__ Dma plan(int s, int k) const {
+        Dma d;
+        int64_t cell;
+        d.n = slice(k, cell);
+        d.krs = make_rsrc(kc + cell * kc_nb1, d.n > 0 ? (uint32_t)((int64_t)(d.n - 1) * kc_nb1 + DK * 2) : 0u);
+        d.sb = ring_lds + (uint32_t)((s * NWAVE + w) * G::STAGE);
+        return d;
+    }
+    template <bool NT = true>
+    __device__ __forceinline__ void put(const Dma & d, int i) const {
+        const uint32_t vo = (i & 1) ? kvoff1 : kvoff0, so = 128u * (uint32_t)(i >> 1);
+        page_dma16<NT>(d.krs, vo, so, d.sb + (uint32_t)(1024 * i));
+    }
+    // the same over an 8-bit cache: the slice as linear 16-byte chunks into its int8 slot of stage s, N8 instructions
+    static constexpr int ROWB = DK / 32 * 34, SLOT8 = WK * ROWB, FULL8 = SLOT8 / 1024, TAIL8 = SLOT8 % 1024 / 16, N8 = FULL8 + 1;
+    static_assert(TAIL8 > 0, "a partial last instruction");
+    template <bool NT = true>
+    __device__ __forceinline__ int put8(int s, int k, int lane) const {
+        int64_t cell;
+        const int n = slice(k, cell);
+        const i32x4 krs = make_rsrc(kc + cell * ROWB, (uint32_t)(n * ROWB));
+        const uint32_t sb = ring_lds + (uint32_t)((s * NWAVE + w) * SLOT8), vo = 16u * (uint32_t)lane;
+#pragma unroll
+        for (int i = 0; i < FULL8; ++i) page_dma16<NT>(krs, vo, 1024u * (uint32_t)i, sb + 1024u * (uint32_t)i);
+        if (lane < TAIL8) page_dma16<NT>(krs, vo, 1024u * (uint32_t)FULL8, sb + 1024u * (uint32_t)FULL8);
+        return n;
+    }
+};
+
+// Non-finite values of an f16 slice set to zero (the whole wavefront, its own slice); b0, b1: which of rows 0 .. 7 and
+// 8 .. 15 held one (a byte per row).  Only for the tiles that some rows of a piece see and others do not: a cell that
+// a row does not see has weight 0 there, and 0 times a NaN or an infinity would reach its sums.
+template <int DK>
+__device__ __forceinline__ void clear_nonfinite(char * sb, int lane, uint64_t & b0, uint64_t & b1) {
+    b0 = b1 = 0;
+    for (int i = 0; i < SliceGeom<DK>::DMA_N; ++i) {        // 1 KB block i: rows 8 (i & 1) .. + 7, eight lanes a row
+        u32x4 * at = reinterpret_cast<u32x4 *>(sb + 1024 * i + 16 * lane);
+        u32x4 v = *at;
+        bool any = false;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            const uint32_t x = ((v[c] & 0x7c007c00u) + 0x04000400u) & 0x80008000u;      // exponent all ones
+            any |= x != 0;
+            v[c] &= ~((x >> 15) * 0xffffu);
+        }
+        const uint64_t b = __builtin_amdgcn_ballot_w64(any);
+        if (b != 0) *at = v;
+        if (i & 1) b1 |= b;
+        else b0 |= b;
+    }
+}
+
+// o / l of 32 rows (row0 .. of the block) to the record or, complete, to dst, in f16 through LDS rows of PITCH bytes
+// at stg: columns c0 .. c0 + NC - 1, whole 16-byte chunks, whole lines per instruction
+template <int DV, int NC, int PITCH>
+__device__ __forceinline__ void rows_out_f16(const AttnArgs & a, const Piece & p, char * rec, const char * stg, int row0, int c0,
+                                             const int * drow, int lane) {
+    constexpr int CPR = NC / 8;
+#pragma unroll
+    for (int it = 0; it < CPR / 2; ++it) {
+        const int q = 64 * it + lane;
+        const int row = q / CPR, ch = q % CPR;
+        const u32x4 v = *reinterpret_cast<const u32x4 *>(stg + row * PITCH + 16 * ch);
+        if (p.slot >= 0) {
+            __builtin_nontemporal_store(v, reinterpret_cast<u32x4 *>(rec + BLOCK_ROWS * 8 + ((size_t)(row0 + row) * DV + c0 + 8 * ch) * 2));
+        } else {
+            const int dr = drow[row0 + row];
+            if (dr >= 0) *reinterpret_cast<u32x4 *>(a.dst + ((size_t)dr * DV + c0 + 8 * ch) * 2) = v;
+        }
+    }
+}
+
+// a lane's four columns of one row, f32, complete, to dst
+__device__ __forceinline__ void out_f32(const AttnArgs & a, int dr, int dv, int col, f32x4 v) {
+    if (dr >= 0) *reinterpret_cast<f32x4 *>(a.dst + ((size_t)dr * dv + col) * 4) = v;
+}
+
+template <int N>
+__device__ __forceinline__ void scale_acc(f32x16 (&o)[N], float f) {
+    // in place on the accumulator registers (kept in AGPRs); the s_nops cover the MFMA -> VALU read distance
+    asm volatile("s_nop 7\n\ts_nop 7\n\ts_nop 7" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            float tmp;
+            asm volatile("v_accvgpr_read_b32 %1, %0\n\tv_mul_f32 %1, %1, %2\n\tv_accvgpr_write_b32 %0, %1"
+                         : "+a"(o[i][r]), "=&v"(tmp) : "v"(f));
+        }
+    asm volatile("s_nop 7" ::: "memory");
+}
+
+// ---------------------------------------------------------------- up to 32 rows
+// (of one block, row0 = 0: at most 32 tokens and heads, so the rows' q lie within 2 GiB of the first, MAX_STRIDE)
+// q of the 32 rows into LDS at qs (f32: q_convert's layout; f16: two slices of 16 rows, as K rows lie), this wave's
+// share; QN instructions
+constexpr uint32_t NO_ROW = 0x80000000u;    // an offset past the resource's records: reads zeros
+template <int DK, bool F16>
+__device__ __forceinline__ void q_rows_dma(const AttnArgs & a, const Piece & p, const int64_t * qoff, uint32_t qs, int w, int lane) {
+    using G = SliceGeom<DK>;
+    const i32x4 rs = make_rsrc(a.q + (int64_t)p.tok0 * a.q_nb2, NO_ROW);
+    if constexpr (F16) {
+        const int r0 = 2 * (lane >> 4) + ((lane >> 3) & 1), row = 8 * w + r0;
+        const uint32_t vo = row < p.rows ? (uint32_t)qoff[row] + 16u * (uint32_t)((lane & 7) ^ row_sw(r0)) : NO_ROW;
+#pragma unroll
+        for (int i = 0; i < G::DMA_N / 2; ++i)
+            page_dma16<false>(rs, vo, 128u * (uint32_t)i, qs + (uint32_t)((w >> 1) * G::STAGE + 1024 * (2 * i + (w & 1))));
+    } else {
+#pragma unroll
+        for (int i = 0; i < G::QD; ++i) {
+            const int x = (w * G::QD + i) * 64 + lane;
+            const int h = x / G::QC, c = (x - h * G::QC) ^ (h & 15);
+            page_dma16<false>(rs, h < p.rows ? (uint32_t)qoff[h] + 16u * (uint32_t)c : NO_ROW, 0u, qs + (uint32_t)((w * G::QD + i) * 1024));
+        }
+    }
+}
+
+template <int DK, int DV, bool Q8>
+__device__ __forceinline__ void narrow_piece(const AttnArgs & a, const Piece & p, PieceLds<DK, DV, Q8> & sh, char * rec) {
+    using G = SliceGeom<DK>;
+    using C = DecodeCfg<DK, DV>;
+    using S = PageStream<DK>;
+    using L = PieceLds<DK, DV, Q8>;
+    const int tid = opaque_tid(), lane = tid & 63;
+    const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int g = lane >> 4, j16 = lane & 15;
+    const S ss(a, p, w, lds_addr(sh.ring), lane);
+    const int n_my = p.tb - p.ta;
+
+    // ---- q by way of LDS the stream does not use yet, the first tile (8 bits: two tiles) behind it ----
+    half8 qreg[2][G::QSTEPS];
+    char * qs = Q8 ? sh.ring + L::TILE : sh.ring + NWAVE * G::STAGE;
+    if (a.q_f16) q_rows_dma<DK, true>(a, p, sh.qoff, lds_addr(qs), w, lane);
+    else q_rows_dma<DK, false>(a, p, sh.qoff, lds_addr(qs), w, lane);
+    int n_cur, n_nxt = 0;                    // cells that are seen, of this wave's slice of the tile and of the next
+    if constexpr (Q8) {
+        n_cur = ss.put8(0, p.ta, lane);
+        if (n_my > 1) {
+            n_nxt = ss.put8(1, p.ta + 1, lane);
+            wait_vm<2 * S::N8>();
+        } else {
+            wait_vm<S::N8>();
+        }
+    } else {
+        const typename S::Dma d0 = ss.plan(0, p.ta);
+#pragma unroll
+        for (int i = 0; i < G::DMA_N; ++i) ss.put(d0, i);
+        n_cur = d0.n;
+        wait_vm<G::DMA_N>();
+    }
+    __syncthreads();
+    if (a.q_f16) {
+        const int a0 = slot_byte(j16, g);
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int s = 0; s < G::QSTEPS; ++s)
+                qreg[n][s] = *reinterpret_cast<const half8 *>(qs + n * G::STAGE + (a0 ^ (64 * (s & 1))) + 2048 * (s >> 1));
+    } else {
+        q_convert<DK>(qs, lane, qreg);
+    }
+    const int lim[2] = {sh.lim[j16], sh.lim[16 + j16]};
+    __syncthreads();
+
+    float m_ref[2] = {M_NONE, M_NONE};       // rows 16 n + j16, log2 units
+    float l_acc = 0.0f;                      // row lane & 31, keys 8 (lane >> 5) .. + 7 of each slice
+    f32x16 o[C::NTQ];                        // o^T tiles, as kqkv_decode.hip
+#pragma unroll
+    for (int i = 0; i < C::NTQ; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[i][r] = 0.0f;
+    const PvAddr pv(lane);
+
+    for (int k = 0; k < n_my; ++k) {
+        const int par = k & 1;
+        const int key = p.key0 + (p.ta + k) * TK + WK * w;       // this wave's first key
+        f32x4 s0, s1;
+        char * sb;
+        int n_new = 0;
+        if constexpr (Q8) {
+            if (k + 1 < n_my) wait_vm<S::N8>();
+            else wait_vm<0>();
+            if (k > 0) __syncthreads();      // every wave is past the P.V of tile k - 1
+            sb = sh.ring + L::TILE + w * G::STAGE;
+            qk_slice_q8<DK, DV>(sh.ring + (par * NWAVE + w) * L::SLOT8, sb, lane, qreg, s0, s1);
+            if (k + 2 < n_my) {              // the slot has been read: tile k + 2 takes it
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+                n_new = ss.put8(par, p.ta + k + 2, lane);
+            }
+        } else {
+            if (k > 0) __syncthreads();
+            sb = sh.ring + (par * NWAVE + w) * G::STAGE;
+            typename S::Dma dn = {};
+            if (k + 1 < n_my) {
+                dn = ss.plan(par ^ 1, p.ta + k + 1);
+                qk_slice<DK, true, S>(ss, dn, sb, lane, qreg, s0, s1);
+            } else {
+                qk_slice<DK, false, S>(ss, dn, sb, lane, qreg, s0, s1);
+            }
+            n_nxt = dn.n;
+        }
+        if (key + WK > p.lim_min && key < p.key1 && p.lim_min < p.key1) {     // some rows see these keys, others do not
+            uint64_t b0, b1;
+            clear_nonfinite<DK>(sb, lane, b0, b1);
+        }
+        float sc[2][4], mx[2];
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+            const int e = min(n_cur, lim[n] - key) - 4 * g;      // keys of this lane's four that the row sees
+            const f32x4 & s = n ? s1 : s0;
+            mx[n] = -INFINITY;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                sc[n][r] = r < e ? s[r] * a.scale_log2 : -INFINITY;
+                mx[n] = fmaxf(mx[n], sc[n][r]);
+            }
+            mx[n] = rows4_max(mx[n]);
+        }
+        half_t * pxv = sh.px[Q8 ? 0 : par];
+        auto put_p = [&]() {
+#pragma unroll
+            for (int n = 0; n < 2; ++n) {
+                half4 ph;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) ph[r] = to_half(exp2_fast(sc[n][r] - m_ref[n]));
+                *reinterpret_cast<half4 *>(&pxv[(16 * n + j16) * C::PROW + WK * w + 4 * g]) = ph;
+            }
+        };
+        put_p();
+        if (lane < 16) {
+            sh.red[par][lane][w] = mx[0];
+            sh.red[par][16 + lane][w] = mx[1];
+        }
+        __syncthreads();
+        bool move = false;
+        float tm[2];
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+            const f32x4 r4 = *reinterpret_cast<const f32x4 *>(&sh.red[par][16 * n + j16][0]);
+            tm[n] = fmaxf(fmaxf(r4[0], r4[1]), fmaxf(r4[2], r4[3]));
+            move |= ref_moves(m_ref[n], tm[n]);
+        }
+        if (__builtin_amdgcn_ballot_w64(move) != 0) {     // rare: move the reference, rescale, redo P
+            float al[2];
+#pragma unroll
+            for (int n = 0; n < 2; ++n) {
+                const bool mv = ref_moves(m_ref[n], tm[n]);
+                al[n] = !mv ? 1.0f : exp2_fast(m_ref[n] - (tm[n] - REF_DROP));      // 0 from M_NONE
+                m_ref[n] = mv ? tm[n] - REF_DROP : m_ref[n];
+            }
+            const float own = al[(lane >> 4) & 1];
+            l_acc *= own;
+            if (k > 0) scale_acc(o, own);
+            put_p();
+            __syncthreads();
+        }
+        pv_tile<DK, DV>(Q8 ? sh.ring + L::TILE : sh.ring, pxv, Q8 ? 0 : par, w, lane, pv, o, l_acc);
+        n_cur = n_nxt;
+        if constexpr (Q8) n_nxt = n_new;
+    }
+    wait_vm<0>();                            // nothing of this wave may still target the ring
+
+    // ---- the end: every wave holds its rows' l and its columns of o ----
+    const int lane_e = opaque_tid() & 63, hl = lane_e & 31, hi4 = 4 * (lane_e >> 5);
+    const float l = halves_sum(l_acc);
+    const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+    if (p.slot < 0 && !a.dst_f16) {
+        const int dr = sh.drow[hl];
+#pragma unroll
+        for (int i = 0; i < C::NTQ; ++i)
+#pragma unroll
+            for (int q4 = 0; q4 < 4; ++q4)
+                out_f32(a, dr, DV, C::DVQ * w + 32 * i + 8 * q4 + hi4,
+                        f32x4{o[i][4 * q4] * inv, o[i][4 * q4 + 1] * inv, o[i][4 * q4 + 2] * inv, o[i][4 * q4 + 3] * inv});
+        return;
+    }
+    if (p.slot >= 0 && w == 0 && lane_e < HG) {
+        const float mr = m_ref[(lane_e >> 4) & 1];
+        reinterpret_cast<f32x2 *>(rec)[lane_e] = f32x2{mr == M_NONE ? -INFINITY : mr, l};
+    }
+    // staging that no other wave reads: this wave's slot of the stage the last tile did not use, or its int8 slot
+    char * stg = Q8 ? sh.ring + w * L::SLOT8 : sh.ring + ((n_my & 1) * NWAVE + w) * G::STAGE;
+    static_assert(!Q8 || HG * C::OPITCH <= L::SLOT8, "the staging fits an int8 slot");
+#pragma unroll
+    for (int i = 0; i < C::NTQ; ++i)
+#pragma unroll
+        for (int q4 = 0; q4 < 4; ++q4) {
+            const half4 hv = {to_half(o[i][4 * q4] * inv), to_half(o[i][4 * q4 + 1] * inv), to_half(o[i][4 * q4 + 2] * inv),
+                              to_half(o[i][4 * q4 + 3] * inv)};
+            *reinterpret_cast<half4 *>(stg + hl * C::OPITCH + (32 * i + 8 * q4 + hi4) * 2) = hv;
+        }
+    rows_out_f16<DV, C::DVQ, C::OPITCH>(a, p, rec, stg, 0, C::DVQ * w, sh.drow, lane_e);
+}
+
+// ---------------------------------------------------------------- up to 128 rows
+// A wave's int8 slice at src -> its f16 slot at dst: per lane, half-blocks (16 values) of one row; rows from n on
+// become zeros
+template <int DK>
+__device__ __forceinline__ void slice_to_f16(const char * src, char * dst, int lane) {
+    using G8 = Q8Geom<DK>;
+    const int row = lane & 15;
+    const char * r = src + row * G8::ROWB;
+#pragma unroll
+    for (int i = 0; i < G8::ITEMS; ++i) {
+        const int hb = (lane >> 4) + 4 * i;                              // half-block
+        const int o = 34 * (hb >> 1) + 2 + 16 * (hb & 1);
+        const uint32_t * q = reinterpret_cast<const uint32_t *>(r + (o & ~3));
+        const half_t d = *reinterpret_cast<const half_t *>(r + 34 * (hb >> 1));
+        const uint32_t sh = (uint32_t)(o & 2);
+        // (the fifth word of an aligned run is the next block's, or past the slot's last row: not used then)
+        const uint32_t x[5] = {q[0], q[1], q[2], q[3], sh ? q[4] : 0u};
+        uint32_t y[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) y[k] = __builtin_amdgcn_alignbyte(x[k + 1], x[k], sh);
+        *reinterpret_cast<half8 *>(dst + slot_byte(row, 2 * hb)) = q8x8_to_f16<0>(y[0], y[1], 0u, d);
+        *reinterpret_cast<half8 *>(dst + slot_byte(row, 2 * hb + 1)) = q8x8_to_f16<0>(y[2], y[3], 0u, d);
+        if (i % 3 == 2) __builtin_amdgcn_sched_barrier(0);               // three half-blocks' loads in flight
+    }
+}
+
+template <int DK, int DV, bool Q8>
+__device__ __forceinline__ void wide_piece(const AttnArgs & a, const Piece & p, PieceLds<DK, DV, Q8> & sh, char * rec) {
+    using G = SliceGeom<DK>;
+    using S = PageStream<DK>;
+    using L = PieceLds<DK, DV, Q8>;
+    constexpr int NB = DV / 32;                         // 32-column o^T tiles per wave
+    constexpr int OPITCH = DV * 2 + 16;
+    static_assert(NWAVE * HG * OPITCH <= L::RING, "the output staging fits the ring");
+    const int tid = opaque_tid(), lane = tid & 63;
+    const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int hl = lane & 31, hi = lane >> 5;
+    const S ss(a, p, w, lds_addr(sh.ring), lane);
+    const bool live_w = HG * w < p.rows;                // a wave without rows only brings in its slices
+    const int n_my = p.tb - p.ta;
+
+    if constexpr (Q8) {
+        const int n0 = ss.template put8<false>(0, p.ta, lane);
+        const int n1 = n_my > 1 ? ss.template put8<false>(1, p.ta + 1, lane) : 0;
+        if (lane == 0) {
+            sh.vc[0][w] = n0;
+            sh.vc[1][w] = n1;
+        }
+    } else {
+        const typename S::Dma d0 = ss.plan(0, p.ta);
+#pragma unroll
+        for (int i = 0; i < G::DMA_N; ++i) ss.template put<false>(d0, i);
+        if (lane == 0) sh.vc[0][w] = d0.n;
+    }
+
+    // ---- q fragments of this wave's rows: qf[st] = row hl, d = 16 st + 8 hi .. + 7 ----
+    half8 qf[DK / 16];
+    const int lim = sh.lim[HG * w + hl];
+    const char * qrow = a.q + (int64_t)p.tok0 * a.q_nb2 + sh.qoff[HG * w + hl];
+    if (a.q_f16) {
+#pragma unroll
+        for (int st = 0; st < DK / 16; ++st) qf[st] = *reinterpret_cast<const half8 *>(qrow + 32 * st + 16 * hi);
+    } else {
+        constexpr int QB = DK / 16 % 6 == 0 ? 6 : 5;    // fragments per batch of loads, a batch ahead of its conversion
+        constexpr int NBT = DK / 16 / QB;
+        static_assert(NBT * QB == DK / 16, "whole batches");
+        f32x4 x[2][QB][2];
+        auto load = [&](int i, f32x4 (&xb)[QB][2]) __attribute__((always_inline)) {
+#pragma unroll
+            for (int b = 0; b < QB; ++b) {
+                xb[b][0] = *reinterpret_cast<const f32x4 *>(qrow + 64 * (QB * i + b) + 32 * hi);
+                xb[b][1] = *reinterpret_cast<const f32x4 *>(qrow + 64 * (QB * i + b) + 32 * hi + 16);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        };
+        load(0, x[0]);
+#pragma unroll
+        for (int i = 0; i < NBT; ++i) {
+            if (i + 1 < NBT) load(i + 1, x[(i + 1) & 1]);
+#pragma unroll
+            for (int b = 0; b < QB; ++b) {
+                const f32x4 (&y)[2] = x[i & 1][b];
+                half8 hq = {to_half(y[0][0]), to_half(y[0][1]), to_half(y[0][2]), to_half(y[0][3]),
+                            to_half(y[1][0]), to_half(y[1][1]), to_half(y[1][2]), to_half(y[1][3])};
+                asm volatile("" : "+v"(hq));            // keep the f16 fragment (not the f32 values) live
+                qf[QB * i + b] = hq;
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    }
+
+    float m_run = M_NONE;                               // row hl, log2 units
+    float l_acc = 0.0f;                                 // row hl, this lane's half of the keys
+    f32x16 o[NB];                                       // o^T tile i: C row = column 32 i + 8 (r / 4) + 4 hi + (r & 3), C col = row hl
+#pragma unroll
+    for (int i = 0; i < NB; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[i][r] = 0.0f;
+    const PairPvAddr pv(lane);
+
+    for (int k = 0; k < n_my; ++k) {
+        const int par = k & 1;
+        const int key_t = p.key0 + (p.ta + k) * TK;
+        char * tile;
+        typename S::Dma dn = {};
+        const bool pf = k + 1 < n_my;
+        if constexpr (Q8) {
+            if (pf) wait_vm<S::N8>();                   // this wave's int8 slice of the tile has landed
+            else wait_vm<0>();
+            if (k > 0) __syncthreads();                 // every wave is past the P.V of tile k - 1
+            tile = sh.ring + L::TILE;
+            slice_to_f16<DK>(sh.ring + (par * NWAVE + w) * L::SLOT8, tile + w * G::STAGE, lane);
+        } else {
+            wait_vm<0>();                               // this wave's slice of the tile has landed
+            tile = sh.ring + par * NWAVE * G::STAGE;
+        }
+        // all keys seen by all rows: no masks; else the rows that do not see a cell take no part of what it holds
+        const bool split = key_t + TK > p.lim_min && p.lim_min < p.key1;
+        if (split) {
+            uint64_t b0, b1;
+            clear_nonfinite<DK>(tile + w * G::STAGE, lane, b0, b1);
+            if (lane == 0) {
+                sh.bad[par][w][0] = b0;
+                sh.bad[par][w][1] = b1;
+            }
+        }
+        __syncthreads();                                // the whole tile is in place; every wave is done with tile k - 1
+        const int4 vc = *reinterpret_cast<const int4 *>(sh.vc[k & 3]);
+        const bool masked = split || key_t + TK > p.key1 || min(min(vc.x, vc.y), min(vc.z, vc.w)) < WK;
+        if constexpr (Q8) {
+            if (k + 2 < n_my) {                         // its int8 slot is free: tile k + 2 takes it
+                const int n = ss.template put8<false>(par, p.ta + k + 2, lane);
+                if (lane == 0) sh.vc[(k + 2) & 3][w] = n;
+            }
+        } else if (pf) {
+            dn = ss.plan(par ^ 1, p.ta + k + 1);
+            if (lane == 0) sh.vc[(k + 1) & 3][w] = dn.n;
+        }
+        if (!live_w) {
+            if constexpr (!Q8) {
+                if (pf) {
+#pragma unroll
+                    for (int i = 0; i < G::DMA_N; ++i) ss.template put<false>(dn, i);
+                }
+            }
+            continue;
+        }
+        half8 abuf[QPF_LANDED];
+        qk_operands<DK>(tile, lane, abuf);
+#pragma unroll 1
+        for (int kp = 0; kp < NWAVE / 2; ++kp) {
+            const char * sb = tile + 2 * kp * G::STAGE;
+            f32x16 s;
+            if (!Q8 && pf) {
+                qk_pair_landed<DK>(sb, lane, qf, abuf, s, [&](int st) {
+                    constexpr int HALF = G::DMA_N / 2;
+                    static_assert(G::DMA_N % 2 == 0 && DK / 16 == 2 * G::DMA_N, "two pairs of slices of row blocks");
+                    if ((st & 3) == 0) ss.template put<false>(dn, HALF * kp + st / 4);
+                });
+            } else {
+                qk_pair_landed<DK>(sb, lane, qf, abuf, s, [](int) {});
+            }
+            constexpr int VPF = 3;
+            half8 vb[VPF];
+#pragma unroll
+            for (int i = 0; i < VPF; ++i) vb[i] = pv.load(sb, i);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[r] *= a.scale_log2;
+            if (masked) {
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    const int sl = 2 * kp + j;
+                    const int n = sl == 0 ? vc.x : sl == 1 ? vc.y : sl == 2 ? vc.z : vc.w;
+                    const int e = min(n, lim - key_t - WK * sl) - 4 * hi;
+                    if (split) {
+                        const uint64_t b0 = sh.bad[par][sl][0], b1 = sh.bad[par][sl][1];
+                        if (__builtin_amdgcn_ballot_w64((b0 | b1) != 0) != 0) {     // a key that holds one has no finite score
+#pragma unroll
+                            for (int i = 0; i < 8; ++i)
+                                if (((((i >> 2) ? b1 : b0) >> (8 * ((i & 3) + 4 * hi))) & 0xff) != 0) s[8 * j + i] = __builtin_nanf("");
+                        }
+                    }
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)                          // key 8 (i >> 2) + (i & 3) + 4 hi of the slice
+                        s[8 * j + i] = 8 * (i >> 2) + (i & 3) < e ? s[8 * j + i] : -INFINITY;
+                }
+            }
+            float mx = -INFINITY;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[r]);
+            if (__builtin_amdgcn_ballot_w64(ref_moves(m_run, mx)) != 0) {
+                // rare: move the reference to the row's max over the pair, rescale
+                float lo, up;
+                halves_pair(mx, lo, up);
+                mx = fmaxf(lo, up);
+                const bool mv = ref_moves(m_run, mx);
+                const bool scale = mv && m_run != M_NONE;
+                const float al = scale ? exp2_fast(m_run - (mx - REF_DROP)) : 1.0f;
+                m_run = mv ? mx - REF_DROP : m_run;
+                if (__builtin_amdgcn_ballot_w64(scale) != 0) {
+                    l_acc *= al;
+                    scale_acc(o, al);
+                }
+            }
+            half8 pt[2];
+            auto put_p = [&](int j, int e0) __attribute__((always_inline)) {
+#pragma unroll
+                for (int e = e0; e < e0 + 4; ++e) pt[j][e] = to_half(exp2_fast(s[8 * j + e] - m_run));
+            };
+            put_p(0, 0);
+            put_p(0, 4);
+#pragma unroll
+            for (int u = 0; u < 2 * NB; ++u) {
+                const half8 va = vb[u % VPF];
+                if (u + VPF < 2 * NB) vb[u % VPF] = pv.load(sb + G::STAGE * ((u + VPF) / NB), (u + VPF) % NB);
+                o[u % NB] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va, pt[u / NB], o[u % NB], 0, 0, 0);
+                if (u == 1) put_p(1, 0);
+                if (u == 3) put_p(1, 4);
+                if (u % NB < 4)
+                    l_acc = __builtin_amdgcn_fdot2(half2{pt[u / NB][2 * (u % NB)], pt[u / NB][2 * (u % NB) + 1]}, ONE2, l_acc, false);
+                if (u == NB + NB / 2 && kp + 1 < NWAVE / 2) qk_operands<DK>(tile + 2 * (kp + 1) * G::STAGE, lane, abuf);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+    }
+    wait_vm<0>();
+    __syncthreads();                                    // the ring becomes the output staging
+    if (!live_w) return;
+    const int lane_e = opaque_tid() & 63, hle = lane_e & 31, hi4 = 4 * (lane_e >> 5);
+    const float l = halves_sum(l_acc);
+    const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+    if (p.slot < 0 && !a.dst_f16) {
+        const int dr = sh.drow[HG * w + hle];
+#pragma unroll
+        for (int i = 0; i < NB; ++i)
+#pragma unroll
+            for (int q4 = 0; q4 < 4; ++q4)
+                out_f32(a, dr, DV, 32 * i + 8 * q4 + hi4,
+                        f32x4{o[i][4 * q4] * inv, o[i][4 * q4 + 1] * inv, o[i][4 * q4 + 2] * inv, o[i][4 * q4 + 3] * inv});
+        return;
+    }
+    if (p.slot >= 0 && lane_e < HG)
+        reinterpret_cast<f32x2 *>(rec)[HG * w + lane_e] = f32x2{m_run == M_NONE ? -INFINITY : m_run, l};
+    char * stg = sh.ring + w * HG * OPITCH;
+#pragma unroll
+    for (int i = 0; i < NB; ++i)
+#pragma unroll
+        for (int q4 = 0; q4 < 4; ++q4) {
+            const half4 hv = {to_half(o[i][4 * q4] * inv), to_half(o[i][4 * q4 + 1] * inv), to_half(o[i][4 * q4 + 2] * inv),
+                              to_half(o[i][4 * q4 + 3] * inv)};
+            *reinterpret_cast<half4 *>(stg + hle * OPITCH + (32 * i + 8 * q4 + hi4) * 2) = hv;
+        }
+    rows_out_f16<DV, DV, OPITCH>(a, p, rec, stg, HG * w, 0, sh.drow, lane_e);
+}
+
+}  // namespace paged
+}  // namespace mla
