@@ -28,8 +28,10 @@ namespace paged {
 namespace {
 
 constexpr int N_WG = 256;                   // one workgroup per CU
-constexpr double OVERHEAD = 1.0;            // a group's start and end, in tiles
 constexpr int MIN_SHARED_TILES = 1;         // fewer shared tiles than this are left to the requests
+// costs, in tenths of a wide tile (all of them times H, so that they are whole numbers)
+constexpr int WIDE_TILE = 10, NARROW_TILE = 7;
+constexpr int WIDE_START = 20, NARROW_START = 12;   // a piece's rows in, its results out
 
 // Workspace: a header, the pieces of every shared block and of every row, the records
 struct Head { int rows, shared_rows; };
@@ -55,77 +57,137 @@ struct Walk {
                                             // token, its number
     __device__ __forceinline__ double edge(int i) const { return i >= n_wg ? all : all * (double)i / (double)n_wg; }
     __device__ __forceinline__ int shared_blocks() const { return (shared_rows + BLOCK_ROWS - 1) / BLOCK_ROWS; }
-    __device__ __forceinline__ double shared_a(int n_head) const { return (double)n_head * ((double)(shared_keys / TK) + OVERHEAD); }
+    __device__ __forceinline__ double shared_a(int n_head) const { return (double)(n_head * WIDE_START) + (double)n_head * (double)(WIDE_TILE * (shared_keys / TK)); }
 };
 
-// request b's place: its tokens, what they see, its blocks and their costs in tiles / H (the j-th: a + 2 (j + 1), as
+// request b's place: its tokens, what they see, its blocks and their costs (the j-th: a + 2 WIDE_TILE (j + 1), as
 // 128 rows on are 128 / H tokens, 2 / H tiles)
 struct Request {
-    int n, past, key0, blocks;
+    int n, past, key0, blocks, first;
+    bool wide;
     double a;
-    __device__ __forceinline__ Request(const AttnArgs & ar, const Walk & wk, int b, int start) {
-        n = min(min(max(ar.n_new[b], 0), ar.nt), ar.nt - start);
-        past = min(clamp_past(ar.past[b]), wk.cap);
+    __device__ __forceinline__ Request(const AttnArgs & ar, const Walk & wk, int n_new, int past_, int b, int start) {
+        n = min(min(max(n_new, 0), ar.nt), ar.nt - start);
+        past = min(clamp_past(past_), wk.cap);
         key0 = b < wk.n_share ? wk.shared_keys : 0;
         blocks = (n * ar.n_head + BLOCK_ROWS - 1) / BLOCK_ROWS;
-        const int first = (min(past + 1, wk.cap) - key0 + TK - 1) / TK;
-        a = (double)ar.n_head * ((double)max(first, 1) + OVERHEAD);
+        wide = n * ar.n_head > HG;
+        first = max((min(past + 1, wk.cap) - key0 + TK - 1) / TK, 1);
+        a = (double)(ar.n_head * start_cost()) + (double)ar.n_head * (double)((wide ? WIDE_TILE : NARROW_TILE) * first);
     }
-    __device__ __forceinline__ double upto(int j) const { return (double)j * a + (double)j * ((double)j + 1.0); }
+    __device__ __forceinline__ Request(const AttnArgs & ar, const Walk & wk, int b, int start)
+        : Request(ar, wk, ar.n_new[b], ar.past[b], b, start) {}
+    __device__ __forceinline__ int start_cost() const { return wide ? WIDE_START : NARROW_START; }
+    __device__ __forceinline__ double upto(int j) const { return (double)j * a + (double)WIDE_TILE * ((double)j * ((double)j + 1.0)); }
     __device__ __forceinline__ double cost() const { return upto(blocks); }
 };
 
-// This workgroup's stretch and its first group, from the lengths.  `mem`: MAX_SEQS * 16 bytes of LDS; red: 64 bytes.
-__device__ __forceinline__ Walk find_place(const AttnArgs & a, char * mem, int * red) {
-    double * cum = reinterpret_cast<double *>(mem);                     // cost before request b
-    int * start = reinterpret_cast<int *>(mem) + 2 * MAX_SEQS;          // its first row
-    int * grp = start + MAX_SEQS;                                       // blocks before it
-    double * red_d = reinterpret_cast<double *>(red) + 4;
-    const int tid = threadIdx.x, lane = tid & 63, H = a.n_head, wg = blockIdx.x;
+// This workgroup's stretch and its first group (b = n_seq: none), from the lengths: two sums over the requests by the
+// whole workgroup, then the thread whose request holds the stretch's start says so.
+struct PlaceLds {
+    int rows[4], shared[4][4];              // per wavefront: rows; sharing requests' cells, number, rows, first
+    double cost[4];
+    uint64_t groups[4];
+    double base;
+    int b, tok0, g;
+};
+__device__ __forceinline__ Walk find_place(const AttnArgs & a, PlaceLds & sh) {
+    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, H = a.n_head, wg = blockIdx.x;
+    const int per = (a.n_seq + NTHR - 1) / NTHR, b0 = min(tid * per, a.n_seq), b1 = min(b0 + per, a.n_seq);
+    const int n_pre = a.prefix != nullptr ? min(max(a.prefix[1], 0), a.n_seq) : 0;
+    const int k_pre = a.prefix != nullptr ? a.prefix[0] : 0;
     Walk k;
     k.cap = a.max_pages << a.page_shift;
-    k.total = uni(min(block_scan<NTHR>(a.n_seq, [&](int b) { return min(max(a.n_new[b], 0), a.nt); }, start, red), a.nt));
+    // the first of this thread's requests stays in registers: up to 256 requests it is the only one
+    const int n0 = b0 < b1 ? a.n_new[b0] : 0, past0 = b0 < b1 ? a.past[b0] : 0;
+    auto n_of = [&](int b) { return b == b0 ? n0 : a.n_new[b]; };
+    auto past_of = [&](int b) { return b == b0 ? past0 : a.past[b]; };
+
+    int own = 0, keys = min(max(k_pre, 0), k.cap), active = 0, srows = 0, by = MAX_SEQS;
+    for (int b = b0; b < b1; ++b) {
+        const int n = min(max(n_of(b), 0), a.nt);
+        own += n;
+        if (b < n_pre && n > 0) {
+            keys = min(keys, clamp_past(past_of(b)));
+            by = min(by, b);
+            srows += n;
+            ++active;
+        }
+    }
+    const int incl = wave_scan(own);
+    if (lane == 63) sh.rows[w] = incl;
+    if (a.prefix != nullptr) {
+        keys = wave_min(keys);
+        by = wave_min(by);
+        active = wave_scan(active);
+        srows = wave_scan(srows);
+        if (lane == 63) {
+            sh.shared[w][0] = keys;
+            sh.shared[w][1] = active;
+            sh.shared[w][2] = srows;
+            sh.shared[w][3] = by;
+        }
+    }
+    if (tid == 0) sh.b = a.n_seq;
+    __syncthreads();
+    int start = incl - own, total = 0;      // rows before this thread's requests
+#pragma unroll
+    for (int i = 0; i < NTHR / 64; ++i) {
+        start += i < w ? sh.rows[i] : 0;
+        total += sh.rows[i];
+    }
+    k.total = uni(min(total, a.nt));
     k.n_share = k.shared_keys = k.shared_rows = k.shared_by = 0;
     if (a.prefix != nullptr) {
         // as many whole tiles of shared cells as all sharing requests with tokens held before them
-        const int n = min(max(a.prefix[1], 0), a.n_seq);
-        int keys = min(max(a.prefix[0], 0), k.cap), active = 0, by = MAX_SEQS;
-        for (int b = tid; b < n; b += NTHR)
-            if (a.n_new[b] > 0) {
-                keys = min(keys, clamp_past(a.past[b]));
-                by = min(by, b);
-                ++active;
-            }
-#pragma unroll
-        for (int i = 1; i < 64; i <<= 1) {
-            keys = min(keys, __shfl_xor(keys, i));
-            by = min(by, __shfl_xor(by, i));
-            active += __shfl_xor(active, i);
-        }
-        if (lane == 0) {
-            red[tid >> 6] = keys;
-            red[4 + (tid >> 6)] = active;
-            red[8 + (tid >> 6)] = by;
-        }
-        __syncthreads();
-        keys = uni(min(min(red[0], red[1]), min(red[2], red[3])) / TK * TK);
-        active = uni(red[4] + red[5] + red[6] + red[7]);
-        k.shared_by = uni(min(min(red[8], red[9]), min(red[10], red[11])));
-        __syncthreads();
+        keys = uni(min(min(sh.shared[0][0], sh.shared[1][0]), min(sh.shared[2][0], sh.shared[3][0])) / TK * TK);
+        active = uni(sh.shared[0][1] + sh.shared[1][1] + sh.shared[2][1] + sh.shared[3][1]);
         if (active > 1 && keys >= MIN_SHARED_TILES * TK) {
-            k.n_share = uni(n);
+            k.n_share = n_pre;
             k.shared_keys = keys;
-            k.shared_rows = uni((n < a.n_seq ? min(start[n], a.nt) : k.total) * H);
+            k.shared_rows = uni(min(sh.shared[0][2] + sh.shared[1][2] + sh.shared[2][2] + sh.shared[3][2], a.nt) * H);
+            k.shared_by = uni(min(min(sh.shared[0][3], sh.shared[1][3]), min(sh.shared[2][3], sh.shared[3][3])));
         }
     }
     const double shared_a = k.shared_a(H), shared_cost = (double)k.shared_blocks() * shared_a;
-    const int n_own = block_scan<NTHR>(a.n_seq, [&](int b) { return Request(a, k, b, min(start[b], a.nt)).blocks; }, grp, red);
-    k.all = shared_cost + block_scan<NTHR>(a.n_seq, [&](int b) { return Request(a, k, b, min(start[b], a.nt)).cost(); }, cum, red_d);
+
+    // costs, and (tiles, groups) in the high and low half of a word
+    double cost = 0.0;
+    uint64_t groups = 0;
+    {
+        int at = min(start, a.nt);
+        for (int b = b0; b < b1; ++b) {
+            const Request rq(a, k, n_of(b), past_of(b), b, at);
+            cost += rq.cost();
+            groups += (uint64_t)rq.blocks + ((uint64_t)(uint32_t)(rq.blocks * rq.first) << 32);
+            at += rq.n;
+        }
+    }
+    const double cost_incl = wave_scan(cost);
+    const uint64_t groups_incl = wave_scan(groups);
+    if (lane == 63) {
+        sh.cost[w] = cost_incl;
+        sh.groups[w] = groups_incl;
+    }
+    __syncthreads();
+    double base = cost_incl - cost;
+    uint64_t grp = groups_incl - groups, all_groups = 0;
+    k.all = 0.0;
+#pragma unroll
+    for (int i = 0; i < NTHR / 64; ++i) {
+        base += i < w ? sh.cost[i] : 0.0;
+        grp += i < w ? sh.groups[i] : 0;
+        k.all += sh.cost[i];
+        all_groups += sh.groups[i];
+    }
+    base += shared_cost;
+    k.all += shared_cost;
     // at most one workgroup per tile
-    const double tiles = k.all / (double)H - OVERHEAD * (double)(k.shared_blocks() + n_own);
-    k.n_wg = uni(min(max((int)min(tiles, 65535.0), 1), (int)gridDim.x));
+    const int64_t tiles = (int64_t)(all_groups >> 32) + (int64_t)k.shared_blocks() * (k.shared_keys / TK);
+    k.n_wg = uni((int)min(max(tiles, (int64_t)1), (int64_t)gridDim.x));
     k.x0 = k.edge(wg);
     k.x1 = k.edge(wg + 1);
+    k.b = a.n_seq;
     if (wg >= k.n_wg || k.total == 0) return k;
 
     if (uni(k.x0 < shared_cost)) {
@@ -135,17 +197,35 @@ __device__ __forceinline__ Walk find_place(const AttnArgs & a, char * mem, int *
         k.b = -1;
         k.base = 0.0;
         k.tok0 = 0;
-        k.j = k.g = j;
-    } else {
-        int b = last_at_most(cum, a.n_seq, k.x0 - shared_cost);
-        // requests without tokens take no place: the last request that begins here is one with tokens, unless only
-        // such ones follow
-        while (b > 0 && Request(a, k, b, min(start[b], a.nt)).blocks == 0) --b;
-        k.b = b;
-        k.base = shared_cost + cum[b];
-        k.tok0 = min(start[b], a.nt);
-        const Request rq(a, k, b, k.tok0);
-        int lo = 0, len = rq.blocks;
+        k.j = k.g = uni(j);
+        return k;
+    }
+    if (base <= k.x0 && k.x0 < base + cost) {
+        int at = min(start, a.nt), g = (int)(uint32_t)grp;
+        for (int b = b0; b < b1; ++b) {
+            const Request rq(a, k, n_of(b), past_of(b), b, at);
+            const double c = rq.cost();
+            if (rq.blocks > 0 && (k.x0 < base + c || b + 1 == b1)) {
+                sh.b = b;
+                sh.tok0 = at;
+                sh.g = g;
+                sh.base = base;
+                break;
+            }
+            base += c;
+            g += rq.blocks;
+            at += rq.n;
+        }
+    }
+    __syncthreads();
+    k.b = uni(sh.b);
+    if (k.b >= a.n_seq) return k;
+    k.tok0 = uni(sh.tok0);
+    k.base = sh.base;
+    int lo = 0;
+    {
+        const Request rq(a, k, k.b, k.tok0);
+        int len = rq.blocks;
         while (len > 1) {
             const int half = len >> 1;
             if (k.base + rq.upto(lo + half) <= k.x0) {
@@ -155,9 +235,9 @@ __device__ __forceinline__ Walk find_place(const AttnArgs & a, char * mem, int *
                 len = half;
             }
         }
-        k.j = lo;
-        k.g = k.shared_blocks() + grp[b] + lo;
     }
+    k.j = uni(lo);
+    k.g = uni(k.shared_blocks() + sh.g + lo);
     return k;
 }
 
@@ -165,22 +245,18 @@ template <int DK, int DV, bool Q8>
 struct KernelLds {
     PieceLds<DK, DV, Q8> piece;
     Walk walk;
+    PlaceLds place;
 };
 
 template <int DK, int DV, bool Q8>
 __global__ __launch_bounds__(NTHR, 1) void kqkv_paged_kernel(AttnArgs a) {
     using L = PieceLds<DK, DV, Q8>;
     __shared__ KernelLds<DK, DV, Q8> lds;
-    static_assert(MAX_SEQS * 16 <= L::RING, "the prefix sums fit the ring");
     L & sh = lds.piece;
     const int tid = threadIdx.x, wg = blockIdx.x;
-    {
-        const Walk k = find_place(a, sh.ring, reinterpret_cast<int *>(sh.qoff));
-        if (wg == 0 && tid == 0) *reinterpret_cast<Head *>(a.work) = Head{k.total * a.n_head, k.shared_rows};
-        if (wg >= k.n_wg || k.total == 0) return;
-        if (tid == 0) lds.walk = k;
-        __syncthreads();
-    }
+    Walk k = find_place(a, lds.place);
+    if (wg == 0 && tid == 0) *reinterpret_cast<Head *>(a.work) = Head{k.total * a.n_head, k.shared_rows};
+    if (k.b >= a.n_seq) return;              // no part of the line
     for (;;) {
         // ---- the group: its rows, keys, tiles and stretch of the line; the place of the next one ----
         Piece p;
@@ -188,15 +264,14 @@ __global__ __launch_bounds__(NTHR, 1) void kqkv_paged_kernel(AttnArgs a) {
         int pieces = 0, j, b;
         Walk next;
         {
-            const Walk k = lds.walk;
             const int H = a.n_head;
             b = uni(k.b);
             j = uni(k.j);
             p.tok0 = uni(k.tok0);
             p.row0 = j * BLOCK_ROWS;
-            double g0, g1;
+            double g0, g1, body;             // its stretch, and where its tiles begin on it
             int n_tiles, blocks, n = 0;
-            double cost = 0.0;
+            double cost;
             bool direct = false;
             if (b < 0) {
                 p.rows = uni(min(BLOCK_ROWS, k.shared_rows - p.row0));
@@ -208,6 +283,7 @@ __global__ __launch_bounds__(NTHR, 1) void kqkv_paged_kernel(AttnArgs a) {
                 const double sa = k.shared_a(H);
                 g0 = (double)j * sa;
                 g1 = (double)(j + 1) * sa;
+                body = g0 + (double)(H * WIDE_START);
                 cost = (double)blocks * sa;
             } else {
                 const Request rq(a, k, b, p.tok0);
@@ -223,10 +299,11 @@ __global__ __launch_bounds__(NTHR, 1) void kqkv_paged_kernel(AttnArgs a) {
                 n_tiles = max(1, (p.key1 - p.key0 + TK - 1) / TK);
                 g0 = k.base + rq.upto(j);
                 g1 = k.base + rq.upto(j + 1);
+                body = g0 + (double)(H * rq.start_cost());
                 direct = uni(b >= k.n_share && g0 >= k.x0 && g1 <= k.x1);
             }
             auto tile_at = [&](double x) {
-                return x <= g0 ? 0 : x >= g1 ? n_tiles : min(n_tiles, (int)((x - g0) / (g1 - g0) * (double)n_tiles + 0.5));
+                return x <= body ? 0 : x >= g1 ? n_tiles : min(n_tiles, (int)((x - body) / (g1 - body) * (double)n_tiles + 0.5));
             };
             p.ta = uni(tile_at(k.x0));
             p.tb = uni(tile_at(k.x1));
@@ -242,17 +319,16 @@ __global__ __launch_bounds__(NTHR, 1) void kqkv_paged_kernel(AttnArgs a) {
             next = k;
             next.j = j + 1;
             next.g = k.g + 1;
-            if (uni(next.j >= blocks)) {                 // the next request with tokens
+            if (!last && uni(next.j >= blocks)) {        // the next request with tokens
                 next.base = k.base + cost;
                 next.tok0 = p.tok0 + n;
                 next.j = 0;
                 next.b = b + 1;
                 while (next.b < a.n_seq && Request(a, k, next.b, next.tok0).blocks == 0) ++next.b;
-                last = last || uni(next.b >= a.n_seq);
+                last = uni(next.b >= a.n_seq);
             }
         }
-        __syncthreads();                     // the last piece's rows and ring, and the place, have been read
-        if (tid == 0) lds.walk = next;
+        if (!last && tid == 0) lds.walk = next;
         piece_rows(a, p, sh.qoff, sh.drow, sh.lim);
         if (first) {
             if (b < 0) {
@@ -266,49 +342,59 @@ __global__ __launch_bounds__(NTHR, 1) void kqkv_paged_kernel(AttnArgs a) {
         __syncthreads();
         if (p.ta >= p.tb) {                  // no tile of the group falls to this workgroup (never where direct)
             if (tid < BLOCK_ROWS) reinterpret_cast<f32x2 *>(rec)[tid] = f32x2{-INFINITY, 0.0f};
-        } else if (p.rows <= HG && p.row0 == 0) {
+        } else if (p.rows <= HG) {
             narrow_piece<DK, DV, Q8>(a, p, sh, rec);
         } else {
             wide_piece<DK, DV, Q8>(a, p, sh, rec);
         }
         if (last) return;
+        k = lds.walk;
+        __syncthreads();                     // the piece's rows and ring, and the place, have been read
     }
 }
 
 // ---------------------------------------------------------------- the merge
-// A workgroup per row (and per DV / CB columns of it): its pieces, those of the row's own group and of its shared
-// block.  LP lanes hold a piece's columns, eight each; 256 / LP pieces at a time.
-template <int DV, int CB>
-__global__ __launch_bounds__(NTHR) void kqkv_paged_merge_kernel(AttnArgs a) {
-    constexpr int LP = DV / CB / 8, PP = NTHR / LP, U = 4;
-    __shared__ float sm[PP], sl[PP];
-    __shared__ f32x4 so[2][NTHR];
-    const int tid = threadIdx.x, c = tid % LP, pi = tid / LP;
-    const int col = (int)blockIdx.y * (DV / CB) + 8 * c;
-    const Head head = *reinterpret_cast<const Head *>(a.work);
-    const Pieces * shared_at = reinterpret_cast<const Pieces *>(a.work + shared_off());
-    const Pieces * own_at = reinterpret_cast<const Pieces *>(a.work + own_off(a.n_head, a.nt));
-    const char * records = a.work + records_off(a.n_head, a.nt);
-    for (int row = blockIdx.x; row < head.rows; row += gridDim.x) {
-        const Pieces own = own_at[row];
-        const int n_own = (int)(own.n_row & 0xffffu), r_own = (int)(own.n_row >> 16);
-        if (n_own == 0) continue;                        // complete already
-        Pieces shd = {0, 0};
-        if (row < head.shared_rows) shd = shared_at[row / BLOCK_ROWS];
-        const int n = n_own + (int)shd.n_row, r_shd = row % BLOCK_ROWS;
-        float m = -INFINITY, l = 0.0f, o[8] = {};
-        for (int q0 = pi; q0 < n; q0 += PP * U) {
+// The pieces of a row: those of its own group, then those of its shared block
+struct RowPieces {
+    int n, n_own, own, shared, r_own, r_shared;
+    __device__ __forceinline__ RowPieces(const AttnArgs & a, const Head & head, int row) {
+        // (both read at once, whatever the row: the shared block's entry lies in the workspace also where there is none)
+        const Pieces o = reinterpret_cast<const Pieces *>(a.work + own_off(a.n_head, a.nt))[row];
+        const Pieces s = reinterpret_cast<const Pieces *>(a.work + shared_off())[row / BLOCK_ROWS];
+        n_own = row < head.rows ? (int)(o.n_row & 0xffffu) : 0;
+        r_own = (int)(o.n_row >> 16);
+        own = o.slot;
+        shared = s.slot;
+        r_shared = row % BLOCK_ROWS;
+        // a row that is complete has none at all: it shares nothing
+        n = n_own + (n_own > 0 && row < head.shared_rows ? (int)s.n_row : 0);
+    }
+    // row q's record and its row of it
+    template <int DV>
+    __device__ __forceinline__ const char * at(const char * records, int q, int & r) const {
+        const bool mine = q < n_own;
+        r = mine ? r_own : r_shared;
+        return records + (size_t)(mine ? own + q : shared + q - n_own) * record_bytes<DV>();
+    }
+};
+
+// (m, l, o) of some pieces, eight columns per lane
+struct Part {
+    float m = -INFINITY, l = 0.0f, o[8] = {};
+    // pieces q0, q0 + step, .. below n
+    template <int DV, int U>
+    __device__ __forceinline__ void add(const RowPieces & rp, const char * records, int q0, int step, int col) {
+        for (; q0 < rp.n; q0 += step * U) {
             float ms[U], ls[U];
             half8 os[U];
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                const int q = min(q0 + PP * u, n - 1);
-                const bool mine = q < n_own;
-                const char * rec = records + (size_t)(mine ? own.slot + q : shd.slot + q - n_own) * record_bytes<DV>();
-                const int r = mine ? r_own : r_shd;
+                const int q = q0 + step * u;
+                int r;
+                const char * rec = rp.at<DV>(records, min(q, rp.n - 1), r);
                 const f32x2 ml = reinterpret_cast<const f32x2 *>(rec)[r];
-                ms[u] = q0 + PP * u < n ? ml[0] : -INFINITY;
-                ls[u] = q0 + PP * u < n ? ml[1] : 0.0f;
+                ms[u] = q < rp.n ? ml[0] : -INFINITY;
+                ls[u] = q < rp.n ? ml[1] : 0.0f;
                 os[u] = *reinterpret_cast<const half8 *>(rec + BLOCK_ROWS * 8 + ((size_t)r * DV + col) * 2);
             }
             float mx = m;
@@ -320,51 +406,136 @@ __global__ __launch_bounds__(NTHR) void kqkv_paged_merge_kernel(AttnArgs a) {
             for (int k = 0; k < 8; ++k) o[k] *= f0;
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                const float f = ls[u] * exp2_unless(ms[u] == -INFINITY, ms[u] - mx);     // a NaN l (no finite score) stays one
+                // without a finite score l is 0, or NaN where every score was; o then holds nothing (an empty piece's
+                // was never written)
+                const bool none = ms[u] == -INFINITY;
+                const float f = none ? ls[u] : ls[u] * exp2_fast(ms[u] - mx);
                 l += f;
 #pragma unroll
-                for (int k = 0; k < 8; ++k) o[k] += ms[u] == -INFINITY ? f : f * (float)os[u][k];   // an empty piece has no o
+                for (int k = 0; k < 8; ++k) o[k] += none ? f : f * (float)os[u][k];
             }
             m = mx;
         }
-        __syncthreads();                                 // the row before has been read
-        if (c == 0) {
-            sm[pi] = m;
-            sl[pi] = l;
+    }
+    __device__ __forceinline__ void add(float m2, float l2, const float (&o2)[8]) {
+        const float mx = fmaxf(m, m2);
+        // (without a finite score: l and o are 0 or NaN)
+        const float f = m == -INFINITY ? 1.0f : exp2_fast(m - mx), f2 = m2 == -INFINITY ? 1.0f : exp2_fast(m2 - mx);
+        l = l * f + l2 * f2;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) o[k] = o[k] * f + o2[k] * f2;
+        m = mx;
+    }
+    template <int DV>
+    __device__ __forceinline__ void out(const AttnArgs & a, int row, int col) const {
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        const int t = row / a.n_head, h = row - t * a.n_head;
+        const size_t at = ((size_t)h * a.nt + t) * DV + col;
+        if (a.dst_f16) {
+            half8 v;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) v[k] = to_half(o[k] * inv);
+            *reinterpret_cast<half8 *>(a.dst + at * 2) = v;
+        } else {
+            f32x4 v[2];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) v[k >> 2][k & 3] = o[k] * inv;
+            *reinterpret_cast<f32x4 *>(a.dst + at * 4) = v[0];
+            *reinterpret_cast<f32x4 *>(a.dst + at * 4 + 16) = v[1];
         }
-        so[0][tid] = f32x4{o[0], o[1], o[2], o[3]};
-        so[1][tid] = f32x4{o[4], o[5], o[6], o[7]};
-        __syncthreads();
-        if (pi == 0) {
-            float M = -INFINITY, Ls = 0.0f;
-            f32x4 r0 = {0.f, 0.f, 0.f, 0.f}, r1 = {0.f, 0.f, 0.f, 0.f};
+    }
+};
+
+// One row by a workgroup: DV / CB columns from c0 on, LP lanes a piece, 256 / LP pieces at a time
+template <int DV, int CB>
+struct RowLds {
+    static constexpr int LP = DV / CB / 8, PP = NTHR / LP;
+    float m[PP], l[PP];
+    f32x4 o[2][NTHR];
+};
+template <int DV, int CB>
+__device__ __forceinline__ void merge_by_workgroup(const AttnArgs & a, const RowPieces & rp, const char * records, int row, int c0,
+                                                   RowLds<DV, CB> & sh) {
+    using R = RowLds<DV, CB>;
+    const int tid = threadIdx.x, c = tid % R::LP, pi = tid / R::LP;
+    Part p;
+    p.template add<DV, 4>(rp, records, pi, R::PP, c0 + 8 * c);
+    if (c == 0) {
+        sh.m[pi] = p.m;
+        sh.l[pi] = p.l;
+    }
+    sh.o[0][tid] = f32x4{p.o[0], p.o[1], p.o[2], p.o[3]};
+    sh.o[1][tid] = f32x4{p.o[4], p.o[5], p.o[6], p.o[7]};
+    __syncthreads();
+    if (pi == 0) {
+        for (int i = 1; i < R::PP; ++i) {
+            const f32x4 x = sh.o[0][i * R::LP + c], y = sh.o[1][i * R::LP + c];
+            const float o2[8] = {x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
+            p.add(sh.m[i], sh.l[i], o2);
+        }
+        p.template out<DV>(a, row, c0 + 8 * c);
+    }
+}
+
+// Few rows: a workgroup per row and DV / CB columns, so that the whole card takes part
+template <int DV, int CB>
+__global__ __launch_bounds__(NTHR) void kqkv_paged_merge_few_kernel(AttnArgs a) {
+    __shared__ RowLds<DV, CB> sh;
+    const Head head = *reinterpret_cast<const Head *>(a.work);
+    const RowPieces rp(a, head, blockIdx.x);
+    if (rp.n == 0) return;
+    merge_by_workgroup<DV, CB>(a, rp, a.work + records_off(a.n_head, a.nt), blockIdx.x, DV / CB * (int)blockIdx.y, sh);
+}
+
+// Many rows: a wavefront per row (D_v 256: half of one per piece, two pieces at a time), four rows a workgroup; a row
+// of many pieces (a long request among short ones) by the whole workgroup
+constexpr int MANY_PIECES = 24;
+template <int DV>
+__global__ __launch_bounds__(NTHR) void kqkv_paged_merge_kernel(AttnArgs a) {
+    constexpr int LP = DV / 8, PW = 64 / LP;
+    __shared__ RowLds<DV, 1> sh;
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    const Head head = *reinterpret_cast<const Head *>(a.work);
+    const char * records = a.work + records_off(a.n_head, a.nt);
+    const int n_rows = a.n_head * a.nt;
+    for (int row0 = 4 * (int)blockIdx.x; row0 < head.rows; row0 += 4 * (int)gridDim.x) {
+        const int row = min(row0 + w, n_rows - 1);
+        const RowPieces rp(a, head, row);
+        const bool mine = row0 + w < head.rows;
+        if (lane == 0) sh.l[w] = mine ? (float)rp.n : 0.0f;
+        if (mine && rp.n > 0 && rp.n <= MANY_PIECES) {
+            const int col = 8 * (lane % LP);
+            Part p;
+            p.template add<DV, 4>(rp, records, lane / LP, PW, col);
+            if constexpr (PW == 2) {
+                Part q;                                  // the other half's
+                float lo, up;
+                halves_pair(p.m, lo, up);
+                q.m = up;
+                p.m = lo;
+                halves_pair(p.l, lo, up);
+                q.l = up;
+                p.l = lo;
 #pragma unroll
-            for (int i = 0; i < PP; ++i) M = fmaxf(M, sm[i]);
-#pragma unroll
-            for (int i = 0; i < PP; ++i) {
-                const float f = exp2_unless(sm[i] == -INFINITY, sm[i] - M);
-                const float e = sm[i] == -INFINITY ? sl[i] : 0.0f;       // 0, or NaN
-                Ls += sl[i] * f + e;
-                r0 += so[0][i * LP + c] * f + e;
-                r1 += so[1][i * LP + c] * f + e;
-            }
-            const float inv = Ls == 0.0f ? 0.0f : 1.0f / Ls;
-            r0 *= inv;
-            r1 *= inv;
-            const int t = row / a.n_head, h = row - t * a.n_head;
-            const size_t at = ((size_t)h * a.nt + t) * DV + col;
-            if (a.dst_f16) {
-                half8 v;
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    v[k] = to_half(r0[k]);
-                    v[4 + k] = to_half(r1[k]);
+                for (int k = 0; k < 8; ++k) {
+                    halves_pair(p.o[k], lo, up);
+                    q.o[k] = up;
+                    p.o[k] = lo;
                 }
-                *reinterpret_cast<half8 *>(a.dst + at * 2) = v;
-            } else {
-                *reinterpret_cast<f32x4 *>(a.dst + at * 4) = r0;
-                *reinterpret_cast<f32x4 *>(a.dst + at * 4 + 16) = r1;
+                p.add(q.m, q.l, q.o);
             }
+            if (lane < LP) p.template out<DV>(a, row, col);
+        }
+        __syncthreads();
+        float n[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) n[i] = sh.l[i];
+        __syncthreads();
+#pragma unroll 1
+        for (int i = 0; i < 4; ++i) {
+            if (n[i] <= (float)MANY_PIECES) continue;
+            merge_by_workgroup<DV, 1>(a, RowPieces(a, head, row0 + i), records, row0 + i, 0, sh);
+            __syncthreads();
         }
     }
 }
@@ -386,8 +557,9 @@ static hipError_t launch(bool q8, const AttnArgs & a, hipStream_t stream) {
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     const int rows = a.n_head * a.nt;
-    if (rows <= 512) hipLaunchKernelGGL((kqkv_paged_merge_kernel<DV, DV / 64>), dim3(rows, DV / 64), dim3(NTHR), 0, stream, a);
-    else hipLaunchKernelGGL((kqkv_paged_merge_kernel<DV, 1>), dim3(rows < 4096 ? rows : 4096), dim3(NTHR), 0, stream, a);
+    if (rows <= 512) hipLaunchKernelGGL((kqkv_paged_merge_few_kernel<DV, DV / 64>), dim3(rows, DV / 64), dim3(NTHR), 0, stream, a);
+    else if (rows <= 1536) hipLaunchKernelGGL((kqkv_paged_merge_few_kernel<DV, 1>), dim3(rows), dim3(NTHR), 0, stream, a);
+    else hipLaunchKernelGGL(kqkv_paged_merge_kernel<DV>, dim3(rows < 4 * 2048 ? (rows + 3) / 4 : 2048), dim3(NTHR), 0, stream, a);
     return hipGetLastError();
 }
 

@@ -120,10 +120,10 @@ struct PageStream {
         cell = ((int64_t)id << shift) + (key & ((1 << shift) - 1));
         return min(WK, key1 - key);
     }
-    __device__ __forceinline__ Dma plan(int s, int k) const {
+    __device__ __forceinline__ Dma plan(int s, int k, bool there = true) const {
         Dma d;
-        int64_t cell;
-        d.n = slice(k, cell);
+        int64_t cell = 0;
+        d.n = there ? slice(k, cell) : 0;
         d.krs = make_rsrc(kc + cell * kc_nb1, d.n > 0 ? (uint32_t)((int64_t)(d.n - 1) * kc_nb1 + DK * 2) : 0u);
         d.sb = ring_lds + (uint32_t)((s * NWAVE + w) * G::STAGE);
         return d;
@@ -213,26 +213,29 @@ __device__ __forceinline__ void scale_acc(f32x16 (&o)[N], float f) {
 }
 
 // ---------------------------------------------------------------- up to 32 rows
-// (of one block, row0 = 0: at most 32 tokens and heads, so the rows' q lie within 2 GiB of the first, MAX_STRIDE)
+// LDS DMA from a 64-bit address per lane (16 bytes; lane l's land at lds_base + 16 l), for rows of q, whose strides have
+// no bound
+__device__ __forceinline__ void row_dma16(const char * at, uint32_t lds_base) {
+    asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, off" :: "v"(at), "{m0}"(lds_base) : "memory");
+}
+
 // q of the 32 rows into LDS at qs (f32: q_convert's layout; f16: two slices of 16 rows, as K rows lie), this wave's
-// share; QN instructions
-constexpr uint32_t NO_ROW = 0x80000000u;    // an offset past the resource's records: reads zeros
+// share.  Rows that are not there bring in the first row again; nothing of theirs is used.
 template <int DK, bool F16>
 __device__ __forceinline__ void q_rows_dma(const AttnArgs & a, const Piece & p, const int64_t * qoff, uint32_t qs, int w, int lane) {
     using G = SliceGeom<DK>;
-    const i32x4 rs = make_rsrc(a.q + (int64_t)p.tok0 * a.q_nb2, NO_ROW);
+    const char * base = a.q + (int64_t)p.tok0 * a.q_nb2;
     if constexpr (F16) {
-        const int r0 = 2 * (lane >> 4) + ((lane >> 3) & 1), row = 8 * w + r0;
-        const uint32_t vo = row < p.rows ? (uint32_t)qoff[row] + 16u * (uint32_t)((lane & 7) ^ row_sw(r0)) : NO_ROW;
+        const int r0 = 2 * (lane >> 4) + ((lane >> 3) & 1);
+        const char * at = base + qoff[8 * w + r0] + 16 * ((lane & 7) ^ row_sw(r0));
 #pragma unroll
-        for (int i = 0; i < G::DMA_N / 2; ++i)
-            page_dma16<false>(rs, vo, 128u * (uint32_t)i, qs + (uint32_t)((w >> 1) * G::STAGE + 1024 * (2 * i + (w & 1))));
+        for (int i = 0; i < G::DMA_N / 2; ++i) row_dma16(at + 128 * i, qs + (uint32_t)((w >> 1) * G::STAGE + 1024 * (2 * i + (w & 1))));
     } else {
-#pragma unroll
+#pragma unroll 1
         for (int i = 0; i < G::QD; ++i) {
             const int x = (w * G::QD + i) * 64 + lane;
             const int h = x / G::QC, c = (x - h * G::QC) ^ (h & 15);
-            page_dma16<false>(rs, h < p.rows ? (uint32_t)qoff[h] + 16u * (uint32_t)c : NO_ROW, 0u, qs + (uint32_t)((w * G::QD + i) * 1024));
+            row_dma16(base + qoff[h] + 16 * c, qs + (uint32_t)((w * G::QD + i) * 1024));
         }
     }
 }
@@ -312,13 +315,9 @@ __device__ __forceinline__ void narrow_piece(const AttnArgs & a, const Piece & p
         } else {
             if (k > 0) __syncthreads();
             sb = sh.ring + (par * NWAVE + w) * G::STAGE;
-            typename S::Dma dn = {};
-            if (k + 1 < n_my) {
-                dn = ss.plan(par ^ 1, p.ta + k + 1);
-                qk_slice<DK, true, S>(ss, dn, sb, lane, qreg, s0, s1);
-            } else {
-                qk_slice<DK, false, S>(ss, dn, sb, lane, qreg, s0, s1);
-            }
+            // (behind the last tile: a slice without cells, whose zeros land in the stage that is free)
+            const typename S::Dma dn = ss.plan(par ^ 1, p.ta + k + 1, k + 1 < n_my);
+            qk_slice<DK, true, S>(ss, dn, sb, lane, qreg, s0, s1);
             n_nxt = dn.n;
         }
         if (key + WK > p.lim_min && key < p.key1 && p.lim_min < p.key1) {     // some rows see these keys, others do not
@@ -429,14 +428,75 @@ __device__ __forceinline__ void slice_to_f16(const char * src, char * dst, int l
         const uint32_t * q = reinterpret_cast<const uint32_t *>(r + (o & ~3));
         const half_t d = *reinterpret_cast<const half_t *>(r + 34 * (hb >> 1));
         const uint32_t sh = (uint32_t)(o & 2);
-        // (the fifth word of an aligned run is the next block's, or past the slot's last row: not used then)
-        const uint32_t x[5] = {q[0], q[1], q[2], q[3], sh ? q[4] : 0u};
+        // (the fifth word of an aligned run is the next block's, or lies behind the slice's last row: not used then)
+        const uint32_t x[5] = {q[0], q[1], q[2], q[3], q[4]};
         uint32_t y[4];
 #pragma unroll
         for (int k = 0; k < 4; ++k) y[k] = __builtin_amdgcn_alignbyte(x[k + 1], x[k], sh);
         *reinterpret_cast<half8 *>(dst + slot_byte(row, 2 * hb)) = q8x8_to_f16<0>(y[0], y[1], 0u, d);
         *reinterpret_cast<half8 *>(dst + slot_byte(row, 2 * hb + 1)) = q8x8_to_f16<0>(y[2], y[3], 0u, d);
         if (i % 3 == 2) __builtin_amdgcn_sched_barrier(0);               // three half-blocks' loads in flight
+    }
+}
+
+// q fragments of a wave's 32 rows: qf[st] = row lane & 31, d = 16 st + 8 (lane >> 5) .. + 7, by way of the wave's own
+// slots of LDS (16 rows of f16 or 8 of f32 each), so that the rows are read in whole lines: lane by lane a fragment
+// is 16 bytes of a row, and 128 rows' lines do not stay in the L1 from one fragment to the next (4 us a piece).
+// slot0, slot1: byte offsets in `ring` of one slot or two; the wave's DMA of before is waited for as well.
+template <int DK, bool F16, int NS>
+__device__ __forceinline__ void q_wide(const char * base, const int64_t * qoff, char * ring, int slot0, int slot1, int lane,
+                                       half8 (&qf)[DK / 16]) {
+    using G = SliceGeom<DK>;
+    constexpr int RPS = F16 ? 16 : 8, ROUNDS = 32 / (NS * RPS);
+    const int hl = lane & 31, hi = lane >> 5;
+    const uint32_t lds = lds_addr(ring);
+#pragma unroll
+    for (int st = 0; st < DK / 16; ++st) qf[st] = half8{0, 0, 0, 0, 0, 0, 0, 0};
+    for (int rd = 0; rd < ROUNDS; ++rd) {
+#pragma unroll
+        for (int s = 0; s < NS; ++s) {
+            const int row0 = RPS * (NS * rd + s);
+            const uint32_t to = lds + (uint32_t)(s ? slot1 : slot0);
+            if constexpr (F16) {
+                const int r0 = 2 * (lane >> 4) + ((lane >> 3) & 1), c0 = 16 * ((lane & 7) ^ row_sw(r0));
+                const char * a0 = base + qoff[row0 + r0] + c0;
+                const char * a1 = base + qoff[row0 + r0 + 8] + c0;
+#pragma unroll 1
+                for (int i = 0; i < G::DMA_N; i += 2, a0 += 128, a1 += 128) {
+                    row_dma16(a0, to + 1024u * (uint32_t)i);
+                    row_dma16(a1, to + 1024u * (uint32_t)i + 1024u);
+                }
+            } else {
+                // row r at 4 DK r, its 16-byte chunk c at c ^ r
+#pragma unroll 1
+                for (int i = 0; i < DK / 32; ++i) {
+                    const int x = 64 * i + lane, r = x / G::QC, c = (x - r * G::QC) ^ r;
+                    row_dma16(base + qoff[row0 + r] + 16 * c, to + 1024u * (uint32_t)i);
+                }
+            }
+        }
+        wait_vm<0>();
+        const int in = hl - NS * RPS * rd;               // this lane's row among the round's
+        if (in >= 0 && in < NS * RPS) {
+            const char * at = ring + (NS > 1 && in >= RPS ? slot1 : slot0);
+            const int r = in % RPS;
+            if constexpr (F16) {
+                const int c0 = slot_byte(r, hi);
+#pragma unroll
+                for (int st = 0; st < DK / 16; ++st) qf[st] = *reinterpret_cast<const half8 *>(at + (c0 ^ (32 * (st & 3))) + 2048 * (st >> 2));
+            } else {
+#pragma unroll
+                for (int st = 0; st < DK / 16; ++st) {
+                    const f32x4 x = *reinterpret_cast<const f32x4 *>(at + 4 * DK * r + 16 * ((4 * st + 2 * hi) ^ r));
+                    const f32x4 y = *reinterpret_cast<const f32x4 *>(at + 4 * DK * r + 16 * ((4 * st + 2 * hi + 1) ^ r));
+                    half8 h = {to_half(x[0]), to_half(x[1]), to_half(x[2]), to_half(x[3]), to_half(y[0]), to_half(y[1]), to_half(y[2]), to_half(y[3])};
+                    asm volatile("" : "+v"(h));          // the f16 fragment is kept, not the f32 values
+                    qf[st] = h;
+                    if (st % 6 == 5) __builtin_amdgcn_sched_barrier(0);
+                }
+            }
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");      // the slots have been read
     }
 }
 
@@ -455,6 +515,11 @@ __device__ __forceinline__ void wide_piece(const AttnArgs & a, const Piece & p, 
     const bool live_w = HG * w < p.rows;                // a wave without rows only brings in its slices
     const int n_my = p.tb - p.ta;
 
+    // ---- the rows' q, then (f16: its slots are q's way) the first tile; 8 bits: the first two tiles, ahead of q ----
+    half8 qf[DK / 16];
+    const int lim = sh.lim[HG * w + hl];
+    const char * qbase = a.q + (int64_t)p.tok0 * a.q_nb2;
+    const int64_t * qoff = sh.qoff + HG * w;
     if constexpr (Q8) {
         const int n0 = ss.template put8<false>(0, p.ta, lane);
         const int n1 = n_my > 1 ? ss.template put8<false>(1, p.ta + 1, lane) : 0;
@@ -462,47 +527,16 @@ __device__ __forceinline__ void wide_piece(const AttnArgs & a, const Piece & p, 
             sh.vc[0][w] = n0;
             sh.vc[1][w] = n1;
         }
+        const int at = L::TILE + w * G::STAGE;
+        if (a.q_f16) q_wide<DK, true, 1>(qbase, qoff, sh.ring, at, at, lane, qf);
+        else q_wide<DK, false, 1>(qbase, qoff, sh.ring, at, at, lane, qf);
     } else {
+        if (a.q_f16) q_wide<DK, true, 2>(qbase, qoff, sh.ring, w * G::STAGE, (NWAVE + w) * G::STAGE, lane, qf);
+        else q_wide<DK, false, 2>(qbase, qoff, sh.ring, w * G::STAGE, (NWAVE + w) * G::STAGE, lane, qf);
         const typename S::Dma d0 = ss.plan(0, p.ta);
 #pragma unroll
         for (int i = 0; i < G::DMA_N; ++i) ss.template put<false>(d0, i);
         if (lane == 0) sh.vc[0][w] = d0.n;
-    }
-
-    // ---- q fragments of this wave's rows: qf[st] = row hl, d = 16 st + 8 hi .. + 7 ----
-    half8 qf[DK / 16];
-    const int lim = sh.lim[HG * w + hl];
-    const char * qrow = a.q + (int64_t)p.tok0 * a.q_nb2 + sh.qoff[HG * w + hl];
-    if (a.q_f16) {
-#pragma unroll
-        for (int st = 0; st < DK / 16; ++st) qf[st] = *reinterpret_cast<const half8 *>(qrow + 32 * st + 16 * hi);
-    } else {
-        constexpr int QB = DK / 16 % 6 == 0 ? 6 : 5;    // fragments per batch of loads, a batch ahead of its conversion
-        constexpr int NBT = DK / 16 / QB;
-        static_assert(NBT * QB == DK / 16, "whole batches");
-        f32x4 x[2][QB][2];
-        auto load = [&](int i, f32x4 (&xb)[QB][2]) __attribute__((always_inline)) {
-#pragma unroll
-            for (int b = 0; b < QB; ++b) {
-                xb[b][0] = *reinterpret_cast<const f32x4 *>(qrow + 64 * (QB * i + b) + 32 * hi);
-                xb[b][1] = *reinterpret_cast<const f32x4 *>(qrow + 64 * (QB * i + b) + 32 * hi + 16);
-            }
-            __builtin_amdgcn_sched_barrier(0);
-        };
-        load(0, x[0]);
-#pragma unroll
-        for (int i = 0; i < NBT; ++i) {
-            if (i + 1 < NBT) load(i + 1, x[(i + 1) & 1]);
-#pragma unroll
-            for (int b = 0; b < QB; ++b) {
-                const f32x4 (&y)[2] = x[i & 1][b];
-                half8 hq = {to_half(y[0][0]), to_half(y[0][1]), to_half(y[0][2]), to_half(y[0][3]),
-                            to_half(y[1][0]), to_half(y[1][1]), to_half(y[1][2]), to_half(y[1][3])};
-                asm volatile("" : "+v"(hq));            // keep the f16 fragment (not the f32 values) live
-                qf[QB * i + b] = hq;
-            }
-            __builtin_amdgcn_sched_barrier(0);
-        }
     }
 
     float m_run = M_NONE;                               // row hl, log2 units
@@ -548,16 +582,15 @@ __device__ __forceinline__ void wide_piece(const AttnArgs & a, const Piece & p, 
                 const int n = ss.template put8<false>(par, p.ta + k + 2, lane);
                 if (lane == 0) sh.vc[(k + 2) & 3][w] = n;
             }
-        } else if (pf) {
-            dn = ss.plan(par ^ 1, p.ta + k + 1);
+        } else {
+            // (behind the last tile: a slice without cells, whose zeros land in the stage that is free)
+            dn = ss.plan(par ^ 1, p.ta + k + 1, pf);
             if (lane == 0) sh.vc[(k + 1) & 3][w] = dn.n;
         }
         if (!live_w) {
             if constexpr (!Q8) {
-                if (pf) {
 #pragma unroll
-                    for (int i = 0; i < G::DMA_N; ++i) ss.template put<false>(dn, i);
-                }
+                for (int i = 0; i < G::DMA_N; ++i) ss.template put<false>(dn, i);
             }
             continue;
         }
@@ -567,15 +600,12 @@ __device__ __forceinline__ void wide_piece(const AttnArgs & a, const Piece & p, 
         for (int kp = 0; kp < NWAVE / 2; ++kp) {
             const char * sb = tile + 2 * kp * G::STAGE;
             f32x16 s;
-            if (!Q8 && pf) {
-                qk_pair_landed<DK>(sb, lane, qf, abuf, s, [&](int st) {
-                    constexpr int HALF = G::DMA_N / 2;
-                    static_assert(G::DMA_N % 2 == 0 && DK / 16 == 2 * G::DMA_N, "two pairs of slices of row blocks");
+            qk_pair_landed<DK>(sb, lane, qf, abuf, s, [&](int st) {
+                constexpr int HALF = G::DMA_N / 2;
+                static_assert(G::DMA_N % 2 == 0 && DK / 16 == 2 * G::DMA_N, "two pairs of slices of row blocks");
+                if constexpr (!Q8)
                     if ((st & 3) == 0) ss.template put<false>(dn, HALF * kp + st / 4);
-                });
-            } else {
-                qk_pair_landed<DK>(sb, lane, qf, abuf, s, [](int) {});
-            }
+            });
             constexpr int VPF = 3;
             half8 vb[VPF];
 #pragma unroll
