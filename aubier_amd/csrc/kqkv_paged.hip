@@ -57,7 +57,7 @@ struct Walk {
                                             // token, its number
     __device__ __forceinline__ double edge(int i) const { return i >= n_wg ? all : all * (double)i / (double)n_wg; }
     __device__ __forceinline__ int shared_blocks() const { return (shared_rows + BLOCK_ROWS - 1) / BLOCK_ROWS; }
-    __device__ __forceinline__ double shared_a(int n_head) const { return (double)(n_head * WIDE_START) + (double)n_head * (double)(WIDE_TILE * (shared_keys / TK)); }
+    __device__ __forceinline__ double shared_a(int n_head) const { return (double)n_head * (double)(WIDE_START + WIDE_TILE * (shared_keys / TK)); }
 };
 
 // request b's place: its tokens, what they see, its blocks and their costs (the j-th: a + 2 WIDE_TILE (j + 1), as
@@ -66,17 +66,17 @@ struct Request {
     int n, past, key0, blocks, first;
     bool wide;
     double a;
-    __device__ __forceinline__ Request(const AttnArgs & ar, const Walk & wk, int n_new, int past_, int b, int start) {
+    __device__ __forceinline__ Request(const AttnArgs & ar, const Walk & wk, int H, int n_new, int past_, int b, int start) {
         n = min(min(max(n_new, 0), ar.nt), ar.nt - start);
         past = min(clamp_past(past_), wk.cap);
         key0 = b < wk.n_share ? wk.shared_keys : 0;
-        blocks = (n * ar.n_head + BLOCK_ROWS - 1) / BLOCK_ROWS;
-        wide = n * ar.n_head > HG;
+        blocks = (n * H + BLOCK_ROWS - 1) / BLOCK_ROWS;
+        wide = n * H > HG;
         first = max((min(past + 1, wk.cap) - key0 + TK - 1) / TK, 1);
-        a = (double)(ar.n_head * start_cost()) + (double)ar.n_head * (double)((wide ? WIDE_TILE : NARROW_TILE) * first);
+        a = (double)H * (double)(start_cost() + (wide ? WIDE_TILE : NARROW_TILE) * first);
     }
-    __device__ __forceinline__ Request(const AttnArgs & ar, const Walk & wk, int b, int start)
-        : Request(ar, wk, ar.n_new[b], ar.past[b], b, start) {}
+    __device__ __forceinline__ Request(const AttnArgs & ar, const Walk & wk, int H, int b, int start)
+        : Request(ar, wk, H, ar.n_new[b], ar.past[b], b, start) {}
     __device__ __forceinline__ int start_cost() const { return wide ? WIDE_START : NARROW_START; }
     __device__ __forceinline__ double upto(int j) const { return (double)j * a + (double)WIDE_TILE * ((double)j * ((double)j + 1.0)); }
     __device__ __forceinline__ double cost() const { return upto(blocks); }
@@ -96,12 +96,20 @@ __device__ __forceinline__ Walk find_place(const AttnArgs & a, PlaceLds & sh) {
     const int per = (a.n_seq + NTHR - 1) / NTHR, b0 = min(tid * per, a.n_seq), b1 = min(b0 + per, a.n_seq);
     const int n_pre = a.prefix != nullptr ? min(max(a.prefix[1], 0), a.n_seq) : 0;
     const int k_pre = a.prefix != nullptr ? a.prefix[0] : 0;
-    Walk k;
+    Walk k = {};
     k.cap = a.max_pages << a.page_shift;
     // the first of this thread's requests stays in registers: up to 256 requests it is the only one
     const int n0 = b0 < b1 ? a.n_new[b0] : 0, past0 = b0 < b1 ? a.past[b0] : 0;
-    auto n_of = [&](int b) { return b == b0 ? n0 : a.n_new[b]; };
-    auto past_of = [&](int b) { return b == b0 ? past0 : a.past[b]; };
+    auto n_of = [=](int b) {
+        int v = n0;
+        if (b != b0) v = a.n_new[b];
+        return v;
+    };
+    auto past_of = [=](int b) {
+        int v = past0;
+        if (b != b0) v = a.past[b];
+        return v;
+    };
 
     int own = 0, keys = min(max(k_pre, 0), k.cap), active = 0, srows = 0, by = MAX_SEQS;
     for (int b = b0; b < b1; ++b) {
@@ -137,7 +145,6 @@ __device__ __forceinline__ Walk find_place(const AttnArgs & a, PlaceLds & sh) {
         total += sh.rows[i];
     }
     k.total = uni(min(total, a.nt));
-    k.n_share = k.shared_keys = k.shared_rows = k.shared_by = 0;
     if (a.prefix != nullptr) {
         // as many whole tiles of shared cells as all sharing requests with tokens held before them
         keys = uni(min(min(sh.shared[0][0], sh.shared[1][0]), min(sh.shared[2][0], sh.shared[3][0])) / TK * TK);
@@ -157,7 +164,7 @@ __device__ __forceinline__ Walk find_place(const AttnArgs & a, PlaceLds & sh) {
     {
         int at = min(start, a.nt);
         for (int b = b0; b < b1; ++b) {
-            const Request rq(a, k, n_of(b), past_of(b), b, at);
+            const Request rq(a, k, H, n_of(b), past_of(b), b, at);
             cost += rq.cost();
             groups += (uint64_t)rq.blocks + ((uint64_t)(uint32_t)(rq.blocks * rq.first) << 32);
             at += rq.n;
@@ -187,23 +194,12 @@ __device__ __forceinline__ Walk find_place(const AttnArgs & a, PlaceLds & sh) {
     k.n_wg = uni((int)min(max(tiles, (int64_t)1), (int64_t)gridDim.x));
     k.x0 = k.edge(wg);
     k.x1 = k.edge(wg + 1);
-    k.b = a.n_seq;
-    if (wg >= k.n_wg || k.total == 0) return k;
 
-    if (uni(k.x0 < shared_cost)) {
-        int j = min((int)(k.x0 / shared_a), k.shared_blocks() - 1);
-        while (j > 0 && (double)j * shared_a > k.x0) --j;
-        while (j + 1 < k.shared_blocks() && (double)(j + 1) * shared_a <= k.x0) ++j;
-        k.b = -1;
-        k.base = 0.0;
-        k.tok0 = 0;
-        k.j = k.g = uni(j);
-        return k;
-    }
-    if (base <= k.x0 && k.x0 < base + cost) {
+    const bool any = wg < k.n_wg && k.total > 0, at_shared = uni(k.x0 < shared_cost);
+    if (any && !at_shared && base <= k.x0 && k.x0 < base + cost) {
         int at = min(start, a.nt), g = (int)(uint32_t)grp;
         for (int b = b0; b < b1; ++b) {
-            const Request rq(a, k, n_of(b), past_of(b), b, at);
+            const Request rq(a, k, H, n_of(b), past_of(b), b, at);
             const double c = rq.cost();
             if (rq.blocks > 0 && (k.x0 < base + c || b + 1 == b1)) {
                 sh.b = b;
@@ -218,26 +214,29 @@ __device__ __forceinline__ Walk find_place(const AttnArgs & a, PlaceLds & sh) {
         }
     }
     __syncthreads();
-    k.b = uni(sh.b);
-    if (k.b >= a.n_seq) return k;
-    k.tok0 = uni(sh.tok0);
-    k.base = sh.base;
-    int lo = 0;
-    {
-        const Request rq(a, k, k.b, k.tok0);
+    k.b = any ? (at_shared ? -1 : uni(sh.b)) : a.n_seq;
+    k.tok0 = at_shared ? 0 : uni(sh.tok0);
+    k.base = at_shared ? 0.0 : sh.base;
+    int j = 0;
+    if (at_shared) {
+        j = min((int)(k.x0 / shared_a), k.shared_blocks() - 1);
+        while (j > 0 && (double)j * shared_a > k.x0) --j;
+        while (j + 1 < k.shared_blocks() && (double)(j + 1) * shared_a <= k.x0) ++j;
+    } else if (k.b < a.n_seq) {
+        const Request rq(a, k, H, k.b, k.tok0);
         int len = rq.blocks;
         while (len > 1) {
             const int half = len >> 1;
-            if (k.base + rq.upto(lo + half) <= k.x0) {
-                lo += half;
+            if (k.base + rq.upto(j + half) <= k.x0) {
+                j += half;
                 len -= half;
             } else {
                 len = half;
             }
         }
     }
-    k.j = uni(lo);
-    k.g = uni(k.shared_blocks() + sh.g + lo);
+    k.j = uni(j);
+    k.g = at_shared ? k.j : uni(k.shared_blocks() + sh.g + j);
     return k;
 }
 
@@ -248,7 +247,7 @@ struct KernelLds {
     PlaceLds place;
 };
 
-template <int DK, int DV, bool Q8>
+template <int DK, int DV, bool Q8, bool QF16>
 __global__ __launch_bounds__(NTHR, 1) void kqkv_paged_kernel(AttnArgs a) {
     using L = PieceLds<DK, DV, Q8>;
     __shared__ KernelLds<DK, DV, Q8> lds;
@@ -264,7 +263,8 @@ __global__ __launch_bounds__(NTHR, 1) void kqkv_paged_kernel(AttnArgs a) {
         int pieces = 0, j, b;
         Walk next;
         {
-            const int H = a.n_head;
+            int H = a.n_head;
+            asm volatile("" : "+s"(H));      // its 64-bit form is taken anew for each piece, not kept through them
             b = uni(k.b);
             j = uni(k.j);
             p.tok0 = uni(k.tok0);
@@ -286,7 +286,7 @@ __global__ __launch_bounds__(NTHR, 1) void kqkv_paged_kernel(AttnArgs a) {
                 body = g0 + (double)(H * WIDE_START);
                 cost = (double)blocks * sa;
             } else {
-                const Request rq(a, k, b, p.tok0);
+                const Request rq(a, k, H, b, p.tok0);
                 n = rq.n;
                 cost = rq.cost();
                 blocks = rq.blocks;
@@ -324,7 +324,7 @@ __global__ __launch_bounds__(NTHR, 1) void kqkv_paged_kernel(AttnArgs a) {
                 next.tok0 = p.tok0 + n;
                 next.j = 0;
                 next.b = b + 1;
-                while (next.b < a.n_seq && Request(a, k, next.b, next.tok0).blocks == 0) ++next.b;
+                while (next.b < a.n_seq && Request(a, k, H, next.b, next.tok0).blocks == 0) ++next.b;
                 last = uni(next.b >= a.n_seq);
             }
         }
@@ -343,9 +343,9 @@ __global__ __launch_bounds__(NTHR, 1) void kqkv_paged_kernel(AttnArgs a) {
         if (p.ta >= p.tb) {                  // no tile of the group falls to this workgroup (never where direct)
             if (tid < BLOCK_ROWS) reinterpret_cast<f32x2 *>(rec)[tid] = f32x2{-INFINITY, 0.0f};
         } else if (p.rows <= HG) {
-            narrow_piece<DK, DV, Q8>(a, p, sh, rec);
+            narrow_piece<DK, DV, Q8, QF16>(a, p, sh, rec);
         } else {
-            wide_piece<DK, DV, Q8>(a, p, sh, rec);
+            wide_piece<DK, DV, Q8, QF16>(a, p, sh, rec);
         }
         if (last) return;
         k = lds.walk;
@@ -552,8 +552,9 @@ size_t attn_workspace_bytes(int, int dv, int n_seq, int n_head, int nt) {
 
 template <int DK, int DV>
 static hipError_t launch(bool q8, const AttnArgs & a, hipStream_t stream) {
-    if (q8) hipLaunchKernelGGL((kqkv_paged_kernel<DK, DV, true>), dim3(N_WG), dim3(NTHR), 0, stream, a);
-    else hipLaunchKernelGGL((kqkv_paged_kernel<DK, DV, false>), dim3(N_WG), dim3(NTHR), 0, stream, a);
+    auto run = [&](void (*kernel)(AttnArgs)) { hipLaunchKernelGGL(kernel, dim3(N_WG), dim3(NTHR), 0, stream, a); };
+    if (q8) run(a.q_f16 ? kqkv_paged_kernel<DK, DV, true, true> : kqkv_paged_kernel<DK, DV, true, false>);
+    else run(a.q_f16 ? kqkv_paged_kernel<DK, DV, false, true> : kqkv_paged_kernel<DK, DV, false, false>);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     const int rows = a.n_head * a.nt;

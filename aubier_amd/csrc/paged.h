@@ -69,7 +69,8 @@ struct AttnArgs {
 };
 bool attn_supported(int dk, int dv);
 size_t attn_workspace_bytes(int dk, int dv, int n_seq, int n_head, int nt);
-constexpr int64_t MAX_STRIDE = 1 << 25;   // bytes between rows of the cache, heads and tokens of q: 32-bit offsets inside a tile
+constexpr int64_t MAX_STRIDE = 1 << 25;   // bytes between rows of the cache: 32-bit offsets inside a tile
+constexpr int64_t Q_SPAN = 1u << 31;      // 128 rows of q span at most this: 127 q_nb2 + n_head q_nb1
 hipError_t launch_attn(int dk, int dv, bool q8, const AttnArgs & a, hipStream_t stream);
 
 }  // namespace paged

@@ -56,7 +56,7 @@ struct PieceLds {
     __attribute__((aligned(16))) char ring[RING];
     __attribute__((aligned(16))) half_t px[Q8 ? 1 : 2][HG * DecodeCfg<DK, DV>::PROW];
     __attribute__((aligned(16))) float red[2][HG][NWAVE];
-    __attribute__((aligned(16))) int64_t qoff[BLOCK_ROWS];              // byte offset of a row's q from the first token's
+    uint32_t qoff[BLOCK_ROWS];                                          // byte offset of a row's q from its block's first token's
     int drow[BLOCK_ROWS];                                               // its row of dst (head * nt + token), -1: none
     int lim[BLOCK_ROWS];                                                // keys it sees
     // cells of a slice that are seen (by tile modulo 4: tile k + 2's are written while others read tile k's), and
@@ -73,13 +73,22 @@ __device__ __forceinline__ int opaque_tid() {
     return t;
 }
 
-__device__ __forceinline__ void piece_rows(const AttnArgs & a, const Piece & p, int64_t * qoff, int * drow, int * lim) {
+// zero likewise (sixteen registers of it were kept in scratch memory between pieces, and their reload waited for the
+// first tile)
+__device__ __forceinline__ float opaque_zero() {
+    float z;
+    asm volatile("v_mov_b32 %0, 0" : "=v"(z));
+    return z;
+}
+
+__device__ __forceinline__ void piece_rows(const AttnArgs & a, const Piece & p, uint32_t * qoff, int * drow, int * lim) {
     const int tid = threadIdx.x;
     if (tid >= BLOCK_ROWS) return;
     const int r = p.row0 + tid;
     const int t = r / a.n_head, h = r - t * a.n_head;
     const bool live = tid < p.rows;
-    qoff[tid] = live ? (int64_t)t * a.q_nb2 + (int64_t)h * a.q_nb1 : 0;
+    // (a row that is not there brings in the first token's first head; nothing of it is used)
+    qoff[tid] = live ? (uint32_t)(t - p.row0 / a.n_head) * (uint32_t)a.q_nb2 + (uint32_t)h * (uint32_t)a.q_nb1 : 0u;
     drow[tid] = live ? h * a.nt + p.tok0 + t : -1;
     lim[tid] = live ? min(p.past + t + 1, p.key1) : 0;
 }
@@ -177,16 +186,21 @@ __device__ __forceinline__ void clear_nonfinite(char * sb, int lane, uint64_t & 
 template <int DV, int NC, int PITCH>
 __device__ __forceinline__ void rows_out_f16(const AttnArgs & a, const Piece & p, char * rec, const char * stg, int row0, int c0,
                                              const int * drow, int lane) {
-    constexpr int CPR = NC / 8;
-#pragma unroll
-    for (int it = 0; it < CPR / 2; ++it) {
-        const int q = 64 * it + lane;
-        const int row = q / CPR, ch = q % CPR;
-        const u32x4 v = *reinterpret_cast<const u32x4 *>(stg + row * PITCH + 16 * ch);
-        if (p.slot >= 0) {
-            __builtin_nontemporal_store(v, reinterpret_cast<u32x4 *>(rec + BLOCK_ROWS * 8 + ((size_t)(row0 + row) * DV + c0 + 8 * ch) * 2));
-        } else {
-            const int dr = drow[row0 + row];
+    constexpr int CPR = NC / 8, RPI = 64 / CPR;         // chunks per row, rows per round of the wavefront
+    static_assert(64 % CPR == 0, "whole rows");
+    const int r = lane / CPR, ch = lane % CPR;
+    stg += r * PITCH + 16 * ch;
+    if (p.slot >= 0) {
+        char * to = rec + BLOCK_ROWS * 8 + ((size_t)(row0 + r) * DV + c0 + 8 * ch) * 2;
+#pragma unroll 8
+        for (int it = 0; it < HG / RPI; ++it, to += RPI * DV * 2, stg += RPI * PITCH)
+            __builtin_nontemporal_store(*reinterpret_cast<const u32x4 *>(stg), reinterpret_cast<u32x4 *>(to));
+    } else {
+        drow += row0 + r;
+#pragma unroll 4
+        for (int it = 0; it < HG / RPI; ++it, stg += RPI * PITCH) {
+            const u32x4 v = *reinterpret_cast<const u32x4 *>(stg);
+            const int dr = drow[RPI * it];
             if (dr >= 0) *reinterpret_cast<u32x4 *>(a.dst + ((size_t)dr * DV + c0 + 8 * ch) * 2) = v;
         }
     }
@@ -213,34 +227,31 @@ __device__ __forceinline__ void scale_acc(f32x16 (&o)[N], float f) {
 }
 
 // ---------------------------------------------------------------- up to 32 rows
-// LDS DMA from a 64-bit address per lane (16 bytes; lane l's land at lds_base + 16 l), for rows of q, whose strides have
-// no bound
-__device__ __forceinline__ void row_dma16(const char * at, uint32_t lds_base) {
-    asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, off" :: "v"(at), "{m0}"(lds_base) : "memory");
-}
-
+// Rows of q are reached by 32-bit offsets from the first token's (Q_SPAN, which the host checks); a 64-bit address per
+// lane (global_load_lds) takes 1 to 2 us more a piece.
 // q of the 32 rows into LDS at qs (f32: q_convert's layout; f16: two slices of 16 rows, as K rows lie), this wave's
-// share.  Rows that are not there bring in the first row again; nothing of theirs is used.
+// share
 template <int DK, bool F16>
-__device__ __forceinline__ void q_rows_dma(const AttnArgs & a, const Piece & p, const int64_t * qoff, uint32_t qs, int w, int lane) {
+__device__ __forceinline__ void q_rows_dma(const AttnArgs & a, const Piece & p, const uint32_t * qoff, uint32_t qs, int w, int lane) {
     using G = SliceGeom<DK>;
-    const char * base = a.q + (int64_t)p.tok0 * a.q_nb2;
+    const i32x4 rs = make_rsrc(a.q + (int64_t)(p.tok0 + p.row0 / a.n_head) * a.q_nb2, (uint32_t)Q_SPAN);
     if constexpr (F16) {
         const int r0 = 2 * (lane >> 4) + ((lane >> 3) & 1);
-        const char * at = base + qoff[8 * w + r0] + 16 * ((lane & 7) ^ row_sw(r0));
+        const uint32_t at = qoff[8 * w + r0] + 16u * (uint32_t)((lane & 7) ^ row_sw(r0));
 #pragma unroll
-        for (int i = 0; i < G::DMA_N / 2; ++i) row_dma16(at + 128 * i, qs + (uint32_t)((w >> 1) * G::STAGE + 1024 * (2 * i + (w & 1))));
+        for (int i = 0; i < G::DMA_N / 2; ++i)
+            page_dma16<false>(rs, at, 128u * (uint32_t)i, qs + (uint32_t)((w >> 1) * G::STAGE + 1024 * (2 * i + (w & 1))));
     } else {
 #pragma unroll 1
         for (int i = 0; i < G::QD; ++i) {
             const int x = (w * G::QD + i) * 64 + lane;
             const int h = x / G::QC, c = (x - h * G::QC) ^ (h & 15);
-            row_dma16(base + qoff[h] + 16 * c, qs + (uint32_t)((w * G::QD + i) * 1024));
+            page_dma16<false>(rs, qoff[h] + 16u * (uint32_t)c, 0u, qs + (uint32_t)((w * G::QD + i) * 1024));
         }
     }
 }
 
-template <int DK, int DV, bool Q8>
+template <int DK, int DV, bool Q8, bool QF16>
 __device__ __forceinline__ void narrow_piece(const AttnArgs & a, const Piece & p, PieceLds<DK, DV, Q8> & sh, char * rec) {
     using G = SliceGeom<DK>;
     using C = DecodeCfg<DK, DV>;
@@ -255,8 +266,7 @@ __device__ __forceinline__ void narrow_piece(const AttnArgs & a, const Piece & p
     // ---- q by way of LDS the stream does not use yet, the first tile (8 bits: two tiles) behind it ----
     half8 qreg[2][G::QSTEPS];
     char * qs = Q8 ? sh.ring + L::TILE : sh.ring + NWAVE * G::STAGE;
-    if (a.q_f16) q_rows_dma<DK, true>(a, p, sh.qoff, lds_addr(qs), w, lane);
-    else q_rows_dma<DK, false>(a, p, sh.qoff, lds_addr(qs), w, lane);
+    q_rows_dma<DK, QF16>(a, p, sh.qoff, lds_addr(qs), w, lane);
     int n_cur, n_nxt = 0;                    // cells that are seen, of this wave's slice of the tile and of the next
     if constexpr (Q8) {
         n_cur = ss.put8(0, p.ta, lane);
@@ -274,7 +284,7 @@ __device__ __forceinline__ void narrow_piece(const AttnArgs & a, const Piece & p
         wait_vm<G::DMA_N>();
     }
     __syncthreads();
-    if (a.q_f16) {
+    if constexpr (QF16) {
         const int a0 = slot_byte(j16, g);
 #pragma unroll
         for (int n = 0; n < 2; ++n)
@@ -290,10 +300,11 @@ __device__ __forceinline__ void narrow_piece(const AttnArgs & a, const Piece & p
     float m_ref[2] = {M_NONE, M_NONE};       // rows 16 n + j16, log2 units
     float l_acc = 0.0f;                      // row lane & 31, keys 8 (lane >> 5) .. + 7 of each slice
     f32x16 o[C::NTQ];                        // o^T tiles, as kqkv_decode.hip
+    const float zero = opaque_zero();
 #pragma unroll
     for (int i = 0; i < C::NTQ; ++i)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) o[i][r] = 0.0f;
+        for (int r = 0; r < 16; ++r) o[i][r] = zero;
     const PvAddr pv(lane);
 
     for (int k = 0; k < n_my; ++k) {
@@ -315,9 +326,9 @@ __device__ __forceinline__ void narrow_piece(const AttnArgs & a, const Piece & p
         } else {
             if (k > 0) __syncthreads();
             sb = sh.ring + (par * NWAVE + w) * G::STAGE;
-            // (behind the last tile: a slice without cells, whose zeros land in the stage that is free)
             const typename S::Dma dn = ss.plan(par ^ 1, p.ta + k + 1, k + 1 < n_my);
-            qk_slice<DK, true, S>(ss, dn, sb, lane, qreg, s0, s1);
+            if (k + 1 < n_my) qk_slice<DK, true, S>(ss, dn, sb, lane, qreg, s0, s1);
+            else qk_slice<DK, false, S>(ss, dn, sb, lane, qreg, s0, s1);
             n_nxt = dn.n;
         }
         if (key + WK > p.lim_min && key < p.key1 && p.lim_min < p.key1) {     // some rows see these keys, others do not
@@ -414,27 +425,27 @@ __device__ __forceinline__ void narrow_piece(const AttnArgs & a, const Piece & p
 }
 
 // ---------------------------------------------------------------- up to 128 rows
-// A wave's int8 slice at src -> its f16 slot at dst: per lane, half-blocks (16 values) of one row; rows from n on
-// become zeros
+// A wave's int8 slice at src -> its f16 slot at dst: per lane, half-blocks (16 values) of one row
 template <int DK>
 __device__ __forceinline__ void slice_to_f16(const char * src, char * dst, int lane) {
     using G8 = Q8Geom<DK>;
-    const int row = lane & 15;
-    const char * r = src + row * G8::ROWB;
+    // half-block h + 4 i of a row, h = lane >> 4: block (h >> 1) + 2 i, so everything moves by constants with i
+    const int row = lane & 15, h = lane >> 4;
+    const int o = 34 * (h >> 1) + 2 + 16 * (h & 1);                      // its first byte of the row; 68 i further on
+    const uint32_t sh = (uint32_t)(o & 2);
+    const char * q = src + row * G8::ROWB + (o & ~3), * d = src + row * G8::ROWB + 34 * (h >> 1);
+    char * t0 = dst + slot_byte(row, 2 * h), * t1 = dst + slot_byte(row, 2 * h + 1);
 #pragma unroll
     for (int i = 0; i < G8::ITEMS; ++i) {
-        const int hb = (lane >> 4) + 4 * i;                              // half-block
-        const int o = 34 * (hb >> 1) + 2 + 16 * (hb & 1);
-        const uint32_t * q = reinterpret_cast<const uint32_t *>(r + (o & ~3));
-        const half_t d = *reinterpret_cast<const half_t *>(r + 34 * (hb >> 1));
-        const uint32_t sh = (uint32_t)(o & 2);
+        uint32_t x[5], y[4];
         // (the fifth word of an aligned run is the next block's, or lies behind the slice's last row: not used then)
-        const uint32_t x[5] = {q[0], q[1], q[2], q[3], q[4]};
-        uint32_t y[4];
+#pragma unroll
+        for (int k = 0; k < 5; ++k) x[k] = *reinterpret_cast<const uint32_t *>(q + 68 * i + 4 * k);
+        const half_t ds = *reinterpret_cast<const half_t *>(d + 68 * i);
 #pragma unroll
         for (int k = 0; k < 4; ++k) y[k] = __builtin_amdgcn_alignbyte(x[k + 1], x[k], sh);
-        *reinterpret_cast<half8 *>(dst + slot_byte(row, 2 * hb)) = q8x8_to_f16<0>(y[0], y[1], 0u, d);
-        *reinterpret_cast<half8 *>(dst + slot_byte(row, 2 * hb + 1)) = q8x8_to_f16<0>(y[2], y[3], 0u, d);
+        *reinterpret_cast<half8 *>(t0 + 2048 * i) = q8x8_to_f16<0>(y[0], y[1], 0u, ds);
+        *reinterpret_cast<half8 *>(t1 + 2048 * i) = q8x8_to_f16<0>(y[2], y[3], 0u, ds);
         if (i % 3 == 2) __builtin_amdgcn_sched_barrier(0);               // three half-blocks' loads in flight
     }
 }
@@ -444,7 +455,7 @@ __device__ __forceinline__ void slice_to_f16(const char * src, char * dst, int l
 // is 16 bytes of a row, and 128 rows' lines do not stay in the L1 from one fragment to the next (4 us a piece).
 // slot0, slot1: byte offsets in `ring` of one slot or two; the wave's DMA of before is waited for as well.
 template <int DK, bool F16, int NS>
-__device__ __forceinline__ void q_wide(const char * base, const int64_t * qoff, char * ring, int slot0, int slot1, int lane,
+__device__ __forceinline__ void q_wide(const i32x4 rs, const uint32_t * qoff, char * ring, int slot0, int slot1, int lane,
                                        half8 (&qf)[DK / 16]) {
     using G = SliceGeom<DK>;
     constexpr int RPS = F16 ? 16 : 8, ROUNDS = 32 / (NS * RPS);
@@ -459,19 +470,15 @@ __device__ __forceinline__ void q_wide(const char * base, const int64_t * qoff, 
             const uint32_t to = lds + (uint32_t)(s ? slot1 : slot0);
             if constexpr (F16) {
                 const int r0 = 2 * (lane >> 4) + ((lane >> 3) & 1), c0 = 16 * ((lane & 7) ^ row_sw(r0));
-                const char * a0 = base + qoff[row0 + r0] + c0;
-                const char * a1 = base + qoff[row0 + r0 + 8] + c0;
-#pragma unroll 1
-                for (int i = 0; i < G::DMA_N; i += 2, a0 += 128, a1 += 128) {
-                    row_dma16(a0, to + 1024u * (uint32_t)i);
-                    row_dma16(a1, to + 1024u * (uint32_t)i + 1024u);
-                }
+                const uint32_t a0 = qoff[row0 + r0] + (uint32_t)c0, a1 = qoff[row0 + r0 + 8] + (uint32_t)c0;
+#pragma unroll
+                for (int i = 0; i < G::DMA_N; ++i) page_dma16<false>(rs, (i & 1) ? a1 : a0, 128u * (uint32_t)(i >> 1), to + 1024u * (uint32_t)i);
             } else {
                 // row r at 4 DK r, its 16-byte chunk c at c ^ r
 #pragma unroll 1
                 for (int i = 0; i < DK / 32; ++i) {
                     const int x = 64 * i + lane, r = x / G::QC, c = (x - r * G::QC) ^ r;
-                    row_dma16(base + qoff[row0 + r] + 16 * c, to + 1024u * (uint32_t)i);
+                    page_dma16<false>(rs, qoff[row0 + r] + 16u * (uint32_t)c, 0u, to + 1024u * (uint32_t)i);
                 }
             }
         }
@@ -500,7 +507,7 @@ __device__ __forceinline__ void q_wide(const char * base, const int64_t * qoff, 
     }
 }
 
-template <int DK, int DV, bool Q8>
+template <int DK, int DV, bool Q8, bool QF16>
 __device__ __forceinline__ void wide_piece(const AttnArgs & a, const Piece & p, PieceLds<DK, DV, Q8> & sh, char * rec) {
     using G = SliceGeom<DK>;
     using S = PageStream<DK>;
@@ -518,8 +525,8 @@ __device__ __forceinline__ void wide_piece(const AttnArgs & a, const Piece & p, 
     // ---- the rows' q, then (f16: its slots are q's way) the first tile; 8 bits: the first two tiles, ahead of q ----
     half8 qf[DK / 16];
     const int lim = sh.lim[HG * w + hl];
-    const char * qbase = a.q + (int64_t)p.tok0 * a.q_nb2;
-    const int64_t * qoff = sh.qoff + HG * w;
+    const i32x4 qrs = make_rsrc(a.q + (int64_t)(p.tok0 + p.row0 / a.n_head) * a.q_nb2, (uint32_t)Q_SPAN);
+    const uint32_t * qoff = sh.qoff + HG * w;
     if constexpr (Q8) {
         const int n0 = ss.template put8<false>(0, p.ta, lane);
         const int n1 = n_my > 1 ? ss.template put8<false>(1, p.ta + 1, lane) : 0;
@@ -528,11 +535,9 @@ __device__ __forceinline__ void wide_piece(const AttnArgs & a, const Piece & p, 
             sh.vc[1][w] = n1;
         }
         const int at = L::TILE + w * G::STAGE;
-        if (a.q_f16) q_wide<DK, true, 1>(qbase, qoff, sh.ring, at, at, lane, qf);
-        else q_wide<DK, false, 1>(qbase, qoff, sh.ring, at, at, lane, qf);
+        q_wide<DK, QF16, 1>(qrs, qoff, sh.ring, at, at, lane, qf);
     } else {
-        if (a.q_f16) q_wide<DK, true, 2>(qbase, qoff, sh.ring, w * G::STAGE, (NWAVE + w) * G::STAGE, lane, qf);
-        else q_wide<DK, false, 2>(qbase, qoff, sh.ring, w * G::STAGE, (NWAVE + w) * G::STAGE, lane, qf);
+        q_wide<DK, QF16, 2>(qrs, qoff, sh.ring, w * G::STAGE, (NWAVE + w) * G::STAGE, lane, qf);
         const typename S::Dma d0 = ss.plan(0, p.ta);
 #pragma unroll
         for (int i = 0; i < G::DMA_N; ++i) ss.template put<false>(d0, i);
@@ -542,10 +547,11 @@ __device__ __forceinline__ void wide_piece(const AttnArgs & a, const Piece & p, 
     float m_run = M_NONE;                               // row hl, log2 units
     float l_acc = 0.0f;                                 // row hl, this lane's half of the keys
     f32x16 o[NB];                                       // o^T tile i: C row = column 32 i + 8 (r / 4) + 4 hi + (r & 3), C col = row hl
+    const float zero = opaque_zero();
 #pragma unroll
     for (int i = 0; i < NB; ++i)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) o[i][r] = 0.0f;
+        for (int r = 0; r < 16; ++r) o[i][r] = zero;
     const PairPvAddr pv(lane);
 
     for (int k = 0; k < n_my; ++k) {
