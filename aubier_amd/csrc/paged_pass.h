@@ -229,8 +229,28 @@ __device__ __forceinline__ void scale_acc(f32x16 (&o)[N], float f) {
 // ---------------------------------------------------------------- up to 32 rows
 // Rows of q are reached by 32-bit offsets from the first token's (Q_SPAN, which the host checks); a 64-bit address per
 // lane (global_load_lds) takes 1 to 2 us more a piece.
-// q of the 32 rows into LDS at qs (f32: q_convert's layout; f16: two slices of 16 rows, as K rows lie), this wave's
-// share
+// Eight rows of f32 q into LDS by a wavefront: DMA instruction i brings chunks 8 i .. 8 i + 7 (16 bytes) of every row, lane
+// l's to 1 KB block i at 16 l.  squeeze() then turns them into f16 in place, row r's 16-byte chunk c at
+// 1024 (c >> 3) + 128 r + 16 ((c & 7) ^ r) of the first half: the fragments' reads find no bank twice.
+__device__ __forceinline__ uint32_t f32_rows_offset(const uint32_t * qoff, int lane) {
+    return qoff[lane >> 3] + 16u * (uint32_t)(lane & 7);
+}
+template <int DK, typename AT>
+__device__ __forceinline__ void squeeze(char * ring, AT && at, char * to, int lane) {
+    using G = SliceGeom<DK>;
+    const int l7 = lane & 7, r = lane >> 3;
+    f32x4 x[G::DMA_N];
+#pragma unroll
+    for (int i = 0; i < G::DMA_N; ++i) x[i] = *reinterpret_cast<const f32x4 *>(ring + at(i) + 16 * lane);
+    char * t = to + 128 * r + 16 * ((l7 >> 1) ^ r) + 8 * (l7 & 1);
+    char * t1 = to + 128 * r + 16 * (((l7 >> 1) + 4) ^ r) + 8 * (l7 & 1);
+#pragma unroll
+    for (int i = 0; i < G::DMA_N; ++i)
+        *reinterpret_cast<half4 *>(((i & 1) ? t1 : t) + 1024 * (i >> 1)) = half4{to_half(x[i][0]), to_half(x[i][1]), to_half(x[i][2]), to_half(x[i][3])};
+}
+
+// q of the 32 rows into LDS at qs, this wave's share: its 8 rows, as f32 (squeezed later), or as f16 half a slice of 16
+// rows, as K rows lie
 template <int DK, bool F16>
 __device__ __forceinline__ void q_rows_dma(const AttnArgs & a, const Piece & p, const uint32_t * qoff, uint32_t qs, int w, int lane) {
     using G = SliceGeom<DK>;
@@ -242,12 +262,9 @@ __device__ __forceinline__ void q_rows_dma(const AttnArgs & a, const Piece & p, 
         for (int i = 0; i < G::DMA_N / 2; ++i)
             page_dma16<false>(rs, at, 128u * (uint32_t)i, qs + (uint32_t)((w >> 1) * G::STAGE + 1024 * (2 * i + (w & 1))));
     } else {
-#pragma unroll 1
-        for (int i = 0; i < G::QD; ++i) {
-            const int x = (w * G::QD + i) * 64 + lane;
-            const int h = x / G::QC, c = (x - h * G::QC) ^ (h & 15);
-            page_dma16<false>(rs, qoff[h] + 16u * (uint32_t)c, 0u, qs + (uint32_t)((w * G::QD + i) * 1024));
-        }
+        const uint32_t at = f32_rows_offset(qoff + 8 * w, lane);
+#pragma unroll
+        for (int i = 0; i < G::DMA_N; ++i) page_dma16<false>(rs, at, 128u * (uint32_t)i, qs + (uint32_t)(w * G::STAGE + 1024 * i));
     }
 }
 
@@ -283,16 +300,17 @@ __device__ __forceinline__ void narrow_piece(const AttnArgs & a, const Piece & p
         n_cur = d0.n;
         wait_vm<G::DMA_N>();
     }
+    if constexpr (!QF16) squeeze<DK>(qs + w * G::STAGE, [](int i) { return 1024 * i; }, qs + w * G::STAGE, lane);
     __syncthreads();
-    if constexpr (QF16) {
-        const int a0 = slot_byte(j16, g);
+    {
+        // chunk 4 s + g of row 16 n + j16
+        const int a0 = QF16 ? slot_byte(j16, g) : (j16 >> 3) * G::STAGE + 128 * (j16 & 7) + 16 * (g ^ (j16 & 7));
 #pragma unroll
         for (int n = 0; n < 2; ++n)
 #pragma unroll
             for (int s = 0; s < G::QSTEPS; ++s)
-                qreg[n][s] = *reinterpret_cast<const half8 *>(qs + n * G::STAGE + (a0 ^ (64 * (s & 1))) + 2048 * (s >> 1));
-    } else {
-        q_convert<DK>(qs, lane, qreg);
+                qreg[n][s] = *reinterpret_cast<const half8 *>(qs + (QF16 ? n : 2 * n) * G::STAGE + (a0 ^ (64 * (s & 1))) +
+                                                              (QF16 ? 2048 : 1024) * (s >> 1));
     }
     const int lim[2] = {sh.lim[j16], sh.lim[16 + j16]};
     __syncthreads();
@@ -450,62 +468,56 @@ __device__ __forceinline__ void slice_to_f16(const char * src, char * dst, int l
     }
 }
 
-// q fragments of a wave's 32 rows: qf[st] = row lane & 31, d = 16 st + 8 (lane >> 5) .. + 7, by way of the wave's own
-// slots of LDS (16 rows of f16 or 8 of f32 each), so that the rows are read in whole lines: lane by lane a fragment
-// is 16 bytes of a row, and 128 rows' lines do not stay in the L1 from one fragment to the next (4 us a piece).
-// slot0, slot1: byte offsets in `ring` of one slot or two; the wave's DMA of before is waited for as well.
-template <int DK, bool F16, int NS>
-__device__ __forceinline__ void q_wide(const i32x4 rs, const uint32_t * qoff, char * ring, int slot0, int slot1, int lane,
-                                       half8 (&qf)[DK / 16]) {
+// q of a wave's 32 rows as fragments, qf[st] = row lane & 31, d = 16 st + 8 (lane >> 5) .. + 7, by way of LDS of the
+// wave's own, so that the rows are read in whole lines: lane by lane a fragment is 16 bytes of a row, and 128 rows'
+// lines do not stay in the L1 from one fragment to the next (4 us a piece).  In units of 16 rows of f16 or 8 of f32, as
+// large as an f16 slice: even ones through buffer A, odd ones through B, two in flight, and the piece's first tiles
+// behind the last even one.  A buffer lies in two halves (the 8-bit ring's slots are half a slice): 1 KB block i at
+// lo + 1024 i below G::DMA_N / 2, at hi + 1024 i from there on.
+struct QBuffer { int lo, hi; };
+template <int DK, bool F16>
+struct QWide {
     using G = SliceGeom<DK>;
-    constexpr int RPS = F16 ? 16 : 8, ROUNDS = 32 / (NS * RPS);
-    const int hl = lane & 31, hi = lane >> 5;
-    const uint32_t lds = lds_addr(ring);
+    static constexpr int RPU = F16 ? 16 : 8, UNITS = 32 / RPU, HALF = G::DMA_N / 2;
+    // unit u's DMA_N instructions
+    static __device__ __forceinline__ void put(const i32x4 rs, const uint32_t * qoff, uint32_t ring, const QBuffer to, int u, int lane) {
+        auto at = [&](int i) { return ring + (uint32_t)(i < HALF ? to.lo : to.hi) + 1024u * (uint32_t)i; };
+        if constexpr (F16) {
+            const int r0 = 2 * (lane >> 4) + ((lane >> 3) & 1);
+            const uint32_t c0 = 16u * (uint32_t)((lane & 7) ^ row_sw(r0));
+            const uint32_t a0 = qoff[RPU * u + r0] + c0, a1 = qoff[RPU * u + r0 + 8] + c0;
 #pragma unroll
-    for (int st = 0; st < DK / 16; ++st) qf[st] = half8{0, 0, 0, 0, 0, 0, 0, 0};
-    for (int rd = 0; rd < ROUNDS; ++rd) {
+            for (int i = 0; i < G::DMA_N; ++i) page_dma16<false>(rs, (i & 1) ? a1 : a0, 128u * (uint32_t)(i >> 1), at(i));
+        } else {
+            const uint32_t a0 = f32_rows_offset(qoff + RPU * u, lane);
 #pragma unroll
-        for (int s = 0; s < NS; ++s) {
-            const int row0 = RPS * (NS * rd + s);
-            const uint32_t to = lds + (uint32_t)(s ? slot1 : slot0);
-            if constexpr (F16) {
-                const int r0 = 2 * (lane >> 4) + ((lane >> 3) & 1), c0 = 16 * ((lane & 7) ^ row_sw(r0));
-                const uint32_t a0 = qoff[row0 + r0] + (uint32_t)c0, a1 = qoff[row0 + r0 + 8] + (uint32_t)c0;
-#pragma unroll
-                for (int i = 0; i < G::DMA_N; ++i) page_dma16<false>(rs, (i & 1) ? a1 : a0, 128u * (uint32_t)(i >> 1), to + 1024u * (uint32_t)i);
-            } else {
-                // row r at 4 DK r, its 16-byte chunk c at c ^ r
-#pragma unroll 1
-                for (int i = 0; i < DK / 32; ++i) {
-                    const int x = 64 * i + lane, r = x / G::QC, c = (x - r * G::QC) ^ r;
-                    page_dma16<false>(rs, qoff[row0 + r] + 16u * (uint32_t)c, 0u, to + 1024u * (uint32_t)i);
-                }
-            }
+            for (int i = 0; i < G::DMA_N; ++i) page_dma16<false>(rs, a0, 128u * (uint32_t)i, at(i));
         }
-        wait_vm<0>();
-        const int in = hl - NS * RPS * rd;               // this lane's row among the round's
-        if (in >= 0 && in < NS * RPS) {
-            const char * at = ring + (NS > 1 && in >= RPS ? slot1 : slot0);
-            const int r = in % RPS;
-            if constexpr (F16) {
-                const int c0 = slot_byte(r, hi);
-#pragma unroll
-                for (int st = 0; st < DK / 16; ++st) qf[st] = *reinterpret_cast<const half8 *>(at + (c0 ^ (32 * (st & 3))) + 2048 * (st >> 2));
-            } else {
-#pragma unroll
-                for (int st = 0; st < DK / 16; ++st) {
-                    const f32x4 x = *reinterpret_cast<const f32x4 *>(at + 4 * DK * r + 16 * ((4 * st + 2 * hi) ^ r));
-                    const f32x4 y = *reinterpret_cast<const f32x4 *>(at + 4 * DK * r + 16 * ((4 * st + 2 * hi + 1) ^ r));
-                    half8 h = {to_half(x[0]), to_half(x[1]), to_half(x[2]), to_half(x[3]), to_half(y[0]), to_half(y[1]), to_half(y[2]), to_half(y[3])};
-                    asm volatile("" : "+v"(h));          // the f16 fragment is kept, not the f32 values
-                    qf[st] = h;
-                    if (st % 6 == 5) __builtin_amdgcn_sched_barrier(0);
-                }
-            }
-        }
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");      // the slots have been read
     }
-}
+    static __device__ __forceinline__ void get(char * ring, const QBuffer from, int u, int lane, half8 (&qf)[DK / 16]) {
+        const int hl = lane & 31, hi = lane >> 5, r = hl - RPU * u;
+        const int lo = from.lo, step = from.hi - from.lo;
+        if constexpr (!F16) squeeze<DK>(ring, [&](int i) { return lo + (i < HALF ? 0 : step) + 1024 * i; }, ring + lo, lane);
+        if (r >= 0 && r < RPU) read(ring, lo, step, r, hi, qf);
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");      // the buffer has been read
+    }
+    static __device__ __forceinline__ void read(const char * ring, int lo, int step, int r, int hi, half8 (&qf)[DK / 16]) {
+        if constexpr (F16) {
+            const int c0 = slot_byte(r, hi);
+#pragma unroll
+            for (int st = 0; st < DK / 16; ++st) {
+                const int blk = 2 * (st >> 2);                           // of rows 0 .. 7; rows 8 .. 15: the next
+                const int o = blk + 1 < HALF ? 0 : blk < HALF ? step * (r >> 3) : step;
+                qf[st] = *reinterpret_cast<const half8 *>(ring + lo + o + (c0 ^ (32 * (st & 3))) + 2048 * (st >> 2));
+            }
+        } else {
+            const int c0 = 128 * r + 16 * (hi ^ r);
+#pragma unroll
+            for (int st = 0; st < DK / 16; ++st)
+                qf[st] = *reinterpret_cast<const half8 *>(ring + lo + (c0 ^ (32 * (st & 3))) + 1024 * (st >> 2));
+        }
+    }
+};
 
 template <int DK, int DV, bool Q8, bool QF16>
 __device__ __forceinline__ void wide_piece(const AttnArgs & a, const Piece & p, PieceLds<DK, DV, Q8> & sh, char * rec) {
@@ -522,36 +534,66 @@ __device__ __forceinline__ void wide_piece(const AttnArgs & a, const Piece & p, 
     const bool live_w = HG * w < p.rows;                // a wave without rows only brings in its slices
     const int n_my = p.tb - p.ta;
 
-    // ---- the rows' q, then (f16: its slots are q's way) the first tile; 8 bits: the first two tiles, ahead of q ----
+    // ---- the rows' q and the first tile (8 bits: two), o ----
+    using QW = QWide<DK, QF16>;
     half8 qf[DK / 16];
-    const int lim = sh.lim[HG * w + hl];
-    const i32x4 qrs = make_rsrc(a.q + (int64_t)(p.tok0 + p.row0 / a.n_head) * a.q_nb2, (uint32_t)Q_SPAN);
-    const uint32_t * qoff = sh.qoff + HG * w;
-    if constexpr (Q8) {
-        const int n0 = ss.template put8<false>(0, p.ta, lane);
-        const int n1 = n_my > 1 ? ss.template put8<false>(1, p.ta + 1, lane) : 0;
-        if (lane == 0) {
-            sh.vc[0][w] = n0;
-            sh.vc[1][w] = n1;
-        }
-        const int at = L::TILE + w * G::STAGE;
-        q_wide<DK, QF16, 1>(qrs, qoff, sh.ring, at, at, lane, qf);
-    } else {
-        q_wide<DK, QF16, 2>(qrs, qoff, sh.ring, w * G::STAGE, (NWAVE + w) * G::STAGE, lane, qf);
-        const typename S::Dma d0 = ss.plan(0, p.ta);
 #pragma unroll
-        for (int i = 0; i < G::DMA_N; ++i) ss.template put<false>(d0, i);
-        if (lane == 0) sh.vc[0][w] = d0.n;
+    for (int st = 0; st < DK / 16; ++st) qf[st] = half8{0, 0, 0, 0, 0, 0, 0, 0};
+    f32x16 o[NB];                                       // o^T tile i: C row = column 32 i + 8 (r / 4) + 4 hi + (r & 3), C col = row hl
+    const int lim = sh.lim[HG * w + hl];
+    {
+        const i32x4 qrs = make_rsrc(a.q + (int64_t)(p.tok0 + p.row0 / a.n_head) * a.q_nb2, (uint32_t)Q_SPAN);
+        const uint32_t * qoff = sh.qoff + HG * w;
+        const uint32_t ring = lds_addr(sh.ring);
+        // buffer A is where the first tiles go: the slot of stage 0, or the int8 slots of both stages
+        constexpr int HALF_BYTES = 1024 * QW::HALF;
+        static_assert(!Q8 || HALF_BYTES <= L::SLOT8, "half a unit fits an int8 slot");
+        const QBuffer A = Q8 ? QBuffer{w * L::SLOT8, (NWAVE + w) * L::SLOT8 - HALF_BYTES} : QBuffer{w * G::STAGE, w * G::STAGE};
+        const int b_at = Q8 ? L::TILE + w * G::STAGE : (NWAVE + w) * G::STAGE;
+        const QBuffer B = {b_at, b_at};
+        QW::put(qrs, qoff, ring, A, 0, lane);
+        QW::put(qrs, qoff, ring, B, 1, lane);
+        const float zero = opaque_zero();
+#pragma unroll
+        for (int i = 0; i < NB; ++i)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) o[i][r] = zero;
+#pragma unroll 1
+        for (int u = 2; u < QW::UNITS; u += 2) {
+            wait_vm<G::DMA_N>();
+            QW::get(sh.ring, A, u - 2, lane, qf);
+            QW::put(qrs, qoff, ring, A, u, lane);
+            wait_vm<G::DMA_N>();
+            QW::get(sh.ring, B, u - 1, lane, qf);
+            QW::put(qrs, qoff, ring, B, u + 1, lane);
+        }
+        wait_vm<G::DMA_N>();
+        QW::get(sh.ring, A, QW::UNITS - 2, lane, qf);
+        if constexpr (Q8) {
+            const int n0 = ss.template put8<false>(0, p.ta, lane);
+            int n1 = 0;
+            if (n_my > 1) {
+                n1 = ss.template put8<false>(1, p.ta + 1, lane);
+                wait_vm<2 * S::N8>();
+            } else {
+                wait_vm<S::N8>();
+            }
+            if (lane == 0) {
+                sh.vc[0][w] = n0;
+                sh.vc[1][w] = n1;
+            }
+        } else {
+            const typename S::Dma d0 = ss.plan(0, p.ta);
+#pragma unroll
+            for (int i = 0; i < G::DMA_N; ++i) ss.template put<false>(d0, i);
+            if (lane == 0) sh.vc[0][w] = d0.n;
+            wait_vm<G::DMA_N>();
+        }
+        QW::get(sh.ring, B, QW::UNITS - 1, lane, qf);
     }
 
     float m_run = M_NONE;                               // row hl, log2 units
     float l_acc = 0.0f;                                 // row hl, this lane's half of the keys
-    f32x16 o[NB];                                       // o^T tile i: C row = column 32 i + 8 (r / 4) + 4 hi + (r & 3), C col = row hl
-    const float zero = opaque_zero();
-#pragma unroll
-    for (int i = 0; i < NB; ++i)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) o[i][r] = zero;
     const PairPvAddr pv(lane);
 
     for (int k = 0; k < n_my; ++k) {
