@@ -29,9 +29,14 @@ namespace {
 
 constexpr int N_WG = 256;                   // one workgroup per CU
 constexpr int MIN_SHARED_TILES = 1;         // fewer shared tiles than this are left to the requests
-// costs, in tenths of a wide tile (all of them times H, so that they are whole numbers)
-constexpr int WIDE_TILE = 10, NARROW_TILE = 7;
-constexpr int WIDE_START = 20, NARROW_START = 12;   // a piece's rows in, its results out
+// Costs, in tenths of a wide tile (all of them times H, so that they are whole numbers): a tile for up to 128 rows and
+// for up to 32, and a piece's start and end (its rows in, its results out).
+template <int DK, bool Q8>
+struct Cost {
+    static constexpr bool BIG = DK == 576;
+    static constexpr int WIDE_TILE = 10, NARROW_TILE = Q8 ? (BIG ? 5 : 6) : BIG ? 6 : 7;
+    static constexpr int WIDE_START = Q8 ? (BIG ? 22 : 20) : BIG ? 21 : 28, NARROW_START = Q8 ? (BIG ? 9 : 11) : BIG ? 11 : 16;
+};
 
 // Workspace: a header, the pieces of every shared block and of every row, the records
 struct Head { int rows, shared_rows; };
@@ -55,13 +60,16 @@ struct Walk {
     int shared_by;                          // the first of them that has tokens
     int b, j, tok0, g;                      // the next group: block j of request b (-1: of the shared rows), its first
                                             // token, its number
-    __device__ __forceinline__ double edge(int i) const { return i >= n_wg ? all : all * (double)i / (double)n_wg; }
+    double per;                             // all / n_wg
+    __device__ __forceinline__ double edge(int i) const { return i >= n_wg ? all : per * (double)i; }
     __device__ __forceinline__ int shared_blocks() const { return (shared_rows + BLOCK_ROWS - 1) / BLOCK_ROWS; }
-    __device__ __forceinline__ double shared_a(int n_head) const { return (double)n_head * (double)(WIDE_START + WIDE_TILE * (shared_keys / TK)); }
+    template <typename C>
+    __device__ __forceinline__ double shared_a(int n_head) const { return (double)n_head * (double)(C::WIDE_START + C::WIDE_TILE * (shared_keys / TK)); }
 };
 
 // request b's place: its tokens, what they see, its blocks and their costs (the j-th: a + 2 WIDE_TILE (j + 1), as
 // 128 rows on are 128 / H tokens, 2 / H tiles)
+template <typename C>
 struct Request {
     int n, past, key0, blocks, first;
     bool wide;
@@ -73,12 +81,12 @@ struct Request {
         blocks = (n * H + BLOCK_ROWS - 1) / BLOCK_ROWS;
         wide = n * H > HG;
         first = max((min(past + 1, wk.cap) - key0 + TK - 1) / TK, 1);
-        a = (double)H * (double)(start_cost() + (wide ? WIDE_TILE : NARROW_TILE) * first);
+        a = (double)H * (double)(start_cost() + (wide ? C::WIDE_TILE : C::NARROW_TILE) * first);
     }
     __device__ __forceinline__ Request(const AttnArgs & ar, const Walk & wk, int H, int b, int start)
-        : Request(ar, wk, H, ar.n_new[b], ar.past[b], b, start) {}
-    __device__ __forceinline__ int start_cost() const { return wide ? WIDE_START : NARROW_START; }
-    __device__ __forceinline__ double upto(int j) const { return (double)j * a + (double)WIDE_TILE * ((double)j * ((double)j + 1.0)); }
+        : Request<C>(ar, wk, H, ar.n_new[b], ar.past[b], b, start) {}
+    __device__ __forceinline__ int start_cost() const { return wide ? C::WIDE_START : C::NARROW_START; }
+    __device__ __forceinline__ double upto(int j) const { return (double)j * a + (double)C::WIDE_TILE * ((double)j * ((double)j + 1.0)); }
     __device__ __forceinline__ double cost() const { return upto(blocks); }
 };
 
@@ -91,6 +99,7 @@ struct PlaceLds {
     double base;
     int b, tok0, g;
 };
+template <typename C>
 __device__ __forceinline__ Walk find_place(const AttnArgs & a, PlaceLds & sh) {
     const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, H = a.n_head, wg = blockIdx.x;
     const int per = (a.n_seq + NTHR - 1) / NTHR, b0 = min(tid * per, a.n_seq), b1 = min(b0 + per, a.n_seq);
@@ -156,7 +165,7 @@ __device__ __forceinline__ Walk find_place(const AttnArgs & a, PlaceLds & sh) {
             k.shared_by = uni(min(min(sh.shared[0][3], sh.shared[1][3]), min(sh.shared[2][3], sh.shared[3][3])));
         }
     }
-    const double shared_a = k.shared_a(H), shared_cost = (double)k.shared_blocks() * shared_a;
+    const double shared_a = k.template shared_a<C>(H), shared_cost = (double)k.shared_blocks() * shared_a;
 
     // costs, and (tiles, groups) in the high and low half of a word
     double cost = 0.0;
@@ -164,7 +173,7 @@ __device__ __forceinline__ Walk find_place(const AttnArgs & a, PlaceLds & sh) {
     {
         int at = min(start, a.nt);
         for (int b = b0; b < b1; ++b) {
-            const Request rq(a, k, H, n_of(b), past_of(b), b, at);
+            const Request<C> rq(a, k, H, n_of(b), past_of(b), b, at);
             cost += rq.cost();
             groups += (uint64_t)rq.blocks + ((uint64_t)(uint32_t)(rq.blocks * rq.first) << 32);
             at += rq.n;
@@ -192,6 +201,7 @@ __device__ __forceinline__ Walk find_place(const AttnArgs & a, PlaceLds & sh) {
     // at most one workgroup per tile
     const int64_t tiles = (int64_t)(all_groups >> 32) + (int64_t)k.shared_blocks() * (k.shared_keys / TK);
     k.n_wg = uni((int)min(max(tiles, (int64_t)1), (int64_t)gridDim.x));
+    k.per = k.all / (double)k.n_wg;
     k.x0 = k.edge(wg);
     k.x1 = k.edge(wg + 1);
 
@@ -199,7 +209,7 @@ __device__ __forceinline__ Walk find_place(const AttnArgs & a, PlaceLds & sh) {
     if (any && !at_shared && base <= k.x0 && k.x0 < base + cost) {
         int at = min(start, a.nt), g = (int)(uint32_t)grp;
         for (int b = b0; b < b1; ++b) {
-            const Request rq(a, k, H, n_of(b), past_of(b), b, at);
+            const Request<C> rq(a, k, H, n_of(b), past_of(b), b, at);
             const double c = rq.cost();
             if (rq.blocks > 0 && (k.x0 < base + c || b + 1 == b1)) {
                 sh.b = b;
@@ -223,7 +233,7 @@ __device__ __forceinline__ Walk find_place(const AttnArgs & a, PlaceLds & sh) {
         while (j > 0 && (double)j * shared_a > k.x0) --j;
         while (j + 1 < k.shared_blocks() && (double)(j + 1) * shared_a <= k.x0) ++j;
     } else if (k.b < a.n_seq) {
-        const Request rq(a, k, H, k.b, k.tok0);
+        const Request<C> rq(a, k, H, k.b, k.tok0);
         int len = rq.blocks;
         while (len > 1) {
             const int half = len >> 1;
@@ -253,7 +263,8 @@ __global__ __launch_bounds__(NTHR, 1) void kqkv_paged_kernel(AttnArgs a) {
     __shared__ KernelLds<DK, DV, Q8> lds;
     L & sh = lds.piece;
     const int tid = threadIdx.x, wg = blockIdx.x;
-    Walk k = find_place(a, lds.place);
+    using C = Cost<DK, Q8>;
+    Walk k = find_place<C>(a, lds.place);
     if (wg == 0 && tid == 0) *reinterpret_cast<Head *>(a.work) = Head{k.total * a.n_head, k.shared_rows};
     if (k.b >= a.n_seq) return;              // no part of the line
     for (;;) {
@@ -280,13 +291,13 @@ __global__ __launch_bounds__(NTHR, 1) void kqkv_paged_kernel(AttnArgs a) {
                 p.table = reinterpret_cast<const int32_t *>(reinterpret_cast<const char *>(a.table) + (int64_t)uni(k.shared_by) * a.t_nb1);
                 n_tiles = p.key1 / TK;
                 blocks = k.shared_blocks();
-                const double sa = k.shared_a(H);
+                const double sa = k.template shared_a<C>(H);
                 g0 = (double)j * sa;
                 g1 = (double)(j + 1) * sa;
-                body = g0 + (double)(H * WIDE_START);
+                body = g0 + (double)(H * C::WIDE_START);
                 cost = (double)blocks * sa;
             } else {
-                const Request rq(a, k, H, b, p.tok0);
+                const Request<C> rq(a, k, H, b, p.tok0);
                 n = rq.n;
                 cost = rq.cost();
                 blocks = rq.blocks;
@@ -302,15 +313,14 @@ __global__ __launch_bounds__(NTHR, 1) void kqkv_paged_kernel(AttnArgs a) {
                 body = g0 + (double)(H * rq.start_cost());
                 direct = uni(b >= k.n_share && g0 >= k.x0 && g1 <= k.x1);
             }
-            auto tile_at = [&](double x) {
-                return x <= body ? 0 : x >= g1 ? n_tiles : min(n_tiles, (int)((x - body) / (g1 - body) * (double)n_tiles + 0.5));
-            };
+            const double rate = (double)n_tiles / (g1 - body);
+            auto tile_at = [&](double x) { return x <= body ? 0 : x >= g1 ? n_tiles : min(n_tiles, (int)((x - body) * rate + 0.5)); };
             p.ta = uni(tile_at(k.x0));
             p.tb = uni(tile_at(k.x1));
             p.slot = direct ? -1 : uni(wg + k.g);
             first = uni(g0 >= k.x0);                     // the group's first piece says how many there are
             if (first && !direct) {
-                int e = min(max((int)(g1 / k.all * (double)k.n_wg), wg + 1), k.n_wg);
+                int e = min(max((int)(g1 / k.per), wg + 1), k.n_wg);
                 while (e > wg + 1 && k.edge(e - 1) >= g1) --e;
                 while (e < k.n_wg && k.edge(e) < g1) ++e;
                 pieces = uni(e - wg);
@@ -324,7 +334,7 @@ __global__ __launch_bounds__(NTHR, 1) void kqkv_paged_kernel(AttnArgs a) {
                 next.tok0 = p.tok0 + n;
                 next.j = 0;
                 next.b = b + 1;
-                while (next.b < a.n_seq && Request(a, k, H, next.b, next.tok0).blocks == 0) ++next.b;
+                while (next.b < a.n_seq && Request<C>(a, k, H, next.b, next.tok0).blocks == 0) ++next.b;
                 last = uni(next.b >= a.n_seq);
             }
         }
@@ -506,7 +516,8 @@ __global__ __launch_bounds__(NTHR) void kqkv_paged_merge_kernel(AttnArgs a) {
         if (mine && rp.n > 0 && rp.n <= MANY_PIECES) {
             const int col = 8 * (lane % LP);
             Part p;
-            p.template add<DV, 4>(rp, records, lane / LP, PW, col);
+            if (rp.n <= 2 * PW) p.template add<DV, 2>(rp, records, lane / LP, PW, col);      // a chunk's rows
+            else p.template add<DV, 4>(rp, records, lane / LP, PW, col);
             if constexpr (PW == 2) {
                 Part q;                                  // the other half's
                 float lo, up;
