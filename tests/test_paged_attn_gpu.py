@@ -247,3 +247,92 @@ def test_two_streams(dev):
     for b, o in zip(bs, outs):
         check(b, o[0])
         assert all(torch.equal(x, o[0]) for x in o)
+
+
+@pytest.mark.parametrize("n_seq", [256, 257, 4096])
+def test_most_requests(dev, n_seq):
+    new = [(1, 0, 2, 0, 0)[i % 5] for i in range(n_seq)]
+    b = Batch(dev, [(29 * i) % 90 for i in range(n_seq)], new, 16, dk=320, H=8, seed=n_seq, pad=1)
+    check(b, b.run(), f"{n_seq} requests")
+    b = Batch(dev, [0] * (n_seq - 1) + [500], [0] * (n_seq - 1) + [3], 16, dk=320, H=8, seed=n_seq)      # only the last
+    check(b, b.run(), "only the last")
+
+
+@pytest.mark.parametrize("H,past,new", [(1024, [70, 130], [1, 1]), (1, [300], [300]), (1, [5, 900, 64], [33, 1, 130]), (7, [1000], [64])])
+def test_rows_across_blocks(dev, H, past, new):
+    """Blocks of 128 rows that begin and end inside a token, tokens that begin and end inside a block."""
+    b = Batch(dev, past, new, 32, dk=320, H=H, seed=H, pad=1)
+    check(b, b.run(b.out(torch.float16)))
+
+
+def test_no_tokens(dev):
+    b = Batch(dev, [50, 0, 7], [0, 0, 0], 16, dk=320, seed=1, pad=4)
+    assert (b.run() == 7.0).all()
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.05, 1e-30])
+def test_scales(dev, scale):
+    b = Batch(dev, [700, 20], [1, 6], 16, dk=320, seed=2)
+    got = A.ggml_m4_kqkv_paged(b.kc, b.q, b.past, b.new, b.table, 16, scale, out=b.out()).double()
+    k, r = b.values.double(), 0
+    for s, (p, n) in enumerate(zip(b.past_l, b.new_l)):
+        for i in range(n):
+            j = torch.arange(p + i + 1, device=dev)
+            kk = k[b.table[s, j // 16].long() * 16 + j % 16]
+            w = torch.softmax(b.q[r].double() @ kk.t() * scale, dim=1)
+            # f16 weights and records: 2^-11 each, twice the former
+            assert ((got[:, r] - w @ kk[:, :256]).abs() <= 4 * 2.0 ** -11 * (w @ kk[:, :256].abs()) + 2.0 ** -24).all()
+            r += 1
+
+
+@pytest.mark.parametrize("dk,H,past,new,prefix,share,cache", [
+    (576, 32, [2100, 2048, 2300, 40], [1, 4, 1, 1], 2048, 3, "f16"), (320, 16, [3000, 10, 0], [1, 200, 1], 0, 0, "q8"),
+    (320, 40, [600, 513, 700], [2, 2, 2], 512, 3, "q8"), (576, 128, [900, 33], [1, 3], 0, 0, "f16")])
+def test_workspace(dev, dk, H, past, new, prefix, share, cache):
+    """What the workspace holds at the start does not matter, nothing behind it (or behind dst) is written, and a byte
+    less is refused."""
+    b = Batch(dev, past, new, 16, dk=dk, H=H, cache=cache, prefix=prefix, share=share, pad=2, seed=31)
+    need = A.kqkv_paged_workspace_bytes(b.kc, b.q, b.past, b.out())
+    big = torch.empty(need + (1 << 20), dtype=torch.uint8, device=dev)
+    got = []
+    for fill in (0, 255, 127):
+        big.fill_(fill)
+        room = torch.full((b.H * b.nt * b.dv + 4096,), 7.0, device=dev)
+        out = room[:b.H * b.nt * b.dv].view(b.H, b.nt, b.dv)
+        b.run(out, workspace=big[:need])
+        assert (big[need:] == fill).all() and (room[b.H * b.nt * b.dv:] == 7.0).all()
+        got.append(out)
+    check(b, got[0])
+    assert torch.equal(got[0], got[1]) and torch.equal(got[0], got[2])
+    with pytest.raises(A.MlaM4Error) as e:
+        b.run(workspace=big[:need - 1])
+    assert e.value.status == -5
+
+
+def test_shared_cells_on_pages_that_are_none(dev):
+    b = Batch(dev, [700, 650, 640], [1, 2, 1], 16, dk=320, H=40, prefix=640, share=3, seed=32)
+    t = b.table.clone()
+    t[:, 4], t[:, 39] = -1, 10 ** 6
+    b.table = t
+    b.kc[torch.isnan(b.kc)] = 1.0
+    check(b, b.run())
+
+
+def test_first_sharer_without_tokens(dev):
+    """The shared cells are read through the table of the first request that has tokens; the others' tables, and what
+    they hold, do not matter."""
+    b = Batch(dev, [400, 420, 330, 500], [0, 1, 2, 1], 64, dk=320, prefix=320, share=4, seed=33)
+    b.table[0] = -1
+    b.past[0] = 3
+    check(b, b.run())
+
+
+def test_same_pages_twice(dev):
+    """Two requests with one table (a forked conversation before it writes): each sees the same cells."""
+    b = Batch(dev, [333, 100], [1, 1], 16, dk=320, seed=34, poison=1.0)
+    b.table[1] = b.table[0]
+    b.past[1] = 333
+    b.q[1] = b.q[0]
+    got = b.run()
+    check(b, got)
+    assert torch.equal(got[:, 0], got[:, 1])
