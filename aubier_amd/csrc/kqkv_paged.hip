@@ -15,8 +15,10 @@
 // for a group's start and end) are laid end to end, and workgroup i of N takes the i-th N-th of the line: pieces of one
 // or several groups.  Every workgroup finds its place by itself from the lengths (two prefix sums over the requests),
 // so nothing is planned on the host and nothing waits for a planning launch.  A group that ends up in one piece, with
-// nothing shared, goes straight to dst; the other pieces leave records, which the second launch merges.  Piece of
-// group g in workgroup i has record i + g: along the line one of the two grows from piece to piece.
+// nothing shared, goes straight to dst; the other pieces leave records, which the second launch merges.  Groups of
+// rows that share cells come first on the line and always leave records: piece of group g in workgroup i has record
+// i + g, as along the line one of the two grows from piece to piece.  Of the other groups a workgroup holds at most two
+// in part, one that began before it and one that goes on behind it: records 2 i and 2 i + 1.
 //
 // All positions on the line are computed by the same expressions in every workgroup (in 64-bit floating point, exact
 // for whole numbers below 2^53), so the workgroups agree where one ends and the next begins.
@@ -38,9 +40,11 @@ struct Cost {
     static constexpr int WIDE_START = Q8 ? (BIG ? 22 : 20) : BIG ? 21 : 28, NARROW_START = Q8 ? (BIG ? 9 : 11) : BIG ? 11 : 16;
 };
 
-// Workspace: a header, the pieces of every shared block and of every row, the records
+// Workspace: a header, the pieces of every shared block and of every row, the records (those of whole groups, two per
+// workgroup, then those of the sharing rows' groups)
 struct Head { int rows, shared_rows; };
 struct Pieces { int slot; unsigned n_row; };                    // first record, pieces (low 16 bits) and row of the block
+constexpr int SHARED_RECORDS = 2 * N_WG;                        // where the latter begin
 __host__ __device__ inline size_t shared_blocks(int n_head, int nt) { return ((size_t)n_head * nt + BLOCK_ROWS - 1) / BLOCK_ROWS; }
 __host__ __device__ inline size_t shared_off() { return 256; }
 __host__ __device__ inline size_t own_off(int n_head, int nt) { return shared_off() + (shared_blocks(n_head, nt) * 8 + 255) / 256 * 256; }
@@ -317,8 +321,8 @@ __global__ __launch_bounds__(NTHR, 1) void kqkv_paged_kernel(AttnArgs a) {
             auto tile_at = [&](double x) { return x <= body ? 0 : x >= g1 ? n_tiles : min(n_tiles, (int)((x - body) * rate + 0.5)); };
             p.ta = uni(tile_at(k.x0));
             p.tb = uni(tile_at(k.x1));
-            p.slot = direct ? -1 : uni(wg + k.g);
             first = uni(g0 >= k.x0);                     // the group's first piece says how many there are
+            p.slot = direct ? -1 : uni(b < k.n_share ? SHARED_RECORDS + wg + k.g : 2 * wg + (first ? 1 : 0));
             if (first && !direct) {
                 int e = min(max((int)(g1 / k.per), wg + 1), k.n_wg);
                 while (e > wg + 1 && k.edge(e - 1) >= g1) --e;
@@ -367,6 +371,7 @@ __global__ __launch_bounds__(NTHR, 1) void kqkv_paged_kernel(AttnArgs a) {
 // The pieces of a row: those of its own group, then those of its shared block
 struct RowPieces {
     int n, n_own, own, shared, r_own, r_shared;
+    bool shares;
     __device__ __forceinline__ RowPieces(const AttnArgs & a, const Head & head, int row) {
         // (both read at once, whatever the row: the shared block's entry lies in the workspace also where there is none)
         const Pieces o = reinterpret_cast<const Pieces *>(a.work + own_off(a.n_head, a.nt))[row];
@@ -376,15 +381,16 @@ struct RowPieces {
         own = o.slot;
         shared = s.slot;
         r_shared = row % BLOCK_ROWS;
-        // a row that is complete has none at all: it shares nothing
-        n = n_own + (n_own > 0 && row < head.shared_rows ? (int)s.n_row : 0);
+        shares = row < head.shared_rows;
+        n = n_own + (shares ? (int)s.n_row : 0);
     }
-    // row q's record and its row of it
+    // piece q's record, and the row's place in it
     template <int DV>
     __device__ __forceinline__ const char * at(const char * records, int q, int & r) const {
         const bool mine = q < n_own;
         r = mine ? r_own : r_shared;
-        return records + (size_t)(mine ? own + q : shared + q - n_own) * record_bytes<DV>();
+        const int of_own = shares ? own + q : own + max(2 * q - 1, 0);
+        return records + (size_t)(mine ? of_own : shared + q - n_own) * record_bytes<DV>();
     }
 };
 
@@ -555,10 +561,12 @@ __global__ __launch_bounds__(NTHR) void kqkv_paged_merge_kernel(AttnArgs a) {
 
 bool attn_supported(int dk, int dv) { return (dk == 576 && dv == 512) || (dk == 320 && dv == 256); }
 
-size_t attn_workspace_bytes(int, int dv, int n_seq, int n_head, int nt) {
-    // records: one per workgroup and group (own blocks: at most one partly filled per request with tokens)
-    const size_t groups = 2 * shared_blocks(n_head, nt) + (size_t)(n_seq < nt ? n_seq : nt);
-    return records_off(n_head, nt) + (N_WG + groups) * (dv == 512 ? record_bytes<512>() : record_bytes<256>());
+size_t attn_workspace_bytes(int dv, int n_seq, int n_head, int nt, bool prefix) {
+    // the sharing rows' records: one per workgroup and group, shared blocks and own ones, of which each request with
+    // tokens has at most one that is not full
+    size_t n = SHARED_RECORDS;
+    if (prefix) n += N_WG + 2 * shared_blocks(n_head, nt) + (size_t)(n_seq < nt ? n_seq : nt);
+    return records_off(n_head, nt) + n * (dv == 512 ? record_bytes<512>() : record_bytes<256>());
 }
 
 template <int DK, int DV>

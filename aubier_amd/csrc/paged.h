@@ -32,6 +32,7 @@ struct PagesArgs {
 hipError_t launch_pages(const PagesArgs & a, hipStream_t stream);
 
 constexpr int MAX_ROPE = 256;       // rope columns of a row
+constexpr int MAX_KV_ROWS = 1 << 24;  // a wavefront each: the grid's threads stay below 2^32
 struct KvRowsArgs {
     const void * x;         // rows of n_out values, f32 or f16
     int64_t x_nb1;
@@ -68,7 +69,7 @@ struct AttnArgs {
     int q_f16, dst_f16;
 };
 bool attn_supported(int dk, int dv);
-size_t attn_workspace_bytes(int dk, int dv, int n_seq, int n_head, int nt);
+size_t attn_workspace_bytes(int dv, int n_seq, int n_head, int nt, bool prefix);
 constexpr int64_t MAX_STRIDE = 1 << 25;   // bytes between rows of the cache: 32-bit offsets inside a tile
 constexpr int64_t Q_SPAN = 1u << 31;      // 128 rows of q span at most this: 127 q_nb2 + n_head q_nb1
 hipError_t launch_attn(int dk, int dv, bool q8, const AttnArgs & a, hipStream_t stream);

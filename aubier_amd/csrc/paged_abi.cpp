@@ -99,7 +99,7 @@ int check_kvrows(const mla_m4_tensor * x, const mla_m4_tensor * nw, const mla_m4
         !std::isfinite(rp->freq_base) || !std::isfinite(rp->freq_scale) || !std::isfinite(rp->eps) ||
         !std::isfinite(rp->ext_factor) || !std::isfinite(rp->attn_factor) || !(rp->beta_fast > 0.0f) || !(rp->beta_slow > 0.0f))
         return MLA_M4_ERR_ARG;
-    if (n_out > 1024 || n_dims > pg::MAX_ROPE || n_rows > INT32_MAX / 4) return MLA_M4_ERR_UNSUPPORTED;
+    if (n_out > 1024 || n_dims > pg::MAX_ROPE || n_rows > pg::MAX_KV_ROWS) return MLA_M4_ERR_UNSUPPORTED;
     return MLA_M4_OK;
 }
 
@@ -220,12 +220,12 @@ int mla_m4_supports_kvrows(const mla_m4_tensor * x, const mla_m4_tensor * kv_nor
 }
 
 size_t mla_m4_kqkv_paged_workspace_bytes(const mla_m4_tensor * kcache, const mla_m4_tensor * q, const mla_m4_tensor * past,
-                                         const mla_m4_tensor * dst) {
+                                         const mla_m4_tensor * prefix, const mla_m4_tensor * dst) {
     if (!kcache || !q || !past || !dst || q->ne[1] < 1 || q->ne[1] > 1024 || q->ne[2] < 1 || q->ne[2] > pg::MAX_ROWS ||
         past->ne[0] < 1 || past->ne[0] > pg::MAX_SEQS || kcache->ne[0] > 4096 || dst->ne[0] > 4096 ||
         !pg::attn_supported((int)kcache->ne[0], (int)dst->ne[0]))
         return 0;
-    return pg::attn_workspace_bytes((int)kcache->ne[0], (int)dst->ne[0], (int)past->ne[0], (int)q->ne[1], (int)q->ne[2]);
+    return pg::attn_workspace_bytes((int)dst->ne[0], (int)past->ne[0], (int)q->ne[1], (int)q->ne[2], prefix && prefix->data);
 }
 
 int mla_m4_kqkv_paged(const mla_m4_tensor * kcache, const mla_m4_tensor * q, const mla_m4_tensor * past,
@@ -235,7 +235,7 @@ int mla_m4_kqkv_paged(const mla_m4_tensor * kcache, const mla_m4_tensor * q, con
     const int rc = check_attn(kcache, q, past, n_new, table, page_size, prefix, dst);
     if (rc != MLA_M4_OK) return rc;
     if (!std::isfinite(kq_scale)) return MLA_M4_ERR_ARG;
-    const size_t need = mla_m4_kqkv_paged_workspace_bytes(kcache, q, past, dst);
+    const size_t need = mla_m4_kqkv_paged_workspace_bytes(kcache, q, past, prefix, dst);
     if (need > 0 && (!workspace || !aligned16(workspace) || workspace_bytes < need)) return MLA_M4_ERR_WORKSPACE;
     pg::AttnArgs a{};
     a.kc = static_cast<const char *>(kcache->data);

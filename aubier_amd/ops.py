@@ -110,7 +110,7 @@ _EXPORTS = {
     "mla_m4_supports_kvrows": (ctypes.c_int, [ctypes.c_void_p] * 7),
     "mla_m4_kqkv_paged": (ctypes.c_int, [ctypes.c_void_p] * 5 + [ctypes.c_int32, ctypes.c_void_p, ctypes.c_float, ctypes.c_void_p,
                                                                  ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]),
-    "mla_m4_kqkv_paged_workspace_bytes": (ctypes.c_size_t, [ctypes.c_void_p] * 4),
+    "mla_m4_kqkv_paged_workspace_bytes": (ctypes.c_size_t, [ctypes.c_void_p] * 5),
     "mla_m4_supports_kqkv_paged": (ctypes.c_int, [ctypes.c_void_p] * 5 + [ctypes.c_int32] + [ctypes.c_void_p] * 2),
 }
 
@@ -512,8 +512,10 @@ def ggml_m4_kvrows(x: torch.Tensor, kv_norm: torch.Tensor, kcache, slot: torch.T
     return out
 
 
-def kqkv_paged_workspace_bytes(kcache, q: torch.Tensor, past: torch.Tensor, out: torch.Tensor) -> int:
-    return int(load_library().mla_m4_kqkv_paged_workspace_bytes(_ptr(view(kcache)), _ptr(view(q)), _ptr(view(past)), _ptr(view(out))))
+def kqkv_paged_workspace_bytes(kcache, q: torch.Tensor, past: torch.Tensor, out: torch.Tensor,
+                               prefix: Optional[torch.Tensor] = None) -> int:
+    return int(load_library().mla_m4_kqkv_paged_workspace_bytes(_ptr(view(kcache)), _ptr(view(q)), _ptr(view(past)), _ptr(view(prefix)),
+                                                                _ptr(view(out))))
 
 
 def ggml_m4_kqkv_paged(kcache, q: torch.Tensor, past: torch.Tensor, n_new: torch.Tensor, table: torch.Tensor, page_size: int,
@@ -529,7 +531,7 @@ def ggml_m4_kqkv_paged(kcache, q: torch.Tensor, past: torch.Tensor, n_new: torch
         out = torch.empty((q.shape[1], q.shape[0], _dv_of(kcache)), dtype=q.dtype, device=q.device)
     (vk, vq, vp, vn, vt, vf, vo), gpu = _descriptors("ggml_m4_kqkv_paged", (kcache, q, past, n_new, table, prefix, out))
     if workspace is None:
-        need = lib.mla_m4_kqkv_paged_workspace_bytes(vk, vq, vp, vo)
+        need = lib.mla_m4_kqkv_paged_workspace_bytes(vk, vq, vp, vf, vo)
         workspace = torch.empty(need, dtype=torch.uint8, device=q.device) if need > 0 else None
     elif workspace.get_device() != gpu:
         raise MlaM4Error("ggml_m4_kqkv_paged", -5)

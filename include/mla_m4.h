@@ -302,7 +302,7 @@ int mla_m4_pages(const mla_m4_tensor * past, const mla_m4_tensor * n_new, const 
  * mode with YaRN, as phase 0, the angles taken in 64 bits.  The row goes to cache row slot, rounded as
  * phase 0 does (f16, or ggml's f32 -> q8_0); a slot outside [0, n_cells) stores nothing.  Kcur is
  * written for every row.  Slots are distinct: of two rows with one slot, either's values may end up
- * there.  d_lat and n_dims multiples of 32, n_dims <= 256, d_lat + n_dims <= 1024. */
+ * there.  d_lat and n_dims multiples of 32, n_dims <= 256, d_lat + n_dims <= 1024, n_rows <= 2^24. */
 int mla_m4_kvrows(const mla_m4_tensor * x, const mla_m4_tensor * kv_norm, const mla_m4_tensor * kcache,
                   const mla_m4_tensor * slot, const mla_m4_tensor * pos, const mla_m4_rope_params * rope,
                   const mla_m4_tensor * dst, void * stream);
@@ -331,8 +331,11 @@ int mla_m4_kqkv_paged(const mla_m4_tensor * kcache, const mla_m4_tensor * q, con
                       const mla_m4_tensor * n_new, const mla_m4_tensor * table, int32_t page_size,
                       const mla_m4_tensor * prefix, float kq_scale, const mla_m4_tensor * dst,
                       void * workspace, size_t workspace_bytes, void * stream);
+/* About 68 MB at D_v 512 and 34 at 256; with a prefix half as much again, 4 D_v bytes for every (token, head)
+ * row and 260 D_v for every request. */
 size_t mla_m4_kqkv_paged_workspace_bytes(const mla_m4_tensor * kcache, const mla_m4_tensor * q,
-                                         const mla_m4_tensor * past, const mla_m4_tensor * dst);
+                                         const mla_m4_tensor * past, const mla_m4_tensor * prefix,
+                                         const mla_m4_tensor * dst);
 
 /* their supports_op mirrors, as below */
 int mla_m4_supports_pages(const mla_m4_tensor * past, const mla_m4_tensor * n_new, const mla_m4_tensor * free_ids,

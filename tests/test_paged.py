@@ -59,6 +59,27 @@ def test_supports_kvrows():
         assert not rows(**bad), bad
 
 
+def test_supports_kvrows_row_limit():
+    for n, ok in ((1 << 24, True), ((1 << 24) + 1, False)):
+        # (nothing is read: the pages of these are never touched)
+        assert ok == rows(x=torch.empty((n, 64), dtype=torch.float16), kv_norm=torch.zeros(32), kcache=torch.zeros((20, 64), dtype=torch.float16),
+                          slot=torch.empty(n, dtype=torch.int64), pos=torch.empty(n, dtype=torch.int32), out=None,
+                          rope=A.rope_params(n_dims=32, **RP))
+
+
+def test_attention_workspace_stays_bounded():
+    """Without shared cells the records number two per workgroup whatever the batch; what grows is 8 bytes a row."""
+    kc, lens = torch.zeros((64, 576), dtype=torch.float16), i32(64)
+    need = {}
+    for nt in (1, 8000):
+        for prefix in (None, i32(2)):
+            q, out = torch.empty((nt, 16, 576), dtype=torch.float16), torch.empty((16, nt, 512), dtype=torch.float16)
+            need[nt, prefix is not None] = A.kqkv_paged_workspace_bytes(kc, q, lens, out, prefix)
+    record = 128 * (8 + 2 * 512)
+    assert 512 * record <= need[1, False] <= need[8000, False] <= 512 * record + 9 * 16 * 8000
+    assert need[8000, False] + 2 * 1000 * record <= need[8000, True] <= need[8000, False] + (256 + 2 * 1000 + 64) * record
+
+
 def attn(dk=576, dv=512, **kw):
     a = dict(kcache=torch.zeros((640, dk), dtype=torch.float16), q=torch.zeros((3, 8, dk), dtype=torch.float16), past=i32(2), n_new=i32(2),
              table=i32(2, 9), page_size=64, prefix=None, out=torch.zeros((8, 3, dv)))

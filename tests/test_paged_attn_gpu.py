@@ -212,7 +212,7 @@ def test_largest_offsets(dev):
 def test_captured_step_replays_with_new_lengths(dev):
     b = Batch(dev, [700, 130, 260, 64], [1, 2, 1, 1], 16, dk=320, prefix=64, share=4, seed=14, pad=2, poison=1.0)
     out = b.out()
-    ws = torch.empty(max(16, A.kqkv_paged_workspace_bytes(b.kc, b.q, b.past, out)), dtype=torch.uint8, device=dev)
+    ws = torch.empty(max(16, A.kqkv_paged_workspace_bytes(b.kc, b.q, b.past, out, b.prefix)), dtype=torch.uint8, device=dev)
     side = torch.cuda.Stream()
     with torch.cuda.stream(side):
         b.run(out, workspace=ws)
@@ -292,7 +292,7 @@ def test_workspace(dev, dk, H, past, new, prefix, share, cache):
     """What the workspace holds at the start does not matter, nothing behind it (or behind dst) is written, and a byte
     less is refused."""
     b = Batch(dev, past, new, 16, dk=dk, H=H, cache=cache, prefix=prefix, share=share, pad=2, seed=31)
-    need = A.kqkv_paged_workspace_bytes(b.kc, b.q, b.past, b.out())
+    need = A.kqkv_paged_workspace_bytes(b.kc, b.q, b.past, b.out(), b.prefix)
     big = torch.empty(need + (1 << 20), dtype=torch.uint8, device=dev)
     got = []
     for fill in (0, 255, 127):
