@@ -18,7 +18,7 @@
 // nothing shared, goes straight to dst; the other pieces leave records, which the second launch merges.  Groups of
 // rows that share cells come first on the line and always leave records: piece of group g in workgroup i has record
 // i + g, as along the line one of the two grows from piece to piece.  Of the other groups a workgroup holds at most two
-// in part, one that began before it and one that goes on behind it: records 2 i and 2 i + 1.
+// in part: one that goes on behind it has record i, one that began before it record N + i.
 //
 // All positions on the line are computed by the same expressions in every workgroup (in 64-bit floating point, exact
 // for whole numbers below 2^53), so the workgroups agree where one ends and the next begins.
@@ -202,9 +202,11 @@ __device__ __forceinline__ Walk find_place(const AttnArgs & a, PlaceLds & sh) {
     }
     base += shared_cost;
     k.all += shared_cost;
-    // at most one workgroup per tile
+    // Where there are fewer tiles than workgroups two workgroups per tile: a stretch is then shorter than a tile, so none
+    // takes two, nor a tile behind another group's start (200 tokens of one prompt: one per tile 39 us, two 30; a
+    // decode over 200 cells 13.8 and 12.4; three and more do not gain, fewer pieces lose 2 us for each tile more in a row)
     const int64_t tiles = (int64_t)(all_groups >> 32) + (int64_t)k.shared_blocks() * (k.shared_keys / TK);
-    k.n_wg = uni((int)min(max(tiles, (int64_t)1), (int64_t)gridDim.x));
+    k.n_wg = uni((int)min(max(2 * tiles, (int64_t)1), (int64_t)gridDim.x));
     k.per = k.all / (double)k.n_wg;
     k.x0 = k.edge(wg);
     k.x1 = k.edge(wg + 1);
@@ -322,7 +324,7 @@ __global__ __launch_bounds__(NTHR, 1) void kqkv_paged_kernel(AttnArgs a) {
             p.ta = uni(tile_at(k.x0));
             p.tb = uni(tile_at(k.x1));
             first = uni(g0 >= k.x0);                     // the group's first piece says how many there are
-            p.slot = direct ? -1 : uni(b < k.n_share ? SHARED_RECORDS + wg + k.g : 2 * wg + (first ? 1 : 0));
+            p.slot = direct ? -1 : uni((b < k.n_share ? SHARED_RECORDS + k.g : first ? 0 : N_WG) + wg);
             if (first && !direct) {
                 int e = min(max((int)(g1 / k.per), wg + 1), k.n_wg);
                 while (e > wg + 1 && k.edge(e - 1) >= g1) --e;
@@ -389,7 +391,7 @@ struct RowPieces {
     __device__ __forceinline__ const char * at(const char * records, int q, int & r) const {
         const bool mine = q < n_own;
         r = mine ? r_own : r_shared;
-        const int of_own = shares ? own + q : own + max(2 * q - 1, 0);
+        const int of_own = own + q + (q > 0 && !shares ? N_WG : 0);
         return records + (size_t)(mine ? of_own : shared + q - n_own) * record_bytes<DV>();
     }
 };
@@ -577,7 +579,11 @@ static hipError_t launch(bool q8, const AttnArgs & a, hipStream_t stream) {
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     const int rows = a.n_head * a.nt;
-    if (rows <= 512) hipLaunchKernelGGL((kqkv_paged_merge_few_kernel<DV, DV / 64>), dim3(rows, DV / 64), dim3(NTHR), 0, stream, a);
+    // The card starts some 400 workgroups per us: as many as take part at once, no more (512 rows, 16 requests of 10,000
+    // to 20,000: eight workgroups a row 65 us, one 55; 64 rows: eight 89.4, four 87.0; 32 rows with 256 pieces each: one
+    // 48, two 36, four 31).  Past 1,536 rows a wavefront each (1,024 rows: 20.3, a workgroup each 19.4; 2,048: 19 and 25).
+    if (rows <= 64) hipLaunchKernelGGL((kqkv_paged_merge_few_kernel<DV, 4>), dim3(rows, 4), dim3(NTHR), 0, stream, a);
+    else if (rows <= 128) hipLaunchKernelGGL((kqkv_paged_merge_few_kernel<DV, 2>), dim3(rows, 2), dim3(NTHR), 0, stream, a);
     else if (rows <= 1536) hipLaunchKernelGGL((kqkv_paged_merge_few_kernel<DV, 1>), dim3(rows), dim3(NTHR), 0, stream, a);
     else hipLaunchKernelGGL(kqkv_paged_merge_kernel<DV>, dim3(rows < 4 * 2048 ? (rows + 3) / 4 : 2048), dim3(NTHR), 0, stream, a);
     return hipGetLastError();
