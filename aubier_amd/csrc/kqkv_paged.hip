@@ -375,14 +375,15 @@ struct RowPieces {
     int n, n_own, own, shared, r_own, r_shared;
     bool shares;
     __device__ __forceinline__ RowPieces(const AttnArgs & a, const Head & head, int row) {
-        // (both read at once, whatever the row: the shared block's entry lies in the workspace also where there is none)
-        const Pieces o = reinterpret_cast<const Pieces *>(a.work + own_off(a.n_head, a.nt))[row];
-        const Pieces s = reinterpret_cast<const Pieces *>(a.work + shared_off())[row / BLOCK_ROWS];
+        // (both read at once, whatever the row: the entries lie in the workspace also where there is no such row)
+        const int at = min(row, a.n_head * a.nt - 1);
+        const Pieces o = reinterpret_cast<const Pieces *>(a.work + own_off(a.n_head, a.nt))[at];
+        const Pieces s = reinterpret_cast<const Pieces *>(a.work + shared_off())[at / BLOCK_ROWS];
         n_own = row < head.rows ? (int)(o.n_row & 0xffffu) : 0;
         r_own = (int)(o.n_row >> 16);
         own = o.slot;
         shared = s.slot;
-        r_shared = row % BLOCK_ROWS;
+        r_shared = at % BLOCK_ROWS;
         shares = row < head.shared_rows;
         n = n_own + (shares ? (int)s.n_row : 0);
     }
@@ -396,15 +397,16 @@ struct RowPieces {
     }
 };
 
-// (m, l, o) of some pieces, eight columns per lane
+// (m, l, o) of some pieces of a lane's row: eight columns of each of S slabs
+template <int DV, int S>
 struct Part {
-    float m = -INFINITY, l = 0.0f, o[8] = {};
-    // pieces q0, q0 + step, .. below n
-    template <int DV, int U>
-    __device__ __forceinline__ void add(const RowPieces & rp, const char * records, int q0, int step, int col) {
+    float m = -INFINITY, l = 0.0f, o[S][8] = {};
+    // pieces q0, q0 + step, .. below n, slabs s0 ..
+    template <int U>
+    __device__ __forceinline__ void add(const RowPieces & rp, const char * records, int q0, int step, int s0, int hi) {
         for (; q0 < rp.n; q0 += step * U) {
             float ms[U], ls[U];
-            half8 os[U];
+            half8 os[U][S];
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 const int q = q0 + step * u;
@@ -413,15 +415,14 @@ struct Part {
                 const f32x2 ml = reinterpret_cast<const f32x2 *>(rec)[r];
                 ms[u] = q < rp.n ? ml[0] : -INFINITY;
                 ls[u] = q < rp.n ? ml[1] : 0.0f;
-                os[u] = *reinterpret_cast<const half8 *>(rec + BLOCK_ROWS * 8 + ((size_t)r * DV + col) * 2);
+                const char * at = rec + BLOCK_ROWS * 8 + (size_t)((r >> 5) * (DV / 16) + s0) * 1024 + 512 * hi + 16 * (r & 31);
+#pragma unroll
+                for (int s = 0; s < S; ++s) os[u][s] = *reinterpret_cast<const half8 *>(at + 1024 * s);
             }
             float mx = m;
 #pragma unroll
             for (int u = 0; u < U; ++u) mx = fmaxf(mx, ms[u]);
-            const float f0 = exp2_unless(m == -INFINITY, m - mx);
-            l *= f0;
-#pragma unroll
-            for (int k = 0; k < 8; ++k) o[k] *= f0;
+            scale(exp2_unless(m == -INFINITY, m - mx));
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 // without a finite score l is 0, or NaN where every score was; o then holds nothing (an empty piece's
@@ -430,130 +431,122 @@ struct Part {
                 const float f = none ? ls[u] : ls[u] * exp2_fast(ms[u] - mx);
                 l += f;
 #pragma unroll
-                for (int k = 0; k < 8; ++k) o[k] += none ? f : f * (float)os[u][k];
+                for (int s = 0; s < S; ++s)
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) o[s][k] += none ? f : f * (float)os[u][s][k];
             }
             m = mx;
         }
     }
-    __device__ __forceinline__ void add(float m2, float l2, const float (&o2)[8]) {
-        const float mx = fmaxf(m, m2);
-        // (without a finite score: l and o are 0 or NaN)
-        const float f = m == -INFINITY ? 1.0f : exp2_fast(m - mx), f2 = m2 == -INFINITY ? 1.0f : exp2_fast(m2 - mx);
-        l = l * f + l2 * f2;
+    __device__ __forceinline__ void scale(float f) {
+        l *= f;
 #pragma unroll
-        for (int k = 0; k < 8; ++k) o[k] = o[k] * f + o2[k] * f2;
-        m = mx;
+        for (int s = 0; s < S; ++s)
+#pragma unroll
+            for (int k = 0; k < 8; ++k) o[s][k] *= f;
     }
-    template <int DV>
-    __device__ __forceinline__ void out(const AttnArgs & a, int row, int col) const {
+    __device__ __forceinline__ void out(const AttnArgs & a, int row, int s0, int hi) const {
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;
         const int t = row / a.n_head, h = row - t * a.n_head;
-        const size_t at = ((size_t)h * a.nt + t) * DV + col;
-        if (a.dst_f16) {
-            half8 v;
+        const size_t at = ((size_t)h * a.nt + t) * DV + 16 * s0 + 8 * hi;
 #pragma unroll
-            for (int k = 0; k < 8; ++k) v[k] = to_half(o[k] * inv);
-            *reinterpret_cast<half8 *>(a.dst + at * 2) = v;
-        } else {
-            f32x4 v[2];
+        for (int s = 0; s < S; ++s) {
+            if (a.dst_f16) {
+                half8 v;
 #pragma unroll
-            for (int k = 0; k < 8; ++k) v[k >> 2][k & 3] = o[k] * inv;
-            *reinterpret_cast<f32x4 *>(a.dst + at * 4) = v[0];
-            *reinterpret_cast<f32x4 *>(a.dst + at * 4 + 16) = v[1];
+                for (int k = 0; k < 8; ++k) v[k] = to_half(o[s][k] * inv);
+                *reinterpret_cast<half8 *>(a.dst + (at + 16 * s) * 2) = v;
+            } else {
+                f32x4 v[2];
+#pragma unroll
+                for (int k = 0; k < 8; ++k) v[k >> 2][k & 3] = o[s][k] * inv;
+                *reinterpret_cast<f32x4 *>(a.dst + (at + 16 * s) * 4) = v[0];
+                *reinterpret_cast<f32x4 *>(a.dst + (at + 16 * s) * 4 + 16) = v[1];
+            }
         }
     }
 };
 
-// One row by a workgroup: DV / CB columns from c0 on, LP lanes a piece, 256 / LP pieces at a time
-template <int DV, int CB>
-struct RowLds {
-    static constexpr int LP = DV / CB / 8, PP = NTHR / LP;
-    float m[PP], l[PP];
-    f32x4 o[2][NTHR];
+// RW rows and one slab by a workgroup of NT: 2 RW lanes a part, the pieces dealt to the parts
+template <int NT>
+struct MergeLds {
+    float m[NT], l[NT];
+    f32x4 o[2][NT];
 };
-template <int DV, int CB>
-__device__ __forceinline__ void merge_by_workgroup(const AttnArgs & a, const RowPieces & rp, const char * records, int row, int c0,
-                                                   RowLds<DV, CB> & sh) {
-    using R = RowLds<DV, CB>;
-    const int tid = threadIdx.x, c = tid % R::LP, pi = tid / R::LP;
-    Part p;
-    p.template add<DV, 4>(rp, records, pi, R::PP, c0 + 8 * c);
-    if (c == 0) {
-        sh.m[pi] = p.m;
-        sh.l[pi] = p.l;
-    }
-    sh.o[0][tid] = f32x4{p.o[0], p.o[1], p.o[2], p.o[3]};
-    sh.o[1][tid] = f32x4{p.o[4], p.o[5], p.o[6], p.o[7]};
-    __syncthreads();
-    if (pi == 0) {
-        for (int i = 1; i < R::PP; ++i) {
-            const f32x4 x = sh.o[0][i * R::LP + c], y = sh.o[1][i * R::LP + c];
-            const float o2[8] = {x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
-            p.add(sh.m[i], sh.l[i], o2);
+template <int DV, int NT, int RW>
+__device__ __forceinline__ void merge_together(const AttnArgs & a, const RowPieces & rp, const char * records, int row, int slab, MergeLds<NT> & sh) {
+    constexpr int LP = 2 * RW;
+    const int tid = threadIdx.x, hi = tid / RW & 1, part = tid / LP;
+    Part<DV, 1> p;
+    p.template add<4>(rp, records, part, NT / LP, slab, hi);
+    auto put = [&]() {
+        sh.m[tid] = p.m;
+        sh.l[tid] = p.l;
+        sh.o[0][tid] = f32x4{p.o[0][0], p.o[0][1], p.o[0][2], p.o[0][3]};
+        sh.o[1][tid] = f32x4{p.o[0][4], p.o[0][5], p.o[0][6], p.o[0][7]};
+    };
+    auto get = [&](int at) {
+        const float m2 = sh.m[at], l2 = sh.l[at], mx = fmaxf(p.m, m2);
+        const f32x4 x = sh.o[0][at], y = sh.o[1][at];
+        // (without a finite score: l and o are 0 or NaN)
+        p.scale(p.m == -INFINITY ? 1.0f : exp2_fast(p.m - mx));
+        const float f2 = m2 == -INFINITY ? 1.0f : exp2_fast(m2 - mx);
+        p.l += l2 * f2;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            p.o[0][k] += x[k] * f2;
+            p.o[0][4 + k] += y[k] * f2;
         }
-        p.template out<DV>(a, row, c0 + 8 * c);
+        p.m = mx;
+    };
+    // four parts into one, until one is left
+#pragma unroll
+    for (int n = NT / LP; n > 1;) {
+        const int f = n % 4 == 0 ? 4 : 2;
+        if (part < n) put();
+        __syncthreads();
+        n /= f;
+        if (part < n) {
+#pragma unroll
+            for (int i = 1; i < f; ++i) get(tid + i * n * LP);
+        }
+        if (n > 1) __syncthreads();
     }
+    if (part == 0 && rp.n > 0) p.out(a, row, slab, hi);
 }
 
-// Few rows: a workgroup per row and DV / CB columns, so that the whole card takes part
-template <int DV, int CB>
-__global__ __launch_bounds__(NTHR) void kqkv_paged_merge_few_kernel(AttnArgs a) {
-    __shared__ RowLds<DV, CB> sh;
+// Few rows: a workgroup per RW rows and slab
+template <int DV, int NT, int RW>
+__global__ __launch_bounds__(NT) void kqkv_paged_merge_few_kernel(AttnArgs a) {
+    __shared__ MergeLds<NT> sh;
     const Head head = *reinterpret_cast<const Head *>(a.work);
-    const RowPieces rp(a, head, blockIdx.x);
-    if (rp.n == 0) return;
-    merge_by_workgroup<DV, CB>(a, rp, a.work + records_off(a.n_head, a.nt), blockIdx.x, DV / CB * (int)blockIdx.y, sh);
+    const int row = RW * (int)blockIdx.x + (int)(threadIdx.x % RW);
+    const RowPieces rp(a, head, row);
+    if (__builtin_amdgcn_ballot_w64(rp.n > 0) == 0) return;      // (the same rows in every wavefront)
+    merge_together<DV, NT, RW>(a, rp, a.work + records_off(a.n_head, a.nt), row, blockIdx.y, sh);
 }
 
-// Many rows: a wavefront per row (D_v 256: half of one per piece, two pieces at a time), four rows a workgroup; a row
-// of many pieces (a long request among short ones) by the whole workgroup
+// Many rows: a wavefront per 32 rows and S slabs; rows of many pieces (a long request among short ones) by the whole
+// workgroup, slab by slab
 constexpr int MANY_PIECES = 24;
-template <int DV>
+template <int DV, int S>
 __global__ __launch_bounds__(NTHR) void kqkv_paged_merge_kernel(AttnArgs a) {
-    constexpr int LP = DV / 8, PW = 64 / LP;
-    __shared__ RowLds<DV, 1> sh;
+    __shared__ MergeLds<NTHR> sh;
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
     const Head head = *reinterpret_cast<const Head *>(a.work);
     const char * records = a.work + records_off(a.n_head, a.nt);
-    const int n_rows = a.n_head * a.nt;
-    for (int row0 = 4 * (int)blockIdx.x; row0 < head.rows; row0 += 4 * (int)gridDim.x) {
-        const int row = min(row0 + w, n_rows - 1);
-        const RowPieces rp(a, head, row);
-        const bool mine = row0 + w < head.rows;
-        if (lane == 0) sh.l[w] = mine ? (float)rp.n : 0.0f;
-        if (mine && rp.n > 0 && rp.n <= MANY_PIECES) {
-            const int col = 8 * (lane % LP);
-            Part p;
-            if (rp.n <= 2 * PW) p.template add<DV, 2>(rp, records, lane / LP, PW, col);      // a chunk's rows
-            else p.template add<DV, 4>(rp, records, lane / LP, PW, col);
-            if constexpr (PW == 2) {
-                Part q;                                  // the other half's
-                float lo, up;
-                halves_pair(p.m, lo, up);
-                q.m = up;
-                p.m = lo;
-                halves_pair(p.l, lo, up);
-                q.l = up;
-                p.l = lo;
-#pragma unroll
-                for (int k = 0; k < 8; ++k) {
-                    halves_pair(p.o[k], lo, up);
-                    q.o[k] = up;
-                    p.o[k] = lo;
-                }
-                p.add(q.m, q.l, q.o);
-            }
-            if (lane < LP) p.template out<DV>(a, row, col);
-        }
-        __syncthreads();
-        float n[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) n[i] = sh.l[i];
-        __syncthreads();
+    const int row = 32 * (int)blockIdx.x + (lane & 31), s0 = 4 * S * (int)blockIdx.y;
+    const RowPieces rp(a, head, row);
+    if (__builtin_amdgcn_ballot_w64(rp.n > 0) == 0) return;
+    if (__builtin_amdgcn_ballot_w64(rp.n > MANY_PIECES) == 0) {
+        Part<DV, S> p;
+        if (__builtin_amdgcn_ballot_w64(rp.n > 2) == 0) p.template add<2>(rp, records, 0, 1, s0 + S * w, lane >> 5);     // a chunk's rows
+        else p.template add<4>(rp, records, 0, 1, s0 + S * w, lane >> 5);
+        if (rp.n > 0) p.out(a, row, s0 + S * w, lane >> 5);
+    } else {
 #pragma unroll 1
-        for (int i = 0; i < 4; ++i) {
-            if (n[i] <= (float)MANY_PIECES) continue;
-            merge_by_workgroup<DV, 1>(a, RowPieces(a, head, row0 + i), records, row0 + i, 0, sh);
+        for (int s = 0; s < 4 * S; ++s) {
+            merge_together<DV, NTHR, 32>(a, rp, records, row, s0 + s, sh);
             __syncthreads();
         }
     }
@@ -579,13 +572,15 @@ static hipError_t launch(bool q8, const AttnArgs & a, hipStream_t stream) {
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     const int rows = a.n_head * a.nt;
-    // The card starts some 400 workgroups per us: as many as take part at once, no more (512 rows, 16 requests of 10,000
-    // to 20,000: eight workgroups a row 65 us, one 55; 64 rows: eight 89.4, four 87.0; 32 rows with 256 pieces each: one
-    // 48, two 36, four 31).  Past 1,536 rows a wavefront each (1,024 rows: 20.3, a workgroup each 19.4; 2,048: 19 and 25).
-    if (rows <= 64) hipLaunchKernelGGL((kqkv_paged_merge_few_kernel<DV, 4>), dim3(rows, 4), dim3(NTHR), 0, stream, a);
-    else if (rows <= 128) hipLaunchKernelGGL((kqkv_paged_merge_few_kernel<DV, 2>), dim3(rows, 2), dim3(NTHR), 0, stream, a);
-    else if (rows <= 1536) hipLaunchKernelGGL((kqkv_paged_merge_few_kernel<DV, 1>), dim3(rows), dim3(NTHR), 0, stream, a);
-    else hipLaunchKernelGGL(kqkv_paged_merge_kernel<DV>, dim3(rows < 4 * 2048 ? (rows + 3) / 4 : 2048), dim3(NTHR), 0, stream, a);
+    // The card starts some 400 workgroups per us, so as many as take part at once, no more; the fewer rows, the more
+    // pieces each has.  Device times of whole calls either side of a limit, the smaller form first: 96 rows 19.2, 21.9 us
+    // and 192 rows 38.7, 41.1; 1,024 rows 51.7, 57.0 and 1,536 44.4, 45.4, but 2,048 71.7, 69.9; 2,048 rows 69.5, 79.4,
+    // 6,400 28.8, 28.9, 32,000 78.4, 77.2.
+    const auto wgs = [=](int r) { return dim3((rows + r - 1) / r, DV / 16); };
+    if (rows <= 256) hipLaunchKernelGGL((kqkv_paged_merge_few_kernel<DV, 512, 8>), wgs(8), dim3(512), 0, stream, a);
+    else if (rows <= 1536) hipLaunchKernelGGL((kqkv_paged_merge_few_kernel<DV, NTHR, 32>), wgs(32), dim3(NTHR), 0, stream, a);
+    else if (rows <= 4096) hipLaunchKernelGGL((kqkv_paged_merge_kernel<DV, 1>), dim3(wgs(32).x, DV / 64), dim3(NTHR), 0, stream, a);
+    else hipLaunchKernelGGL((kqkv_paged_merge_kernel<DV, 4>), dim3(wgs(32).x, DV / 256), dim3(NTHR), 0, stream, a);
     return hipGetLastError();
 }
 

@@ -30,6 +30,8 @@ __device__ __forceinline__ void page_dma16(i32x4 rsrc, uint32_t voff, uint32_t s
 
 constexpr int BLOCK_ROWS = 128;             // rows of the wide form
 
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+
 // Where the keys of a piece are and which of its rows sees which (uniform over the workgroup)
 struct Piece {
     int row0, rows;         // its rows: flat rows row0 .. row0 + rows - 1 of the tokens from tok0 on
@@ -43,7 +45,9 @@ struct Piece {
 };
 
 // Records: (m, l) of the block's 128 rows, m in log2 units (a reference for the scores, at most 15 below their
-// maximum; -inf: no key), then o / l in f16, D_v per row.
+// maximum; -inf: no key), then o / l in f16 as the accumulators' lanes hold it, so that neither side needs LDS: for every
+// 32 rows D_v / 16 slabs of 1 KB, slab s holding columns 16 s .. + 15, lane l's 8 of them (of row l & 31, the upper 8 in
+// the upper half) at 16 l.
 template <int DV>
 constexpr size_t record_bytes() { return BLOCK_ROWS * 8 + (size_t)BLOCK_ROWS * DV * 2; }
 
@@ -181,28 +185,38 @@ __device__ __forceinline__ void clear_nonfinite(char * sb, int lane, uint64_t & 
     }
 }
 
-// o / l of 32 rows (row0 .. of the block) to the record or, complete, to dst, in f16 through LDS rows of PITCH bytes
-// at stg: columns c0 .. c0 + NC - 1, whole 16-byte chunks, whole lines per instruction
-template <int DV, int NC, int PITCH>
-__device__ __forceinline__ void rows_out_f16(const AttnArgs & a, const Piece & p, char * rec, const char * stg, int row0, int c0,
-                                             const int * drow, int lane) {
-    constexpr int CPR = NC / 8, RPI = 64 / CPR;         // chunks per row, rows per round of the wavefront
-    static_assert(64 % CPR == 0, "whole rows");
-    const int r = lane / CPR, ch = lane % CPR;
-    stg += r * PITCH + 16 * ch;
-    if (p.slot >= 0) {
-        char * to = rec + BLOCK_ROWS * 8 + ((size_t)(row0 + r) * DV + c0 + 8 * ch) * 2;
-#pragma unroll 8
-        for (int it = 0; it < HG / RPI; ++it, to += RPI * DV * 2, stg += RPI * PITCH)
-            __builtin_nontemporal_store(*reinterpret_cast<const u32x4 *>(stg), reinterpret_cast<u32x4 *>(to));
-    } else {
-        drow += row0 + r;
-#pragma unroll 4
-        for (int it = 0; it < HG / RPI; ++it, stg += RPI * PITCH) {
-            const u32x4 v = *reinterpret_cast<const u32x4 *>(stg);
-            const int dr = drow[RPI * it];
-            if (dr >= 0) *reinterpret_cast<u32x4 *>(a.dst + ((size_t)dr * DV + c0 + 8 * ch) * 2) = v;
+// o / l of 32 rows (rg-th of the block), columns c0 .. c0 + 32 N - 1, in f16 to the record, or, complete, to dst: the
+// halves swap four columns, so that every lane has eight in a row
+template <int DV, int N>
+__device__ __forceinline__ void rows_out_f16(const AttnArgs & a, const Piece & p, const f32x16 (&o)[N], float inv, char * rec, int rg, int c0,
+                                             int dr, int lane) {
+    auto chunk = [&](int i, int qp) {
+        u32x2 x[2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const int e = 8 * qp + 4 * j;
+            x[j] = __builtin_bit_cast(u32x2, half4{to_half(o[i][e] * inv), to_half(o[i][e + 1] * inv), to_half(o[i][e + 2] * inv),
+                                                   to_half(o[i][e + 3] * inv)});
         }
+        const auto s0 = __builtin_amdgcn_permlane32_swap(x[0][0], x[1][0], false, false);
+        const auto s1 = __builtin_amdgcn_permlane32_swap(x[0][1], x[1][1], false, false);
+        return u32x4{s0[0], s1[0], s0[1], s1[1]};
+    };
+    if (p.slot >= 0) {
+        char * to = rec + BLOCK_ROWS * 8 + (size_t)(rg * (DV / 16) + c0 / 16) * 1024 + 16 * lane;
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+#pragma unroll
+            for (int qp = 0; qp < 2; ++qp) __builtin_nontemporal_store(chunk(i, qp), reinterpret_cast<u32x4 *>(to + 1024 * (2 * i + qp)));
+    } else {
+        char * to = a.dst + ((size_t)max(dr, 0) * DV + c0 + 8 * (lane >> 5)) * 2;
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+#pragma unroll
+            for (int qp = 0; qp < 2; ++qp) {
+                const u32x4 v = chunk(i, qp);
+                if (dr >= 0) *reinterpret_cast<u32x4 *>(to + 32 * (2 * i + qp)) = v;
+            }
     }
 }
 
@@ -428,18 +442,7 @@ __device__ __forceinline__ void narrow_piece(const AttnArgs & a, const Piece & p
         const float mr = m_ref[(lane_e >> 4) & 1];
         reinterpret_cast<f32x2 *>(rec)[lane_e] = f32x2{mr == M_NONE ? -INFINITY : mr, l};
     }
-    // staging that no other wave reads: this wave's slot of the stage the last tile did not use, or its int8 slot
-    char * stg = Q8 ? sh.ring + w * L::SLOT8 : sh.ring + ((n_my & 1) * NWAVE + w) * G::STAGE;
-    static_assert(!Q8 || HG * C::OPITCH <= L::SLOT8, "the staging fits an int8 slot");
-#pragma unroll
-    for (int i = 0; i < C::NTQ; ++i)
-#pragma unroll
-        for (int q4 = 0; q4 < 4; ++q4) {
-            const half4 hv = {to_half(o[i][4 * q4] * inv), to_half(o[i][4 * q4 + 1] * inv), to_half(o[i][4 * q4 + 2] * inv),
-                              to_half(o[i][4 * q4 + 3] * inv)};
-            *reinterpret_cast<half4 *>(stg + hl * C::OPITCH + (32 * i + 8 * q4 + hi4) * 2) = hv;
-        }
-    rows_out_f16<DV, C::DVQ, C::OPITCH>(a, p, rec, stg, 0, C::DVQ * w, sh.drow, lane_e);
+    rows_out_f16<DV, C::NTQ>(a, p, o, inv, rec, 0, C::DVQ * w, sh.drow[hl], lane_e);
 }
 
 // ---------------------------------------------------------------- up to 128 rows
@@ -525,8 +528,6 @@ __device__ __forceinline__ void wide_piece(const AttnArgs & a, const Piece & p, 
     using S = PageStream<DK>;
     using L = PieceLds<DK, DV, Q8>;
     constexpr int NB = DV / 32;                         // 32-column o^T tiles per wave
-    constexpr int OPITCH = DV * 2 + 16;
-    static_assert(NWAVE * HG * OPITCH <= L::RING, "the output staging fits the ring");
     const int tid = opaque_tid(), lane = tid & 63;
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int hl = lane & 31, hi = lane >> 5;
@@ -718,8 +719,7 @@ __device__ __forceinline__ void wide_piece(const AttnArgs & a, const Piece & p, 
             }
         }
     }
-    wait_vm<0>();
-    __syncthreads();                                    // the ring becomes the output staging
+    wait_vm<0>();                                       // nothing of this wave may still target the ring
     if (!live_w) return;
     const int lane_e = opaque_tid() & 63, hle = lane_e & 31, hi4 = 4 * (lane_e >> 5);
     const float l = halves_sum(l_acc);
@@ -736,16 +736,7 @@ __device__ __forceinline__ void wide_piece(const AttnArgs & a, const Piece & p, 
     }
     if (p.slot >= 0 && lane_e < HG)
         reinterpret_cast<f32x2 *>(rec)[HG * w + lane_e] = f32x2{m_run == M_NONE ? -INFINITY : m_run, l};
-    char * stg = sh.ring + w * HG * OPITCH;
-#pragma unroll
-    for (int i = 0; i < NB; ++i)
-#pragma unroll
-        for (int q4 = 0; q4 < 4; ++q4) {
-            const half4 hv = {to_half(o[i][4 * q4] * inv), to_half(o[i][4 * q4 + 1] * inv), to_half(o[i][4 * q4 + 2] * inv),
-                              to_half(o[i][4 * q4 + 3] * inv)};
-            *reinterpret_cast<half4 *>(stg + hle * OPITCH + (32 * i + 8 * q4 + hi4) * 2) = hv;
-        }
-    rows_out_f16<DV, DV, OPITCH>(a, p, rec, stg, HG * w, 0, sh.drow, lane_e);
+    rows_out_f16<DV, NB>(a, p, o, inv, rec, w, 0, sh.drow[HG * w + hle], lane_e);
 }
 
 }  // namespace paged
