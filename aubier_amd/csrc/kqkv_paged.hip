@@ -30,7 +30,6 @@ namespace paged {
 namespace {
 
 constexpr int N_WG = 256;                   // one workgroup per CU
-constexpr int MIN_SHARED_TILES = 1;         // fewer shared tiles than this are left to the requests
 // Costs, in tenths of a wide tile (all of them times H, so that they are whole numbers): a tile for up to 128 rows and
 // for up to 32, and a piece's start and end (its rows in, its results out).
 template <int DK, bool Q8>
@@ -39,6 +38,18 @@ struct Cost {
     static constexpr int WIDE_TILE = 10, NARROW_TILE = Q8 ? (BIG ? 5 : 6) : BIG ? 6 : 7;
     static constexpr int WIDE_START = Q8 ? (BIG ? 22 : 20) : BIG ? 21 : 28, NARROW_START = Q8 ? (BIG ? 9 : 11) : BIG ? 11 : 16;
 };
+
+// Shared cells are taken once where that pays: where it saves every workgroup SHARE_GAIN, as it costs a wide piece more
+// with its records (7 us of the larger geometry).  A request that takes them by itself pays for a tile, which it then
+// finds in the caches: 5 with up to 32 rows, else 6 and one for every 32 rows of a block, so a block of 128 gains
+// nothing.  Device times, shared and not, 32 heads of one token, the larger geometry: 32 requests behind 1,024 cells
+// 26.7 and 21.1 us, behind 4,096 32.5 and 32.0, behind 16,384 60.2 and 75.7; 64 behind 4,096 44.1 and 49.3; 4 behind 16,384
+// 30.8 and 25.6.
+constexpr int SHARE_GAIN = 16;
+__device__ __forceinline__ int repeat_cost(int rows) {
+    const int part = rows % BLOCK_ROWS;
+    return rows <= HG ? (rows > 0 ? 5 : 0) : rows / BLOCK_ROWS * 10 + (part > 0 ? 6 + (part + 31) / 32 : 0);
+}
 
 // Workspace: a header, the pieces of every shared block and of every row, the records (those of whole groups, two per
 // workgroup, then those of the sharing rows' groups)
@@ -97,8 +108,8 @@ struct Request {
 // This workgroup's stretch and its first group (b = n_seq: none), from the lengths: two sums over the requests by the
 // whole workgroup, then the thread whose request holds the stretch's start says so.
 struct PlaceLds {
-    int rows[4], shared[4][4];              // per wavefront: rows; sharing requests' cells, number, rows, first
-    double cost[4];
+    int rows[4], shared[4][3];              // per wavefront: rows; sharing requests' cells, rows, first
+    double repeat[4], cost[4];
     uint64_t groups[4];
     double base;
     int b, tok0, g;
@@ -124,7 +135,8 @@ __device__ __forceinline__ Walk find_place(const AttnArgs & a, PlaceLds & sh) {
         return v;
     };
 
-    int own = 0, keys = min(max(k_pre, 0), k.cap), active = 0, srows = 0, by = MAX_SEQS;
+    int own = 0, keys = min(max(k_pre, 0), k.cap), srows = 0, by = MAX_SEQS;
+    double repeat = 0.0;
     for (int b = b0; b < b1; ++b) {
         const int n = min(max(n_of(b), 0), a.nt);
         own += n;
@@ -132,7 +144,7 @@ __device__ __forceinline__ Walk find_place(const AttnArgs & a, PlaceLds & sh) {
             keys = min(keys, clamp_past(past_of(b)));
             by = min(by, b);
             srows += n;
-            ++active;
+            repeat += (double)repeat_cost(n * H);
         }
     }
     const int incl = wave_scan(own);
@@ -140,13 +152,13 @@ __device__ __forceinline__ Walk find_place(const AttnArgs & a, PlaceLds & sh) {
     if (a.prefix != nullptr) {
         keys = wave_min(keys);
         by = wave_min(by);
-        active = wave_scan(active);
+        repeat = wave_scan(repeat);
         srows = wave_scan(srows);
         if (lane == 63) {
             sh.shared[w][0] = keys;
-            sh.shared[w][1] = active;
-            sh.shared[w][2] = srows;
-            sh.shared[w][3] = by;
+            sh.shared[w][1] = srows;
+            sh.shared[w][2] = by;
+            sh.repeat[w] = repeat;
         }
     }
     if (tid == 0) sh.b = a.n_seq;
@@ -161,12 +173,15 @@ __device__ __forceinline__ Walk find_place(const AttnArgs & a, PlaceLds & sh) {
     if (a.prefix != nullptr) {
         // as many whole tiles of shared cells as all sharing requests with tokens held before them
         keys = uni(min(min(sh.shared[0][0], sh.shared[1][0]), min(sh.shared[2][0], sh.shared[3][0])) / TK * TK);
-        active = uni(sh.shared[0][1] + sh.shared[1][1] + sh.shared[2][1] + sh.shared[3][1]);
-        if (active > 1 && keys >= MIN_SHARED_TILES * TK) {
+        k.shared_keys = keys;
+        k.shared_rows = uni(min(sh.shared[0][1] + sh.shared[1][1] + sh.shared[2][1] + sh.shared[3][1], a.nt) * H);
+        const double saved = (sh.repeat[0] + sh.repeat[1] + sh.repeat[2] + sh.repeat[3]) * (double)(keys / TK) * (double)H -
+                             (double)k.shared_blocks() * k.template shared_a<C>(H);
+        if (uni(saved > (double)(SHARE_GAIN * N_WG) * (double)H)) {
             k.n_share = n_pre;
-            k.shared_keys = keys;
-            k.shared_rows = uni(min(sh.shared[0][2] + sh.shared[1][2] + sh.shared[2][2] + sh.shared[3][2], a.nt) * H);
-            k.shared_by = uni(min(min(sh.shared[0][3], sh.shared[1][3]), min(sh.shared[2][3], sh.shared[3][3])));
+            k.shared_by = uni(min(min(sh.shared[0][2], sh.shared[1][2]), min(sh.shared[2][2], sh.shared[3][2])));
+        } else {
+            k.shared_keys = k.shared_rows = 0;
         }
     }
     const double shared_a = k.template shared_a<C>(H), shared_cost = (double)k.shared_blocks() * shared_a;

@@ -315,10 +315,11 @@ int mla_m4_kvrows(const mla_m4_tensor * x, const mla_m4_tensor * kv_norm, const 
  *   q       F32|F16 ne [D_k, H, nt] nb[0] = element size, 16-byte aligned strides, H <= 1024,
  *                                   H nb[1] + 127 nb[2] <= 2 GiB (128 rows of q are read by 32-bit offsets)
  *   prefix  I32 ne [2], or NULL     (cells, requests): the tables of the first `requests` requests begin
- *                                   with the same pages, for at least `cells` cells.  Those cells are
- *                                   then read and multiplied once for all of them, through the table of
- *                                   the first of them that has tokens.  Without it, or where one of them
- *                                   holds fewer cells, the result is the same up to rounding
+ *                                   with the same pages, for at least `cells` cells.  Where that is less
+ *                                   work (many requests of few rows, long prefixes) those cells are read
+ *                                   and multiplied once for all of them, through the table of the first
+ *                                   of them that has tokens.  The result is the same up to rounding, also
+ *                                   where one of them holds fewer cells
  *   dst     F32|F16 ne [D_v, nt, H] contiguous; rows of tokens behind the last request are not written
  * (D_k, D_v) = (576, 512) or (320, 256).  A page id outside the pool has no cells: the keys there are not
  * seen.  A token that sees no key gets zeros.  What lies in cells that no token of a request sees (the
