@@ -21,7 +21,7 @@
 // in part: one that goes on behind it has record i, one that began before it record N + i.
 //
 // All positions on the line are computed by the same expressions in every workgroup (in 64-bit floating point, exact
-// for whole numbers below 2^53), so the workgroups agree where one ends and the next begins.
+// for whole numbers below 2^53, which MAX_LINE keeps them), so the workgroups agree where one ends and the next begins.
 #include "paged_pass.h"
 
 namespace mla {
@@ -186,7 +186,8 @@ __device__ __forceinline__ Walk find_place(const AttnArgs & a, PlaceLds & sh) {
     }
     const double shared_a = k.template shared_a<C>(H), shared_cost = (double)k.shared_blocks() * shared_a;
 
-    // costs, and (tiles, groups) in the high and low half of a word
+    // costs, and (tiles, groups) in the high and low half of a word; of a request's tiles no more than N_WG each way count,
+    // as all that is asked is whether there are fewer than workgroups
     double cost = 0.0;
     uint64_t groups = 0;
     {
@@ -194,7 +195,7 @@ __device__ __forceinline__ Walk find_place(const AttnArgs & a, PlaceLds & sh) {
         for (int b = b0; b < b1; ++b) {
             const Request<C> rq(a, k, H, n_of(b), past_of(b), b, at);
             cost += rq.cost();
-            groups += (uint64_t)rq.blocks + ((uint64_t)(uint32_t)(rq.blocks * rq.first) << 32);
+            groups += (uint64_t)rq.blocks + ((uint64_t)(uint32_t)(min(rq.blocks, N_WG) * min(rq.first, N_WG)) << 32);
             at += rq.n;
         }
     }

@@ -150,6 +150,7 @@ int check_attn(const mla_m4_tensor * kc, const mla_m4_tensor * q, const mla_m4_t
         127 * (int64_t)q->nb[2] + q->ne[1] * (int64_t)q->nb[1] > pg::Q_SPAN)
         return MLA_M4_ERR_UNSUPPORTED;
     if (q->ne[1] > 1024 || q->ne[2] > pg::MAX_ROWS || kc->ne[1] / page_size > INT32_MAX) return MLA_M4_ERR_UNSUPPORTED;
+    if ((double)(q->ne[1] * q->ne[1] * q->ne[2]) * ((double)table->ne[0] * page_size) > pg::MAX_LINE) return MLA_M4_ERR_UNSUPPORTED;
     return MLA_M4_OK;
 }
 

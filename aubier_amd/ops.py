@@ -533,7 +533,7 @@ def ggml_m4_kqkv_paged(kcache, q: torch.Tensor, past: torch.Tensor, n_new: torch
     if workspace is None:
         need = lib.mla_m4_kqkv_paged_workspace_bytes(vk, vq, vp, vf, vo)
         workspace = torch.empty(need, dtype=torch.uint8, device=q.device) if need > 0 else None
-    elif workspace.get_device() != gpu:
+    elif workspace.get_device() != gpu or not workspace.is_contiguous():
         raise MlaM4Error("ggml_m4_kqkv_paged", -5)
     ws_ptr, ws_bytes = (workspace.data_ptr(), workspace.numel() * workspace.element_size()) if workspace is not None else (None, 0)
     _run_on("ggml_m4_kqkv_paged", gpu, lib.mla_m4_kqkv_paged, vk, vq, vp, vn, vt, page_size, vf, kq_scale, vo, ws_ptr, ws_bytes)

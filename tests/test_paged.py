@@ -99,6 +99,14 @@ def test_supports_kqkv_paged():
         assert not attn(**bad), bad
 
 
+def test_supports_kqkv_paged_work_limit():
+    """The places on the line of work are whole numbers in 64-bit floating point."""
+    q, out = torch.empty((4096, 1024, 320), dtype=torch.float16), torch.empty((1024, 4096, 256), dtype=torch.float16)   # (never touched)
+    kc = torch.zeros((65536, 320), dtype=torch.float16)
+    for pages, ok in ((1 << 12, True), ((1 << 12) + 1, False), (1 << 14, False)):
+        assert ok == attn(320, 256, q=q, out=out, kcache=kc, table=i32(2, pages), page_size=65536)
+
+
 def test_entry_points_reject_before_launching():
     """Refused by the host's checks: nothing is launched, no pointer is followed."""
     lib, P = A.load_library(), lambda t: ctypes.byref(ops.view(t))  # noqa: E731

@@ -304,9 +304,10 @@ def test_workspace(dev, dk, H, past, new, prefix, share, cache):
         got.append(out)
     check(b, got[0])
     assert torch.equal(got[0], got[1]) and torch.equal(got[0], got[2])
-    with pytest.raises(A.MlaM4Error) as e:
-        b.run(workspace=big[:need - 1])
-    assert e.value.status == -5
+    for bad in (big[:need - 1], big[1:], big[:1].expand(need), big.cpu()):
+        with pytest.raises(A.MlaM4Error) as e:
+            b.run(workspace=bad)
+        assert e.value.status == -5
 
 
 def test_shared_cells_on_pages_that_are_none(dev):
