@@ -20,6 +20,13 @@
 // i + g, as along the line one of the two grows from piece to piece.  Of the other groups a workgroup holds at most two
 // in part: one that goes on behind it has record i, one that began before it record N + i.
 //
+// What it comes to (device times in a graph, both launches; narrow pieces read at 6.3 TB/s, wide ones run at 1.08
+// PFLOP/s, where a large copy moves 5.2 and a large f16 matrix product 1.18): 4 requests of 90,000 to 131,000 cells, 16
+// heads, 82 us; 48 of 300 to 9,000, 32 heads, 44.5; 64 behind 32,768 shared cells 165; 9 requests and a chunk of 700
+// tokens, 40 heads, 126; one of 200 cells 11.7.  Around the tiles a call spends 2.5 us on the places, 0.8 on a piece's
+// setup, 2 (narrow) to 4 (wide) on its q, 1 to 2 on its results, and 4 to 22 on the second launch, whose bytes are the
+// records'.
+//
 // All positions on the line are computed by the same expressions in every workgroup (in 64-bit floating point, exact
 // for whole numbers below 2^53, which MAX_LINE keeps them), so the workgroups agree where one ends and the next begins.
 #include "paged_pass.h"
@@ -31,7 +38,9 @@ namespace {
 
 constexpr int N_WG = 256;                   // one workgroup per CU
 // Costs, in tenths of a wide tile (all of them times H, so that they are whole numbers): a tile for up to 128 rows and
-// for up to 32, and a piece's start and end (its rows in, its results out).
+// for up to 32, and a piece's start and end (its rows in, its results out).  Times of tiles and pieces per geometry and
+// cache; one set for all of them took 50.5 us instead of 48 for 40 8-bit requests behind 12,000 cells, starts of 8 less 88.7
+// instead of 78.2 for 1,000 tokens of one prompt, of 4 more 40.2 instead of 38.2 for four tokens of 24 requests.
 template <int DK, bool Q8>
 struct Cost {
     static constexpr bool BIG = DK == 576;
@@ -542,30 +551,19 @@ __global__ __launch_bounds__(NT) void kqkv_paged_merge_few_kernel(AttnArgs a) {
     merge_together<DV, NT, RW>(a, rp, a.work + records_off(a.n_head, a.nt), row, blockIdx.y, sh);
 }
 
-// Many rows: a wavefront per 32 rows and S slabs; rows of many pieces (a long request among short ones) by the whole
-// workgroup, slab by slab
-constexpr int MANY_PIECES = 24;
+// Many rows: a wavefront per 32 rows and S slabs (also rows of many pieces, a long request among short ones: 100,000 cells
+// beside 63 requests of 50 88.6 us, and 93.9 with such rows' pieces dealt to four wavefronts)
 template <int DV, int S>
 __global__ __launch_bounds__(NTHR) void kqkv_paged_merge_kernel(AttnArgs a) {
-    __shared__ MergeLds<NTHR> sh;
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, hi = lane >> 5;
     const Head head = *reinterpret_cast<const Head *>(a.work);
     const char * records = a.work + records_off(a.n_head, a.nt);
-    const int row = 32 * (int)blockIdx.x + (lane & 31), s0 = 4 * S * (int)blockIdx.y;
+    const int row = 32 * (int)blockIdx.x + (lane & 31), s0 = S * (4 * (int)blockIdx.y + (int)(threadIdx.x >> 6));
     const RowPieces rp(a, head, row);
-    if (__builtin_amdgcn_ballot_w64(rp.n > 0) == 0) return;
-    if (__builtin_amdgcn_ballot_w64(rp.n > MANY_PIECES) == 0) {
-        Part<DV, S> p;
-        if (__builtin_amdgcn_ballot_w64(rp.n > 2) == 0) p.template add<2>(rp, records, 0, 1, s0 + S * w, lane >> 5);     // a chunk's rows
-        else p.template add<4>(rp, records, 0, 1, s0 + S * w, lane >> 5);
-        if (rp.n > 0) p.out(a, row, s0 + S * w, lane >> 5);
-    } else {
-#pragma unroll 1
-        for (int s = 0; s < 4 * S; ++s) {
-            merge_together<DV, NTHR, 32>(a, rp, records, row, s0 + s, sh);
-            __syncthreads();
-        }
-    }
+    Part<DV, S> p;
+    if (__builtin_amdgcn_ballot_w64(rp.n > 2) == 0) p.template add<2>(rp, records, 0, 1, s0, hi);     // a chunk's rows
+    else p.template add<4>(rp, records, 0, 1, s0, hi);
+    if (rp.n > 0) p.out(a, row, s0, hi);
 }
 
 }  // namespace
@@ -590,7 +588,7 @@ static hipError_t launch(bool q8, const AttnArgs & a, hipStream_t stream) {
     const int rows = a.n_head * a.nt;
     // The card starts some 400 workgroups per us, so as many as take part at once, no more; the fewer rows, the more
     // pieces each has.  Device times of whole calls either side of a limit, the smaller form first: 96 rows 19.2, 21.9 us
-    // and 192 rows 38.7, 41.1; 1,024 rows 51.7, 57.0 and 1,536 44.4, 45.4, but 2,048 71.7, 69.9; 2,048 rows 69.5, 79.4,
+    // and 192 rows 38.7, 41.1; 384 rows 25.0, 29.6 and 1,536 44.7, 45.6, but 2,048 70.8, 68.6; 2,048 rows 69.5, 79.4,
     // 6,400 28.8, 28.9, 32,000 78.4, 77.2.
     const auto wgs = [=](int r) { return dim3((rows + r - 1) / r, DV / 16); };
     if (rows <= 256) hipLaunchKernelGGL((kqkv_paged_merge_few_kernel<DV, 512, 8>), wgs(8), dim3(512), 0, stream, a);
