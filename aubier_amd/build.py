@@ -1,8 +1,8 @@
-"""Build the gfx950 kernel library (aubier_amd/libmla_m4.so) and the CPU oracle
-(oracle/libmla_oracle.so), in-tree.
+"""Build the gfx950 kernel library (aubier_amd/libmla_m4.so), the compiled calls of the paged operators
+(aubier_amd/_binding.so) and the CPU oracle (oracle/libmla_oracle.so), in-tree.
 
-    python -m aubier_amd.build            # both
-    python -m aubier_amd.build --lib      # kernels only
+    python -m aubier_amd.build            # all
+    python -m aubier_amd.build --lib      # kernels and calls only
 
 Every HIP translation unit is compiled with hipcc for gfx950 only, with packed-FP32 VALU
 instructions disabled (-packed-fp32-ops), then linked into one shared library exporting the C ABI
@@ -23,6 +23,8 @@ ROOT = PKG.parent
 CSRC = PKG / "csrc"
 BUILD = PKG / "_build"
 LIB = PKG / "libmla_m4.so"
+BINDING_SRC = PKG / "binding.cpp"
+BINDING = PKG / "_binding.so"
 ORACLE_SRC = ROOT / "oracle" / "mla_oracle.c"
 ORACLE_LIB = ROOT / "oracle" / "libmla_oracle.so"
 
@@ -66,6 +68,31 @@ def build_lib(verbose: bool = True) -> Path:
     return LIB
 
 
+def build_binding(verbose: bool = True) -> Path | None:
+    """The compiled calls need PyTorch's C++ headers; without them, or where they do not fit, Python's calls go through
+    ctypes and there is no module (an old one is removed)."""
+    import sysconfig
+
+    import torch
+    from torch.utils import cpp_extension
+
+    tmp = BINDING.with_suffix(".so.tmp")
+    inc = [ROOT / "include", sysconfig.get_paths()["include"], *cpp_extension.include_paths()]
+    libs = cpp_extension.library_paths()
+    try:
+        _run([shutil.which("g++") or "c++", "-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+              *(x for i in inc for x in ("-I", str(i))), str(BINDING_SRC), "-o", str(tmp), *(x for d in libs for x in ("-L", str(d))),
+              "-lc10", "-ltorch_cpu", "-ltorch_python"])
+    except (RuntimeError, OSError) as e:
+        BINDING.unlink(missing_ok=True)
+        print(f"{BINDING_SRC.relative_to(ROOT)} not built, the calls go through ctypes: {str(e)[-2000:]}")
+        return None
+    os.replace(tmp, BINDING)
+    if verbose:
+        print(f"built {BINDING.relative_to(ROOT)}")
+    return BINDING
+
+
 def build_oracle(verbose: bool = True) -> Path:
     cc = shutil.which("gcc") or "cc"
     tmp = ORACLE_LIB.with_suffix(".so.tmp")
@@ -85,6 +112,7 @@ def main(argv=None) -> int:
     every = not (args.lib or args.oracle)
     if args.lib or every:
         build_lib()
+        build_binding()
     if args.oracle or every:
         build_oracle()
     return 0

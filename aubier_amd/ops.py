@@ -214,7 +214,8 @@ def _check(op: str, rc: int) -> None:
 
 
 # The operators of a paged batch run once per layer or step on a handful of small tensors, so the host's time per call
-# counts: their descriptors are packed in one go instead of one ctypes structure each (24 -> 13 us a call).
+# counts: a compiled module makes them (binding.cpp, 6 us), or else their descriptors are packed in one go instead of one
+# ctypes structure each (24 -> 13 us a call).
 _FIELDS = "Pii4q4Q"                         # struct mla_m4_tensor
 _DESC_BYTES = struct.calcsize(_FIELDS)
 _packers: dict = {}
@@ -284,9 +285,44 @@ def _run_on(op: str, dev: int, fn, *args):
         raise MlaM4Error(op, rc)
 
 
+_get_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
 def _raw_stream(dev: int) -> int:
-    get = getattr(torch._C, "_cuda_getCurrentRawStream", None)
-    return get(dev) if get is not None else torch.cuda.current_stream(dev).cuda_stream
+    return _get_raw_stream(dev) if _get_raw_stream is not None else torch.cuda.current_stream(dev).cuda_stream
+
+
+_native = None
+
+
+def _calls():
+    """The paged operators' calls as compiled from binding.cpp (13 -> 6 us of host time each), or False where that module is
+    not built or was built for another PyTorch: then they go through ctypes, with the same results."""
+    global _native
+    if _native is None:
+        lib = load_library()
+        try:
+            from . import _binding
+        except ImportError:
+            _native = False
+        else:
+            _binding.bind(*(ctypes.cast(getattr(lib, f), ctypes.c_void_p).value for f in (
+                "mla_m4_pages", "mla_m4_kvrows", "mla_m4_kqkv_paged", "mla_m4_kqkv_paged_workspace_bytes")))
+            _native = _binding
+    return _native
+
+
+def _stream_of(op: str, t: torch.Tensor) -> int:
+    dev = t.get_device()
+    if dev < 0:
+        raise MlaM4Error(op, -1)
+    return _raw_stream(dev)
+
+
+def _done(op: str, r):
+    if type(r) is int:
+        raise MlaM4Error(op, r)
+    return r
 
 
 # ------------------------------------------------------------------------------------ ops
@@ -489,6 +525,10 @@ def ggml_m4_pages(past: torch.Tensor, n_new: torch.Tensor, free: torch.Tensor, t
     """Block tables and slot maps from request lengths (include/mla_m4.h mla_m4_pages): past, n_new int32 [n_seq];
     free int32 [n_free], the ids that may be taken; table int32 [n_seq, max_pages], the new pages entered in place.
     Returns slot int64 [n_rows] (-1: no cell), pos int32 [n_rows] and used int32 [2] (pages taken, rows of the batch)."""
+    calls = _native or _calls()
+    if calls:
+        return _done("ggml_m4_pages", calls.pages(past, n_new, free, table, page_size, n_rows, slot, pos, used,
+                                                  _stream_of("ggml_m4_pages", table)))
     lib = load_library()
     dev = table.device
     slot = torch.empty(n_rows, dtype=torch.int64, device=dev) if slot is None else slot
@@ -504,6 +544,11 @@ def ggml_m4_kvrows(x: torch.Tensor, kv_norm: torch.Tensor, kcache, slot: torch.T
     """A batch's latent rows into the cache (include/mla_m4.h mla_m4_kvrows): x f32 or f16 [n_rows, d_lat + n_dims], the
     wkv_a product; kv_norm f32 [d_lat]; kcache f16 [n_cells, d_lat + n_dims] or Q8_0, row slot[r] written in place (none for
     a slot outside the cache); slot int64 [n_rows], pos int32 [n_rows] -> Kcur f32 [n_rows, d_lat + n_dims]."""
+    calls = _native or _calls()
+    if calls:
+        kc, ne0 = (kcache.blocks, kcache.ne0) if isinstance(kcache, Q8_0) else (kcache, 0)
+        return _done("ggml_m4_kvrows", calls.kvrows(x, kv_norm, kc, ne0, slot, pos, ctypes.addressof(rope), out,
+                                                    _stream_of("ggml_m4_kvrows", x)))
     lib = load_library()
     if out is None:
         out = torch.empty(x.shape, dtype=torch.float32, device=x.device)
@@ -526,6 +571,11 @@ def ggml_m4_kqkv_paged(kcache, q: torch.Tensor, past: torch.Tensor, n_new: torch
     [n_seq]; table int32 [n_seq, max_pages]; prefix int32 [2] (cells, requests) or None: the first requests' tables begin
     with the same pages, whose cells are then read once for all of them.  out [H, nt, D_v], of q's type unless given; rows
     behind the last request are left as they are (in a new `out`: not set).  workspace: optional uint8 device buffer."""
+    calls = _native or _calls()
+    if calls:
+        kc, ne0 = (kcache.blocks, kcache.ne0) if isinstance(kcache, Q8_0) else (kcache, 0)
+        return _done("ggml_m4_kqkv_paged", calls.kqkv_paged(kc, ne0, q, past, n_new, table, page_size, kq_scale, prefix, out, _dv_of(kcache),
+                                                            workspace, _stream_of("ggml_m4_kqkv_paged", q)))
     lib = load_library()
     if out is None:
         out = torch.empty((q.shape[1], q.shape[0], _dv_of(kcache)), dtype=q.dtype, device=q.device)
