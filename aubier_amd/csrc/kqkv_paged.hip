@@ -3,16 +3,16 @@
 //   dst[h][t][:] = softmax_j(kq_scale q[t][h] . K[cell(j)]) . V[cell(j)],  V = the first D_v columns of a row,
 // and the cells that the first requests share are taken once for all of them.
 //
-// The rows (token, head) of a request are cut into blocks of 128, those of all sharing requests together into blocks
-// of 128 against the shared cells: these are the groups, each with its run of 64-key tiles.  A request with at most 32
-// rows (a decode step) streams its cells at the memory's rate with four waves on the same 32 rows; the others reuse
-// each tile for up to 128 rows, where the matrix cores and the memory are about even (128 rows x 2 x (D_k + D_v)
-// operations per 2 D_k bytes of a key), and the shared cells, read once per 128 rows of the whole batch, are a dense
-// product.
+// The rows (token, head) of a request are cut into blocks of 128 (of 32 where there is little to do: FEW_TILES), those
+// of all sharing requests together into blocks of 128 against the shared cells: these are the groups, each with its run
+// of 64-key tiles.  Up to 32 rows (a decode step) stream their cells at the memory's rate with four waves on the same
+// rows; more reuse each tile for up to 128, where the matrix cores and the memory are about even (128 rows x 2 x
+// (D_k + D_v) operations per 2 D_k bytes of a key), and the shared cells, read once per 128 rows of the whole batch, are
+// a dense product.
 //
 // Work split.  The lengths are on the device and very different, a CU holds one workgroup (150 KB of LDS), and a
-// second round of workgroups that is mostly empty costs a whole one.  So the groups' costs (tiles, and OVERHEAD tiles
-// for a group's start and end) are laid end to end, and workgroup i of N takes the i-th N-th of the line: pieces of one
+// second round of workgroups that is mostly empty costs a whole one.  So the groups' costs (of their tiles
+// and of a group's start and end) are laid end to end, and workgroup i of N takes the i-th N-th of the line: pieces of one
 // or several groups.  Every workgroup finds its place by itself from the lengths (two prefix sums over the requests),
 // so nothing is planned on the host and nothing waits for a planning launch.  A group that ends up in one piece, with
 // nothing shared, goes straight to dst; the other pieces leave records, which the second launch merges.  Groups of
@@ -60,6 +60,13 @@ __device__ __forceinline__ int repeat_cost(int rows) {
     return rows <= HG ? (rows > 0 ? 5 : 0) : rows / BLOCK_ROWS * 10 + (part > 0 ? 6 + (part + 31) / 32 : 0);
 }
 
+// Of few tiles in all (counted for 32 rows each; nothing shared) every group is of 32 rows: its q, its results and its
+// records are a quarter, and the card is not full. Device times with groups of 32 and of 128 rows: 2 requests of 7,500 cells,
+// 128 heads (944 tiles) 24.0 and 32.0 us, one of 20,000 (1,252) 25.0 and 31.7, one of 29,000 (1,816) 30.4 and 33.2, of 50,000
+// (3,128) 39.2 and 38.8; 4 tokens of 50 requests of 84 to 283 cells (800) 27.0 and 31.6, of 16 of 1,700 (1,728) 36.9 and
+// 33.8; over (320, 256) one of 40,000 (2,504) 25.6 and 23.9.
+constexpr int FEW_TILES = 1600;
+
 // Workspace: a header, the pieces of every shared block and of every row, the records (those of whole groups, two per
 // workgroup, then those of the sharing rows' groups)
 struct Head { int rows, shared_rows; };
@@ -80,6 +87,7 @@ struct Walk {
     int n_wg;
     int total;                              // rows (tokens) of the batch
     int cap;                                // cells that a table lists
+    int block;                              // rows of a request's group: 128, or 32 (few tiles in all)
     int n_share, shared_keys, shared_rows;  // sharing requests, their cells, their rows (token, head)
     int shared_by;                          // the first of them that has tokens
     int b, j, tok0, g;                      // the next group: block j of request b (-1: of the shared rows), its first
@@ -91,33 +99,35 @@ struct Walk {
     __device__ __forceinline__ double shared_a(int n_head) const { return (double)n_head * (double)(C::WIDE_START + C::WIDE_TILE * (shared_keys / TK)); }
 };
 
-// request b's place: its tokens, what they see, its blocks and their costs (the j-th: a + 2 WIDE_TILE (j + 1), as
-// 128 rows on are 128 / H tokens, 2 / H tiles)
+// request b's place: its tokens, what they see, its blocks and their costs (the j-th of 128 rows: a + 2 WIDE_TILE (j + 1),
+// as 128 rows on are 128 / H tokens, 2 / H tiles; of 32 rows: a + NARROW_TILE (j + 1) / 2)
 template <typename C>
 struct Request {
     int n, past, key0, blocks, first;
     bool wide;
-    double a;
+    double a, more;
     __device__ __forceinline__ Request(const AttnArgs & ar, const Walk & wk, int H, int n_new, int past_, int b, int start) {
         n = min(min(max(n_new, 0), ar.nt), ar.nt - start);
         past = min(clamp_past(past_), wk.cap);
         key0 = b < wk.n_share ? wk.shared_keys : 0;
-        blocks = (n * H + BLOCK_ROWS - 1) / BLOCK_ROWS;
-        wide = n * H > HG;
+        const bool narrow = wk.block == HG;
+        blocks = (n * H + wk.block - 1) >> (narrow ? 5 : 7);
+        wide = n * H > HG && !narrow;
+        more = narrow ? 0.25 * (double)C::NARROW_TILE : (double)C::WIDE_TILE;
         first = max((min(past + 1, wk.cap) - key0 + TK - 1) / TK, 1);
         a = (double)H * (double)(start_cost() + (wide ? C::WIDE_TILE : C::NARROW_TILE) * first);
     }
     __device__ __forceinline__ Request(const AttnArgs & ar, const Walk & wk, int H, int b, int start)
         : Request<C>(ar, wk, H, ar.n_new[b], ar.past[b], b, start) {}
     __device__ __forceinline__ int start_cost() const { return wide ? C::WIDE_START : C::NARROW_START; }
-    __device__ __forceinline__ double upto(int j) const { return (double)j * a + (double)C::WIDE_TILE * ((double)j * ((double)j + 1.0)); }
+    __device__ __forceinline__ double upto(int j) const { return (double)j * a + more * ((double)j * ((double)j + 1.0)); }
     __device__ __forceinline__ double cost() const { return upto(blocks); }
 };
 
 // This workgroup's stretch and its first group (b = n_seq: none), from the lengths: two sums over the requests by the
 // whole workgroup, then the thread whose request holds the stretch's start says so.
 struct PlaceLds {
-    int rows[4], shared[4][3];              // per wavefront: rows; sharing requests' cells, rows, first
+    int rows[4], tiles[4], shared[4][3];    // per wavefront: rows; narrow tiles; sharing requests' cells, rows, first
     double repeat[4], cost[4];
     uint64_t groups[4];
     double base;
@@ -144,11 +154,14 @@ __device__ __forceinline__ Walk find_place(const AttnArgs & a, PlaceLds & sh) {
         return v;
     };
 
-    int own = 0, keys = min(max(k_pre, 0), k.cap), srows = 0, by = MAX_SEQS;
+    int own = 0, tiles32 = 0, keys = min(max(k_pre, 0), k.cap), srows = 0, by = MAX_SEQS;
     double repeat = 0.0;
     for (int b = b0; b < b1; ++b) {
         const int n = min(max(n_of(b), 0), a.nt);
         own += n;
+        // (no more than FEW_TILES of either factor, nor more than one past it of a request, count)
+        const int tiles = min((n * H + HG - 1) / HG, FEW_TILES) * min((min(clamp_past(past_of(b)), k.cap) + n / 2) / TK + 1, FEW_TILES);
+        tiles32 += min(tiles, FEW_TILES + 1);
         if (b < n_pre && n > 0) {
             keys = min(keys, clamp_past(past_of(b)));
             by = min(by, b);
@@ -157,7 +170,11 @@ __device__ __forceinline__ Walk find_place(const AttnArgs & a, PlaceLds & sh) {
         }
     }
     const int incl = wave_scan(own);
-    if (lane == 63) sh.rows[w] = incl;
+    tiles32 = wave_scan(tiles32);
+    if (lane == 63) {
+        sh.rows[w] = incl;
+        sh.tiles[w] = tiles32;
+    }
     if (a.prefix != nullptr) {
         keys = wave_min(keys);
         by = wave_min(by);
@@ -193,6 +210,7 @@ __device__ __forceinline__ Walk find_place(const AttnArgs & a, PlaceLds & sh) {
             k.shared_keys = k.shared_rows = 0;
         }
     }
+    k.block = uni(k.n_share == 0 && sh.tiles[0] + sh.tiles[1] + sh.tiles[2] + sh.tiles[3] <= FEW_TILES ? HG : BLOCK_ROWS);
     const double shared_a = k.template shared_a<C>(H), shared_cost = (double)k.shared_blocks() * shared_a;
 
     // costs, and (tiles, groups) in the high and low half of a word; of a request's tiles no more than N_WG each way count,
@@ -310,7 +328,7 @@ __global__ __launch_bounds__(NTHR, 1) void kqkv_paged_kernel(AttnArgs a) {
             b = uni(k.b);
             j = uni(k.j);
             p.tok0 = uni(k.tok0);
-            p.row0 = j * BLOCK_ROWS;
+            p.row0 = j * (b < 0 ? BLOCK_ROWS : k.block);
             double g0, g1, body;             // its stretch, and where its tiles begin on it
             int n_tiles, blocks, n = 0;
             double cost;
@@ -332,7 +350,7 @@ __global__ __launch_bounds__(NTHR, 1) void kqkv_paged_kernel(AttnArgs a) {
                 n = rq.n;
                 cost = rq.cost();
                 blocks = rq.blocks;
-                p.rows = uni(min(BLOCK_ROWS, n * H - p.row0));
+                p.rows = uni(min(k.block, n * H - p.row0));
                 p.past = uni(rq.past);
                 p.key0 = uni(rq.key0);
                 p.key1 = uni(min(rq.past + (p.row0 + p.rows - 1) / H + 1, k.cap));
