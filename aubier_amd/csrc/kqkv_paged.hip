@@ -88,10 +88,12 @@ struct Walk {
     int total;                              // rows (tokens) of the batch
     int cap;                                // cells that a table lists
     int block;                              // rows of a request's group: 128, or 32 (few tiles in all)
+    int single;                             // 1: a workgroup per tile
     int n_share, shared_keys, shared_rows;  // sharing requests, their cells, their rows (token, head)
     int shared_by;                          // the first of them that has tokens
     int b, j, tok0, g;                      // the next group: block j of request b (-1: of the shared rows), its first
                                             // token, its number
+    int n_new, past;                        // request b's, as given
     double per;                             // all / n_wg
     __device__ __forceinline__ double edge(int i) const { return i >= n_wg ? all : per * (double)i; }
     __device__ __forceinline__ int shared_blocks() const { return (shared_rows + BLOCK_ROWS - 1) / BLOCK_ROWS; }
@@ -103,8 +105,8 @@ struct Walk {
 // as 128 rows on are 128 / H tokens, 2 / H tiles; of 32 rows: a + NARROW_TILE (j + 1) / 2)
 template <typename C>
 struct Request {
-    int n, past, key0, blocks, first;
-    bool wide;
+    int n, past, key0, blocks;
+    bool wide, free_start;
     double a, more;
     __device__ __forceinline__ Request(const AttnArgs & ar, const Walk & wk, int H, int n_new, int past_, int b, int start) {
         n = min(min(max(n_new, 0), ar.nt), ar.nt - start);
@@ -113,13 +115,14 @@ struct Request {
         const bool narrow = wk.block == HG;
         blocks = (n * H + wk.block - 1) >> (narrow ? 5 : 7);
         wide = n * H > HG && !narrow;
-        more = narrow ? 0.25 * (double)C::NARROW_TILE : (double)C::WIDE_TILE;
-        first = max((min(past + 1, wk.cap) - key0 + TK - 1) / TK, 1);
+        more = wk.single != 0 ? 0.0 : narrow ? 0.25 * (double)C::NARROW_TILE : (double)C::WIDE_TILE;
+        free_start = wk.single != 0;
+        const int first = max((min(past + 1, wk.cap) - key0 + TK - 1) / TK, 1);
         a = (double)H * (double)(start_cost() + (wide ? C::WIDE_TILE : C::NARROW_TILE) * first);
     }
     __device__ __forceinline__ Request(const AttnArgs & ar, const Walk & wk, int H, int b, int start)
-        : Request<C>(ar, wk, H, ar.n_new[b], ar.past[b], b, start) {}
-    __device__ __forceinline__ int start_cost() const { return wide ? C::WIDE_START : C::NARROW_START; }
+        : Request<C>(ar, wk, H, wk.n_new, wk.past, b, start) {}
+    __device__ __forceinline__ int start_cost() const { return free_start ? 0 : wide ? C::WIDE_START : C::NARROW_START; }
     __device__ __forceinline__ double upto(int j) const { return (double)j * a + more * ((double)j * ((double)j + 1.0)); }
     __device__ __forceinline__ double cost() const { return upto(blocks); }
 };
@@ -129,9 +132,9 @@ struct Request {
 struct PlaceLds {
     int rows[4], tiles[4], shared[4][3];    // per wavefront: rows; narrow tiles; sharing requests' cells, rows, first
     double repeat[4], cost[4];
-    uint64_t groups[4];
+    int groups[4];
     double base;
-    int b, tok0, g;
+    int b, tok0, g, n_new, past;
 };
 template <typename C>
 __device__ __forceinline__ Walk find_place(const AttnArgs & a, PlaceLds & sh) {
@@ -210,58 +213,58 @@ __device__ __forceinline__ Walk find_place(const AttnArgs & a, PlaceLds & sh) {
             k.shared_keys = k.shared_rows = 0;
         }
     }
-    k.block = uni(k.n_share == 0 && sh.tiles[0] + sh.tiles[1] + sh.tiles[2] + sh.tiles[3] <= FEW_TILES ? HG : BLOCK_ROWS);
+    tiles32 = sh.tiles[0] + sh.tiles[1] + sh.tiles[2] + sh.tiles[3];
+    k.block = uni(k.n_share == 0 && tiles32 <= FEW_TILES ? HG : BLOCK_ROWS);
+    k.single = uni(k.n_share == 0 && tiles32 <= N_WG ? 1 : 0);
     const double shared_a = k.template shared_a<C>(H), shared_cost = (double)k.shared_blocks() * shared_a;
 
-    // costs, and (tiles, groups) in the high and low half of a word; of a request's tiles no more than N_WG each way count,
-    // as all that is asked is whether there are fewer than workgroups
     double cost = 0.0;
-    uint64_t groups = 0;
+    int groups = 0;
     {
         int at = min(start, a.nt);
         for (int b = b0; b < b1; ++b) {
             const Request<C> rq(a, k, H, n_of(b), past_of(b), b, at);
             cost += rq.cost();
-            groups += (uint64_t)rq.blocks + ((uint64_t)(uint32_t)(min(rq.blocks, N_WG) * min(rq.first, N_WG)) << 32);
+            groups += rq.blocks;
             at += rq.n;
         }
     }
     const double cost_incl = wave_scan(cost);
-    const uint64_t groups_incl = wave_scan(groups);
+    const int groups_incl = wave_scan(groups);
     if (lane == 63) {
         sh.cost[w] = cost_incl;
         sh.groups[w] = groups_incl;
     }
     __syncthreads();
     double base = cost_incl - cost;
-    uint64_t grp = groups_incl - groups, all_groups = 0;
+    int grp = groups_incl - groups;
     k.all = 0.0;
 #pragma unroll
     for (int i = 0; i < NTHR / 64; ++i) {
         base += i < w ? sh.cost[i] : 0.0;
         grp += i < w ? sh.groups[i] : 0;
         k.all += sh.cost[i];
-        all_groups += sh.groups[i];
     }
     base += shared_cost;
     k.all += shared_cost;
-    // Where there are fewer tiles than workgroups two workgroups per tile: a stretch is then shorter than a tile, so none
-    // takes two, nor a tile behind another group's start (200 tokens of one prompt: one per tile 39 us, two 30; a
-    // decode over 200 cells 13.8 and 12.4; three and more do not gain, fewer pieces lose 2 us for each tile more in a row)
-    const int64_t tiles = (int64_t)(all_groups >> 32) + (int64_t)k.shared_blocks() * (k.shared_keys / TK);
-    k.n_wg = uni((int)min(max(2 * tiles, (int64_t)1), (int64_t)gridDim.x));
+    // Where there are fewer tiles than workgroups, one workgroup each: tiles alone make up the line then, as every piece
+    // starts anew. With starts on it and all workgroups: 64 requests of 150 to 250 cells 17.9 instead of 16.0 us, 100 tokens of a
+    // prompt 17.1 instead of 12.8, 8 requests of 500 to 700 15.2 instead of 14.1; but of more tiles (290) 18.0 instead of 21.5.
+    k.n_wg = k.single != 0 ? uni(max(tiles32, 1)) : (int)gridDim.x;
     k.per = k.all / (double)k.n_wg;
     k.x0 = k.edge(wg);
     k.x1 = k.edge(wg + 1);
 
     const bool any = wg < k.n_wg && k.total > 0, at_shared = uni(k.x0 < shared_cost);
     if (any && !at_shared && base <= k.x0 && k.x0 < base + cost) {
-        int at = min(start, a.nt), g = (int)(uint32_t)grp;
+        int at = min(start, a.nt), g = grp;
         for (int b = b0; b < b1; ++b) {
             const Request<C> rq(a, k, H, n_of(b), past_of(b), b, at);
             const double c = rq.cost();
             if (rq.blocks > 0 && (k.x0 < base + c || b + 1 == b1)) {
                 sh.b = b;
+                sh.n_new = n_of(b);
+                sh.past = past_of(b);
                 sh.tok0 = at;
                 sh.g = g;
                 sh.base = base;
@@ -282,6 +285,8 @@ __device__ __forceinline__ Walk find_place(const AttnArgs & a, PlaceLds & sh) {
         while (j > 0 && (double)j * shared_a > k.x0) --j;
         while (j + 1 < k.shared_blocks() && (double)(j + 1) * shared_a <= k.x0) ++j;
     } else if (k.b < a.n_seq) {
+        k.n_new = uni(sh.n_new);
+        k.past = uni(sh.past);
         const Request<C> rq(a, k, H, k.b, k.tok0);
         int len = rq.blocks;
         while (len > 1) {
@@ -383,8 +388,12 @@ __global__ __launch_bounds__(NTHR, 1) void kqkv_paged_kernel(AttnArgs a) {
                 next.tok0 = p.tok0 + n;
                 next.j = 0;
                 next.b = b + 1;
-                while (next.b < a.n_seq && Request<C>(a, k, H, next.b, next.tok0).blocks == 0) ++next.b;
+                for (; next.b < a.n_seq; ++next.b) {
+                    next.n_new = uni(a.n_new[next.b]);
+                    if (next.n_new > 0 && next.tok0 < a.nt) break;
+                }
                 last = uni(next.b >= a.n_seq);
+                if (!last) next.past = uni(a.past[next.b]);
             }
         }
         if (!last && tid == 0) lds.walk = next;

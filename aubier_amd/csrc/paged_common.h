@@ -14,11 +14,6 @@ __device__ __forceinline__ int dpp_from(int none, int v) { return __builtin_amdg
 template <int CTRL, int ROWS>
 __device__ __forceinline__ int step_sum(int v) { return v + dpp_from<CTRL, ROWS>(0, v); }
 template <int CTRL, int ROWS>
-__device__ __forceinline__ uint64_t step_sum(uint64_t v) {
-    const uint32_t lo = (uint32_t)dpp_from<CTRL, ROWS>(0, (int)(uint32_t)v), hi = (uint32_t)dpp_from<CTRL, ROWS>(0, (int)(uint32_t)(v >> 32));
-    return v + ((uint64_t)hi << 32 | lo);
-}
-template <int CTRL, int ROWS>
 __device__ __forceinline__ double step_sum(double v) {
     const uint64_t u = __builtin_bit_cast(uint64_t, v);
     const uint32_t lo = (uint32_t)dpp_from<CTRL, ROWS>(0, (int)(uint32_t)u), hi = (uint32_t)dpp_from<CTRL, ROWS>(0, (int)(uint32_t)(u >> 32));
