@@ -71,7 +71,7 @@ struct AttnArgs {
 bool attn_supported(int dk, int dv);
 size_t attn_workspace_bytes(int dv, int n_seq, int n_head, int nt, bool prefix);
 // n_head^2 nt and the cells that a table lists: the line of work (kqkv_paged.hip), in units of a tenth of a tile's cost by
-// n_head, is at most 10 / 8192 of it and 2^50 for the requests' last blocks long, so it stays below 2^53
+// n_head, is at most 10 / 8192 of it long and 2^49 for the requests' last blocks, so it stays below 2^51
 constexpr double MAX_LINE = 1152921504606846976.0;      // 2^60
 constexpr int64_t MAX_STRIDE = 1 << 25;   // bytes between rows of the cache: 32-bit offsets inside a tile
 constexpr int64_t Q_SPAN = 1u << 31;      // 128 rows of q span at most this: 127 q_nb2 + n_head q_nb1
