@@ -398,7 +398,7 @@ __global__ __launch_bounds__(NTHR, 1) void kqkv_paged_kernel(AttnArgs a) {
             }
         }
         if (!last && tid == 0) lds.walk = next;
-        piece_rows(a, p, sh.qoff, sh.drow, sh.lim);
+        piece_rows(a, p, sh);
         if (first) {
             if (b < 0) {
                 if (tid == 0) reinterpret_cast<Pieces *>(a.work + shared_off())[j] = Pieces{p.slot, (unsigned)pieces};
@@ -415,6 +415,11 @@ __global__ __launch_bounds__(NTHR, 1) void kqkv_paged_kernel(AttnArgs a) {
             narrow_piece<DK, DV, Q8, QF16>(a, p, sh, rec);
         } else {
             wide_piece<DK, DV, Q8, QF16>(a, p, sh, rec);
+        }
+        if (p.lim_min < p.key1 && sh.odd != 0) {     // (the same for all: written ahead of a barrier of the piece's)
+            wait_vm<0>();
+            __syncthreads();                 // the results are in place
+            seen_nonfinite<DK, DV, Q8, QF16>(a, sh, rec);
         }
         if (last) return;
         k = lds.walk;

@@ -67,6 +67,8 @@ struct PieceLds {
     // the rows of a slice that hold a NaN or an infinity (by tile parity)
     __attribute__((aligned(16))) int vc[4][NWAVE];
     uint64_t bad[2][NWAVE][2];
+    Piece piece;                                                        // of rows that see different cells: for seen_nonfinite,
+    int odd;                                                            // and whether it has to run
 };
 
 // the thread index by way of an opaque move, so that what follows from it is computed where it is used, rather than
@@ -85,16 +87,21 @@ __device__ __forceinline__ float opaque_zero() {
     return z;
 }
 
-__device__ __forceinline__ void piece_rows(const AttnArgs & a, const Piece & p, uint32_t * qoff, int * drow, int * lim) {
+template <typename L>
+__device__ __forceinline__ void piece_rows(const AttnArgs & a, const Piece & p, L & sh) {
     const int tid = threadIdx.x;
+    if (tid == 0 && p.lim_min < p.key1) {
+        sh.piece = p;
+        sh.odd = 0;
+    }
     if (tid >= BLOCK_ROWS) return;
     const int r = p.row0 + tid;
     const int t = r / a.n_head, h = r - t * a.n_head;
     const bool live = tid < p.rows;
     // (a row that is not there brings in the first token's first head; nothing of it is used)
-    qoff[tid] = live ? (uint32_t)(t - p.row0 / a.n_head) * (uint32_t)a.q_nb2 + (uint32_t)h * (uint32_t)a.q_nb1 : 0u;
-    drow[tid] = live ? h * a.nt + p.tok0 + t : -1;
-    lim[tid] = live ? min(p.past + t + 1, p.key1) : 0;
+    sh.qoff[tid] = live ? (uint32_t)(t - p.row0 / a.n_head) * (uint32_t)a.q_nb2 + (uint32_t)h * (uint32_t)a.q_nb1 : 0u;
+    sh.drow[tid] = live ? h * a.nt + p.tok0 + t : -1;
+    sh.lim[tid] = live ? min(p.past + t + 1, p.key1) : 0;
 }
 
 // A wave's view of a piece's keys
@@ -162,13 +169,14 @@ struct PageStream {
     }
 };
 
-// Non-finite values of an f16 slice set to zero (the whole wavefront, its own slice); b0, b1: which of rows 0 .. 7 and
-// 8 .. 15 held one (a byte per row).  Only for the tiles that some rows of a piece see and others do not: a cell that
-// a row does not see has weight 0 there, and 0 times a NaN or an infinity would reach its sums.
-template <int DK>
+// Non-finite values of the first COLS columns of an f16 slice set to zero (the whole wavefront, its own slice); b0, b1:
+// which of rows 0 .. 7 and 8 .. 15 held one (a byte per row).  Only for the tiles that some rows of a piece see and others
+// do not: a cell that a row does not see has weight 0 there, and 0 times a NaN or an infinity would reach its sums.  What
+// they mean for the rows that do see them is put in by seen_nonfinite.
+template <int COLS>
 __device__ __forceinline__ void clear_nonfinite(char * sb, int lane, uint64_t & b0, uint64_t & b1) {
     b0 = b1 = 0;
-    for (int i = 0; i < SliceGeom<DK>::DMA_N; ++i) {        // 1 KB block i: rows 8 (i & 1) .. + 7, eight lanes a row
+    for (int i = 0; i < COLS / 32; ++i) {                   // 1 KB block i: rows 8 (i & 1) .. + 7, eight lanes a row, 64 columns
         u32x4 * at = reinterpret_cast<u32x4 *>(sb + 1024 * i + 16 * lane);
         u32x4 v = *at;
         bool any = false;
@@ -182,6 +190,71 @@ __device__ __forceinline__ void clear_nonfinite(char * sb, int lane, uint64_t & 
         if (b != 0) *at = v;
         if (i & 1) b1 |= b;
         else b0 |= b;
+    }
+}
+
+// A piece whose tiles held NaN or infinities that clear_nonfinite has taken out: their effect on the rows that see them, after
+// the piece's results have been stored (all waves).  By the definition, of a seen cell whose score is NaN or +inf the
+// whole row is NaN (inf - inf); one of score -inf has weight 0, and the columns in which it is not finite are NaN (0
+// times infinity).  The score's class comes from the cell's non-finite values alone.  The cells are read again, a wavefront
+// per cell, as this hardly ever runs.
+template <int DK, int DV, bool Q8, bool QF16>
+__device__ __forceinline__ void seen_nonfinite(const AttnArgs & a, const PieceLds<DK, DV, Q8> & sh, char * rec) {
+    static_assert(DK % 64 == 0 && DV % 64 == 0, "64 columns at a time");
+    const int tid = opaque_tid(), lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const Piece p = sh.piece;
+    const char * q = a.q + (int64_t)(p.tok0 + p.row0 / a.n_head) * a.q_nb2;
+    auto put_nan = [&](int r, int c) {
+        if (p.slot >= 0) {
+            char * o = rec + BLOCK_ROWS * 8 + (size_t)((r >> 5) * (DV / 16) + (c >> 4)) * 1024 + 16 * ((r & 31) + 4 * (c & 8)) + 2 * (c & 7);
+            *reinterpret_cast<half_t *>(o) = (half_t)__builtin_nanf("");
+        } else {
+            const size_t at = (size_t)sh.drow[r] * DV + c;
+            if (a.dst_f16) reinterpret_cast<half_t *>(a.dst)[at] = (half_t)__builtin_nanf("");
+            else reinterpret_cast<float *>(a.dst)[at] = __builtin_nanf("");
+        }
+    };
+    const int ka = p.key0 + TK * p.ta, kb = min(p.key1, p.key0 + TK * p.tb);
+    // from the first tile that not all rows see
+    for (int j = max(ka, p.key0 + max(p.lim_min - p.key0, 0) / TK * TK) + w; j < kb; j += NWAVE) {
+        const int id = __builtin_amdgcn_readfirstlane(p.table[j >> a.page_shift]);
+        if (id < 0 || id >= a.n_pages) continue;
+        const char * cell = a.kc + (((int64_t)id << a.page_shift) + (j & ((1 << a.page_shift) - 1))) * a.kc_nb1;
+        float score[2] = {0.0f, 0.0f};                      // of rows lane and 64 + lane
+        bool any = false;
+        for (int d0 = 0; d0 < DK; d0 += 64) {
+            half_t v;
+            if constexpr (Q8) {
+                const char * blk = cell + (d0 + lane) / 32 * 34;
+                v = to_half((float)*reinterpret_cast<const half_t *>(blk) * (float)*reinterpret_cast<const int8_t *>(blk + 2 + (lane & 31)));
+            } else {
+                v = *reinterpret_cast<const half_t *>(cell + 2 * (d0 + lane));
+            }
+            const int bits = __builtin_bit_cast(uint16_t, v);
+            for (uint64_t bad = __builtin_amdgcn_ballot_w64((bits & 0x7c00) == 0x7c00); bad != 0; bad &= bad - 1) {
+                const int at = __builtin_ctzll(bad), d = d0 + at;
+                const float x = (float)__builtin_bit_cast(half_t, (uint16_t)__builtin_amdgcn_readlane(bits, at));
+                any = true;
+#pragma unroll
+                for (int n = 0; n < 2; ++n) {
+                    const int r = lane + 64 * n;
+                    if (j >= sh.lim[r]) continue;           // (0 for a row that is not there)
+                    const char * qd = q + sh.qoff[r];
+                    const half_t qv = QF16 ? reinterpret_cast<const half_t *>(qd)[d] : to_half(reinterpret_cast<const float *>(qd)[d]);
+                    score[n] += (float)qv * x;
+                    if (d < DV) put_nan(r, d);
+                }
+            }
+        }
+        if (!any) continue;
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+            const int r = lane + 64 * n;
+            const float s = score[n] * a.scale_log2;
+            if (j >= sh.lim[r] || (s == s && s != INFINITY)) continue;
+            if (p.slot >= 0) reinterpret_cast<f32x2 *>(rec)[r][1] = __builtin_nanf("");
+            for (int c = 0; c < DV; ++c) put_nan(r, c);
+        }
     }
 }
 
@@ -367,8 +440,9 @@ __device__ __forceinline__ void narrow_piece(const AttnArgs & a, const Piece & p
             n_nxt = dn.n;
         }
         if (key + WK > p.lim_min && key < p.key1 && p.lim_min < p.key1) {     // some rows see these keys, others do not
-            uint64_t b0, b1;
-            clear_nonfinite<DK>(sb, lane, b0, b1);
+            uint64_t b0, b1;                 // (the scores have been taken)
+            clear_nonfinite<DV>(sb, lane, b0, b1);
+            if ((b0 | b1) != 0 && lane == 0) sh.odd = 1;
         }
         float sc[2][4], mx[2];
 #pragma unroll
@@ -619,7 +693,8 @@ __device__ __forceinline__ void wide_piece(const AttnArgs & a, const Piece & p, 
             wait_vm<0>();                               // this wave's slice of the tile has landed
             tile = sh.ring + par * NWAVE * G::STAGE;
         }
-        // all keys seen by all rows: no masks; else the rows that do not see a cell take no part of what it holds
+        // all keys seen by all rows: no masks; else the rows that do not see a cell take no part of what it holds, and a cell
+        // that holds a NaN or an infinity has no finite score: weight 0 here, the rest is seen_nonfinite's
         const bool split = key_t + TK > p.lim_min && p.lim_min < p.key1;
         if (split) {
             uint64_t b0, b1;
@@ -627,6 +702,7 @@ __device__ __forceinline__ void wide_piece(const AttnArgs & a, const Piece & p, 
             if (lane == 0) {
                 sh.bad[par][w][0] = b0;
                 sh.bad[par][w][1] = b1;
+                if ((b0 | b1) != 0) sh.odd = 1;
             }
         }
         __syncthreads();                                // the whole tile is in place; every wave is done with tile k - 1
@@ -676,10 +752,10 @@ __device__ __forceinline__ void wide_piece(const AttnArgs & a, const Piece & p, 
                     const int e = min(n, lim - key_t - WK * sl) - 4 * hi;
                     if (split) {
                         const uint64_t b0 = sh.bad[par][sl][0], b1 = sh.bad[par][sl][1];
-                        if (__builtin_amdgcn_ballot_w64((b0 | b1) != 0) != 0) {     // a key that holds one has no finite score
+                        if (__builtin_amdgcn_ballot_w64((b0 | b1) != 0) != 0) {
 #pragma unroll
                             for (int i = 0; i < 8; ++i)
-                                if (((((i >> 2) ? b1 : b0) >> (8 * ((i & 3) + 4 * hi))) & 0xff) != 0) s[8 * j + i] = __builtin_nanf("");
+                                if (((((i >> 2) ? b1 : b0) >> (8 * ((i & 3) + 4 * hi))) & 0xff) != 0) s[8 * j + i] = -INFINITY;
                         }
                     }
 #pragma unroll
