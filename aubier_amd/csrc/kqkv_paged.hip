@@ -483,8 +483,8 @@ struct Part {
             scale(exp2_unless(m == -INFINITY, m - mx));
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                // without a finite score l is 0, or NaN where every score was; o then holds nothing (an empty piece's
-                // was never written)
+                // without a key l is 0, or NaN where every score was; o then holds nothing (an empty piece's was never
+                // written).  (M_NONE, where no score was above -inf, is as any other: l is 0, o is 0 or NaN.)
                 const bool none = ms[u] == -INFINITY;
                 const float f = none ? ls[u] : ls[u] * exp2_fast(ms[u] - mx);
                 l += f;
@@ -504,7 +504,8 @@ struct Part {
             for (int k = 0; k < 8; ++k) o[s][k] *= f;
     }
     __device__ __forceinline__ void out(const AttnArgs & a, int row, int s0, int hi) const {
-        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        // (no key: zeros; keys, but no score above -inf: 0 / 0)
+        const float inv = l != 0.0f ? 1.0f / l : m == -INFINITY ? 0.0f : __builtin_nanf("");
         const int t = row / a.n_head, h = row - t * a.n_head;
         const size_t at = ((size_t)h * a.nt + t) * DV + 16 * s0 + 8 * hi;
 #pragma unroll

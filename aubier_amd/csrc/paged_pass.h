@@ -45,7 +45,7 @@ struct Piece {
 };
 
 // Records: (m, l) of the block's 128 rows, m in log2 units (a reference for the scores, at most 15 below their
-// maximum; -inf: no key), then o / l in f16 as the accumulators' lanes hold it, so that neither side needs LDS: for every
+// maximum; M_NONE: keys were seen, but no score is above -inf; -inf: no key was seen, and o need not be there), then o / l in f16 as the accumulators' lanes hold it, so that neither side needs LDS: for every
 // 32 rows D_v / 16 slabs of 1 KB, slab s holding columns 16 s .. + 15, lane l's 8 of them (of row l & 31, the upper 8 in
 // the upper half) at 16 l.
 template <int DV>
@@ -67,8 +67,8 @@ struct PieceLds {
     // the rows of a slice that hold a NaN or an infinity (by tile parity)
     __attribute__((aligned(16))) int vc[4][NWAVE];
     uint64_t bad[2][NWAVE][2];
-    Piece piece;                                                        // of rows that see different cells: for seen_nonfinite,
-    int odd;                                                            // and whether it has to run
+    Piece piece;                                                        // for what hardly ever runs behind the tiles: saw_any and
+    int odd;                                                            // seen_nonfinite, and whether the latter has to
 };
 
 // the thread index by way of an opaque move, so that what follows from it is computed where it is used, rather than
@@ -90,7 +90,7 @@ __device__ __forceinline__ float opaque_zero() {
 template <typename L>
 __device__ __forceinline__ void piece_rows(const AttnArgs & a, const Piece & p, L & sh) {
     const int tid = threadIdx.x;
-    if (tid == 0 && p.lim_min < p.key1) {
+    if (tid == 0) {
         sh.piece = p;
         sh.odd = 0;
     }
@@ -168,6 +168,24 @@ struct PageStream {
         return n;
     }
 };
+
+// Of a row whose piece found no score above -inf: whether it sees a key at all, one whose page is there.  By the definition
+// the first has weights 0 / 0, NaN, if the other pieces find none either, and an infinity that it sees is NaN times weight
+// 0 in the others; the second adds nothing.  Both hardly ever run, so the table is asked again, 64 pages at a time (the
+// whole wavefront; lim: keys that the lane's row sees; none: rows without a score).
+__device__ __forceinline__ bool saw_any(const AttnArgs & a, const Piece & in_lds, bool none, int lim, int lane) {
+    if (__builtin_amdgcn_ballot_w64(none && lim > 0) == 0) return false;        // (0: a row that is not there)
+    const Piece p = in_lds;
+    const int ka = p.key0 + TK * p.ta, kb = min(p.key1, p.key0 + TK * p.tb);
+    if (__builtin_amdgcn_ballot_w64(none && lim > ka) == 0) return false;
+    for (int at = ka >> a.page_shift; at <= (kb - 1) >> a.page_shift; at += 64) {
+        const bool in = at + lane <= (kb - 1) >> a.page_shift;
+        const int id = in ? p.table[at + lane] : -1;
+        const uint64_t there = __builtin_amdgcn_ballot_w64(id >= 0 && id < a.n_pages);
+        if (there != 0) return lim > max(ka, (at + __builtin_ctzll(there)) << a.page_shift);
+    }
+    return false;
+}
 
 // Non-finite values of the first COLS columns of an f16 slice set to zero (the whole wavefront, its own slice); b0, b1:
 // which of rows 0 .. 7 and 8 .. 15 held one (a byte per row).  Only for the tiles that some rows of a piece see and others
@@ -503,8 +521,9 @@ __device__ __forceinline__ void narrow_piece(const AttnArgs & a, const Piece & p
 
     // ---- the end: every wave holds its rows' l and its columns of o ----
     const int lane_e = opaque_tid() & 63, hl = lane_e & 31, hi4 = 4 * (lane_e >> 5);
-    const float l = halves_sum(l_acc);
-    const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+    const float l = halves_sum(l_acc), mr = m_ref[(lane_e >> 4) & 1];
+    const bool none = mr == M_NONE, saw = saw_any(a, sh.piece, none, lim[(lane_e >> 4) & 1], lane_e);
+    const float inv = l > 0.0f ? 1.0f / l : none && saw && p.slot < 0 ? __builtin_nanf("") : 0.0f;
     if (p.slot < 0 && !a.dst_f16) {
         const int dr = sh.drow[hl];
 #pragma unroll
@@ -515,10 +534,7 @@ __device__ __forceinline__ void narrow_piece(const AttnArgs & a, const Piece & p
                         f32x4{o[i][4 * q4] * inv, o[i][4 * q4 + 1] * inv, o[i][4 * q4 + 2] * inv, o[i][4 * q4 + 3] * inv});
         return;
     }
-    if (p.slot >= 0 && w == 0 && lane_e < HG) {
-        const float mr = m_ref[(lane_e >> 4) & 1];
-        reinterpret_cast<f32x2 *>(rec)[lane_e] = f32x2{mr == M_NONE ? -INFINITY : mr, l};
-    }
+    if (p.slot >= 0 && w == 0 && lane_e < HG) reinterpret_cast<f32x2 *>(rec)[lane_e] = f32x2{none && !saw ? -INFINITY : mr, l};
     rows_out_f16<DV, C::NTQ>(a, p, o, inv, rec, 0, C::DVQ * w, sh.drow[hl], lane_e);
 }
 
@@ -805,7 +821,8 @@ __device__ __forceinline__ void wide_piece(const AttnArgs & a, const Piece & p, 
     if (!live_w) return;
     const int lane_e = opaque_tid() & 63, hle = lane_e & 31, hi4 = 4 * (lane_e >> 5);
     const float l = halves_sum(l_acc);
-    const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+    const bool none = m_run == M_NONE, saw = saw_any(a, sh.piece, none, lim, lane_e);
+    const float inv = l > 0.0f ? 1.0f / l : none && saw && p.slot < 0 ? __builtin_nanf("") : 0.0f;
     if (p.slot < 0 && !a.dst_f16) {
         const int dr = sh.drow[HG * w + hle];
 #pragma unroll
@@ -817,7 +834,7 @@ __device__ __forceinline__ void wide_piece(const AttnArgs & a, const Piece & p, 
         return;
     }
     if (p.slot >= 0 && lane_e < HG)
-        reinterpret_cast<f32x2 *>(rec)[HG * w + lane_e] = f32x2{m_run == M_NONE ? -INFINITY : m_run, l};
+        reinterpret_cast<f32x2 *>(rec)[HG * w + lane_e] = f32x2{none && !saw ? -INFINITY : m_run, l};
     rows_out_f16<DV, NB>(a, p, o, inv, rec, w, 0, sh.drow[HG * w + hle], lane_e);
 }
 

@@ -155,3 +155,56 @@ def test_behind_shared_cells(dev, cache):
     plant(b, 0, 1000, [90], INF)
     plant(b, 11, 2560 + 78, [20], -INF)
     check(b, b.run())
+
+
+# cells whose tile holds nothing else that a row sees, or whole tiles of them: a piece of the row's keys without a score
+ALONE = [([64], [1], 32, [(0, 64, [5], INF)]), ([64, 30], [1, 1], 32, [(0, 64, [290], INF), (1, 3, [300], INF)]),
+         ([60], [9], 32, [(0, 64, [5], -INF)]), ([60, 640], [9, 1], 8, [(0, 64, [77, 130], INF), (1, 640, [9], INF)]),
+         ([300], [1], 16, [(0, k, [70], INF) for k in range(64, 128)]), ([300, 9], [2, 1], 40, [(0, k, [300], INF) for k in range(128, 192)]),
+         ([0, 20], [1, 1], 32, [(0, 0, [3], INF)]), ([0, 50], [3, 1], 32, [(0, 0, [300], -INF), (0, 1, [301], INF)]),
+         ([30, 5], [1, 2], 16, [(0, k, [280], INF) for k in range(31)])]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("case", range(len(ALONE)))
+@pytest.mark.parametrize("cache,q_type,dst", [("f16", torch.float16, torch.float32), ("q8", torch.float32, torch.float16)])
+def test_pieces_without_a_score(dev, case, cache, q_type, dst):
+    past, new, H, odd = ALONE[case]
+    for dk in (320, 576):
+        b = Batch(dev, past, new, 16, dk=dk, H=H, cache=cache, q_type=q_type, seed=case, pad=1, poison=1.0)
+        if case == 8:                                        # every key of a request -inf for half its heads: 0 / 0
+            b.q[0, ::2, 280] = b.q[0, ::2, 280].abs()
+        for at in odd:
+            plant(b, *at)
+        check(b, b.run(b.out(dst)), f"{dk} {past} {new}")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("past,new,H,odd", [
+    ([9024], [9], 40, [(0, 9024, [5], INF)]), ([9024], [9], 40, [(0, k, [k % 256], INF) for k in range(9024, 9030)]),
+    ([7] * 40, [60] * 40, 32, [(i, 64, [100], -INF) for i in range(40)]),
+    ([9024], [9], 40, [(0, k, [7], INF) for k in range(64 * 16, 64 * 30)]), ([0], [700], 40, [(0, 0, [300], INF), (0, 64, [7], INF), (0, 640, [9], -INF)])])
+@pytest.mark.parametrize("cache,q_type,dst", [("f16", torch.float16, torch.float32), ("q8", torch.float32, torch.float16)])
+def test_pieces_without_a_score_in_blocks_of_128(dev, past, new, H, odd, cache, q_type, dst):
+    b = Batch(dev, past, new, 16, dk=320, H=H, cache=cache, q_type=q_type, seed=len(odd), pad=1, poison=1.0)
+    assert sum(-(-n * H // 32) * ((p + n // 2) // 64 + 1) for p, n in zip(past, new)) > 1600
+    for at in odd:
+        plant(b, *at)
+    check(b, b.run(b.out(dst)), f"{past} {new}")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("absent", [(0, 8), (4, 70), (0, 69)])
+def test_without_a_score_and_without_a_page(dev, absent):
+    """Keys whose pages are none are no keys: a row that sees only such gets zeros, one that sees others of score -inf NaN."""
+    b = Batch(dev, [1100, 20], [3, 1], 16, dk=320, H=16, seed=5, pad=1, poison=1.0)
+    b.q[:, :, 300] = b.q[:, :, 300].abs() + 0.1
+    for k in range(1103):
+        plant(b, 0, k, [300], -INF)
+    b.table[0, absent[0]:absent[1]] = -1
+    got = b.run()
+    if absent == (0, 69):                                    # 1,104 cells: all of them
+        assert (got[:, :3] == 0).all()
+    else:
+        assert torch.isnan(got[:, :3]).all()
+    assert torch.isfinite(got[:, 3]).all() and (got[:, 4] == 7.0).all()
