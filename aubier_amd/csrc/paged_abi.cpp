@@ -226,7 +226,8 @@ size_t mla_m4_kqkv_paged_workspace_bytes(const mla_m4_tensor * kcache, const mla
         past->ne[0] < 1 || past->ne[0] > pg::MAX_SEQS || kcache->ne[0] > 4096 || dst->ne[0] > 4096 ||
         !pg::attn_supported((int)kcache->ne[0], (int)dst->ne[0]))
         return 0;
-    return pg::attn_workspace_bytes((int)dst->ne[0], (int)past->ne[0], (int)q->ne[1], (int)q->ne[2], prefix && prefix->data);
+    // (a prefix that is not allocated yet counts: a planner asks before it allocates)
+    return pg::attn_workspace_bytes((int)dst->ne[0], (int)past->ne[0], (int)q->ne[1], (int)q->ne[2], prefix != nullptr);
 }
 
 int mla_m4_kqkv_paged(const mla_m4_tensor * kcache, const mla_m4_tensor * q, const mla_m4_tensor * past,
@@ -236,6 +237,7 @@ int mla_m4_kqkv_paged(const mla_m4_tensor * kcache, const mla_m4_tensor * q, con
     const int rc = check_attn(kcache, q, past, n_new, table, page_size, prefix, dst);
     if (rc != MLA_M4_OK) return rc;
     if (!std::isfinite(kq_scale)) return MLA_M4_ERR_ARG;
+    if (prefix && !prefix->data) prefix = nullptr;
     const size_t need = mla_m4_kqkv_paged_workspace_bytes(kcache, q, past, prefix, dst);
     if (need > 0 && (!workspace || !aligned16(workspace) || workspace_bytes < need)) return MLA_M4_ERR_WORKSPACE;
     pg::AttnArgs a{};

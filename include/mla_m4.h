@@ -333,8 +333,8 @@ int mla_m4_kqkv_paged(const mla_m4_tensor * kcache, const mla_m4_tensor * q, con
                       const mla_m4_tensor * n_new, const mla_m4_tensor * table, int32_t page_size,
                       const mla_m4_tensor * prefix, float kq_scale, const mla_m4_tensor * dst,
                       void * workspace, size_t workspace_bytes, void * stream);
-/* About 68 MB at D_v 512 and 34 at 256; with a prefix half as much again, 4 D_v bytes for every (token, head)
- * row and 260 D_v for every request. */
+/* About 68 MB at D_v 512 and 34 at 256; with a prefix (any descriptor, also one whose data is not set yet) half
+ * as much again, 4 D_v bytes for every (token, head) row and 260 D_v for every request. */
 size_t mla_m4_kqkv_paged_workspace_bytes(const mla_m4_tensor * kcache, const mla_m4_tensor * q,
                                          const mla_m4_tensor * past, const mla_m4_tensor * prefix,
                                          const mla_m4_tensor * dst);
