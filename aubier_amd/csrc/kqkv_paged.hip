@@ -25,7 +25,8 @@
 // heads, 82 us; 48 of 300 to 9,000, 32 heads, 43.8; 64 of 150 to 250 15.9; 64 behind 32,768 shared cells 166; 9 requests
 // and a chunk of 700 tokens, 40 heads, 126; one of 200 cells 11.9.  Around the tiles a call spends 2.5 us on the places,
 // 0.8 on a piece's setup, 2 (narrow) to 4 (wide, f16) or 7 (wide, f32) on its q, 1 to 2 on its results, and 4 to 22 on the
-// second launch, whose bytes are the records'.
+// second launch, whose bytes are the records'.  Requests without tokens cost a workgroup that passes them between two
+// groups 0.09 us each: 5 live ones of 9,000 cells among 5, 256, 1,024 and 4,096 slots 22, 26, 44 and 119 us.
 //
 // All positions on the line are computed by the same expressions in every workgroup (in 64-bit floating point, exact
 // for multiples of a quarter below 2^51, which MAX_LINE keeps them), so the workgroups agree where one ends and the next
@@ -623,7 +624,9 @@ static hipError_t launch(bool q8, const AttnArgs & a, hipStream_t stream) {
     // The card starts some 400 workgroups per us, so as many as take part at once, no more; the fewer rows, the more
     // pieces each has.  Device times of whole calls either side of a limit, the smaller form first: 96 rows 19.2, 21.9 us
     // and 192 rows 38.7, 41.1; 384 rows 25.0, 29.6 and 1,536 44.7, 45.6, but 2,048 70.8, 68.6; 2,048 rows 69.5, 79.4,
-    // 6,400 28.8, 28.9, 32,000 78.4, 77.2.
+    // 6,400 28.8, 28.9, 32,000 78.4, 77.2.  The rows that count are those there is room for, as the lengths are on the device:
+    // few live rows of many pieces in a call with much room take the last form: 2 requests of 60,000 cells, 32 heads, 34.6
+    // us in a call of 2 rows, 139 in one of 256; 256 requests of 200 cells 20.8.
     const auto wgs = [=](int r) { return dim3((rows + r - 1) / r, DV / 16); };
     if (rows <= 256) hipLaunchKernelGGL((kqkv_paged_merge_few_kernel<DV, 512, 8>), wgs(8), dim3(512), 0, stream, a);
     else if (rows <= 1536) hipLaunchKernelGGL((kqkv_paged_merge_few_kernel<DV, NTHR, 32>), wgs(32), dim3(NTHR), 0, stream, a);

@@ -48,6 +48,9 @@ struct Piece {
 // maximum; M_NONE: keys were seen, but no score is above -inf; -inf: no key was seen, and o need not be there), then o / l in f16 as the accumulators' lanes hold it, so that neither side needs LDS: for every
 // 32 rows D_v / 16 slabs of 1 KB, slab s holding columns 16 s .. + 15, lane l's 8 of them (of row l & 31, the upper 8 in
 // the upper half) at 16 l.
+// Why f16: |o / l| <= max |V| cannot overflow, and records are half the bytes; in f32 the calls whose groups are cut took 7
+// to 15% longer.  The rounding moves a result by 2.0e-4 (relative 2-norm), as much as storing the result in f16 does; a
+// group in one piece has none.
 template <int DV>
 constexpr size_t record_bytes() { return BLOCK_ROWS * 8 + (size_t)BLOCK_ROWS * DV * 2; }
 
@@ -332,11 +335,15 @@ __device__ __forceinline__ void scale_acc(f32x16 (&o)[N], float f) {
 }
 
 // ---------------------------------------------------------------- up to 32 rows
-// Bound by the memory: 480 MB of four long contexts in 76 us, 6.3 TB/s, a tile of 72 KB per workgroup in 2.75 us; the
-// next tile's DMA is spread through this one's Q.K^T.  A tile's latency, 2 us where a workgroup has the card to itself, is why
+// Over an f16 cache bound by the memory: 480 MB of four long contexts in 76 us, 6.3 TB/s (counters: 1.002 of the bytes read,
+// matrix pipes busy in 14% of the cycles), a tile of 72 KB per workgroup in 2.75 us; the next tile's DMA is spread through
+// this one's Q.K^T.  Over an 8-bit cache by the conversion's instructions and the waits at four phases' barriers: 48 requests of
+// 300 to 9,000 cells at (320, 256) run at 1.9 TB/s, 53 MB in 28 us, where reading alone takes 10.  A tile's latency, 2 us where a workgroup has the card to itself, is why
 // small batches are cut into single tiles.
 // Rows of q are reached by 32-bit offsets from the first token's (Q_SPAN, which the host checks); a 64-bit address per
 // lane (global_load_lds) takes 1 to 2 us more a piece.
+// q enters Q.K^T as f16, the weights P.V as f16: the matrix instructions for f32 operands have an eighth of their rate.  A weight's
+// rounding moves a result by 1.0e-4 (relative 2-norm; 200 cells, 32 heads), an f32 q's by 3.4e-4.
 // Eight rows of f32 q into LDS by a wavefront: DMA instruction i brings chunks 8 i .. 8 i + 7 (16 bytes) of every row, lane
 // l's to 1 KB block i at 16 l.  squeeze() then turns them into f16 in place, row r's 16-byte chunk c at
 // 1024 (c >> 3) + 128 r + 16 ((c & 7) ^ r) of the first half: the fragments' reads find no bank twice.
@@ -539,9 +546,11 @@ __device__ __forceinline__ void narrow_piece(const AttnArgs & a, const Piece & p
 }
 
 // ---------------------------------------------------------------- up to 128 rows
-// Bound by the matrix cores' power, then by LDS reads (each wave reads the whole tile: 0.55 MB a tile and CU): 4.24 us a
-// tile on all CUs, 1.08 PFLOP/s, at (576, 512), 2.46 at (320, 256); over an 8-bit cache 4.71 and 2.72, as the slices'
-// conversion stands between two barriers.
+// 4.24 us a tile on all CUs, 1.08 PFLOP/s, at (576, 512), 2.46 at (320, 256); over an 8-bit cache 4.71 and 2.72, as the
+// slices' conversion stands between two barriers.  Counters at (576, 512): the matrix pipes are busy in 44% of the cycles,
+// the LDS pipe in 45% (each wave reads the whole tile, 0.55 MB a tile and CU; half of it bank conflicts of the transpose
+// reads), at 2.0 GHz of the card's 2.4.  No unit is full: with every register taken there is one wave per SIMD, and its
+// chain of operand reads, products and exponentials takes the time.
 // A wave's int8 slice at src -> its f16 slot at dst: per lane, half-blocks (16 values) of one row
 template <int DK>
 __device__ __forceinline__ void slice_to_f16(const char * src, char * dst, int lane) {
