@@ -146,10 +146,11 @@ int check_attn(const mla_m4_tensor * kc, const mla_m4_tensor * q, const mla_m4_t
     if (rc != MLA_M4_OK) return rc;
     if (kc->ne[1] < page_size) return MLA_M4_ERR_SHAPE;         // not one page
     if (!pg::attn_supported((int)(kc->ne[0] > 4096 ? 0 : kc->ne[0]), (int)(dst->ne[0] > 4096 ? 0 : dst->ne[0]))) return MLA_M4_ERR_UNSUPPORTED;
-    if (kc->nb[1] > pg::MAX_STRIDE || q->nb[1] > pg::Q_SPAN || q->nb[2] > pg::Q_SPAN ||
-        127 * (int64_t)q->nb[2] + q->ne[1] * (int64_t)q->nb[1] > pg::Q_SPAN)
-        return MLA_M4_ERR_UNSUPPORTED;
     if (q->ne[1] > 1024 || q->ne[2] > pg::MAX_ROWS || kc->ne[1] / page_size > INT32_MAX) return MLA_M4_ERR_UNSUPPORTED;
+    if (kc->nb[1] > pg::MAX_STRIDE || q->nb[1] > pg::Q_SPAN || q->nb[2] > pg::Q_SPAN) return MLA_M4_ERR_UNSUPPORTED;
+    // 128 rows, to the end of the last one (of a single head nb[1] says nothing about a row's length)
+    const int64_t row_end = q->ne[1] > 1 ? q->ne[1] * (int64_t)q->nb[1] : q->ne[0] * (int64_t)es;
+    if (127 * (int64_t)q->nb[2] + row_end > pg::Q_SPAN) return MLA_M4_ERR_UNSUPPORTED;
     if ((double)(q->ne[1] * q->ne[1] * q->ne[2]) * ((double)table->ne[0] * page_size) > pg::MAX_LINE) return MLA_M4_ERR_UNSUPPORTED;
     return MLA_M4_OK;
 }

@@ -313,7 +313,8 @@ int mla_m4_kvrows(const mla_m4_tensor * x, const mla_m4_tensor * kv_norm, const 
  *   kcache  F16 ne [D_k, n_cells]   nb[1] a multiple of 16 (at most 32 MiB); or Q8_0, contiguous rows;
  *                                   16-byte aligned.  Of any size: there is no 4 GiB bound
  *   q       F32|F16 ne [D_k, H, nt] nb[0] = element size, 16-byte aligned strides, H <= 1024,
- *                                   H nb[1] + 127 nb[2] <= 2 GiB (128 rows of q are read by 32-bit offsets),
+ *                                   H nb[1] + 127 nb[2] <= 2 GiB (128 rows of q are read by 32-bit offsets; of
+ *                                   a single head its row's bytes for nb[1]),
  *                                   H^2 nt max_pages page_size <= 2^60
  *   prefix  I32 ne [2], or NULL     (cells, requests): the tables of the first `requests` requests begin
  *                                   with the same pages, for at least `cells` cells.  Where that is less

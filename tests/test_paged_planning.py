@@ -21,3 +21,18 @@ def test_workspace_of_a_prefix_that_is_not_allocated():
         return lib.mla_m4_kqkv_paged_workspace_bytes(*(ctypes.byref(v) if v is not None else None for v in views))
 
     assert need(prefix, True) == need(prefix, False) > need(None, True) == need(None, False) > 0
+
+
+def test_the_rows_of_one_head_end_inside_their_span():
+    """128 rows of q are reached by 32-bit offsets, the last one's end too; a single head's stride says nothing of its length."""
+    i32, h = torch.int32, torch.float16
+    room = torch.empty((1 << 30) + (1 << 12), dtype=h)                           # (never touched)
+    kc, past, table, out = torch.zeros((640, 576), dtype=h), torch.zeros(2, dtype=i32), torch.zeros((2, 9), dtype=i32), torch.zeros((1, 128, 512))
+
+    def fits(token_bytes, head_bytes):
+        q = room.as_strided((128, 1, 576), (token_bytes // 2, head_bytes // 2, 1))
+        return A.supports_kqkv_paged(kc, q, past, past, table, 64, None, out)
+
+    assert 127 * 16909296 + 1152 <= 2 ** 31 < 127 * 16909312 + 1152
+    for head_bytes in (16, 1152):
+        assert fits(16909296, head_bytes) and not fits(16909312, head_bytes)
