@@ -374,7 +374,8 @@ __global__ __launch_bounds__(NTHR, 1) void kqkv_paged_kernel(AttnArgs a) {
             p.ta = uni(tile_at(k.x0));
             p.tb = uni(tile_at(k.x1));
             first = uni(g0 >= k.x0);                     // the group's first piece says how many there are
-            p.slot = direct ? -1 : uni((b < k.n_share ? SHARED_RECORDS + k.g : first ? 0 : N_WG) + wg);
+            // (in range whatever the lengths: something that writes them during a call must not turn into an address)
+            p.slot = direct ? -1 : uni(min((b < k.n_share ? SHARED_RECORDS + k.g : first ? 0 : N_WG) + wg, a.n_records - 1));
             if (first && !direct) {
                 int e = min(max((int)(g1 / k.per), wg + 1), k.n_wg);
                 while (e > wg + 1 && k.edge(e - 1) >= g1) --e;
@@ -429,30 +430,33 @@ __global__ __launch_bounds__(NTHR, 1) void kqkv_paged_kernel(AttnArgs a) {
 }
 
 // ---------------------------------------------------------------- the merge
-// The pieces of a row: those of its own group, then those of its shared block
+// The pieces of a row: those of its own group, then those of its shared block.  What the workspace says is brought into range
+// (rows, counts, records): another call that writes it between the two launches spoils results, not memory.
 struct RowPieces {
-    int n, n_own, own, shared, r_own, r_shared;
+    int n, n_own, own, shared, r_own, r_shared, last;
     bool shares;
     __device__ __forceinline__ RowPieces(const AttnArgs & a, const Head & head, int row) {
         // (both read at once, whatever the row: the entries lie in the workspace also where there is no such row)
         const int at = min(row, a.n_head * a.nt - 1);
         const Pieces o = reinterpret_cast<const Pieces *>(a.work + own_off(a.n_head, a.nt))[at];
         const Pieces s = reinterpret_cast<const Pieces *>(a.work + shared_off())[at / BLOCK_ROWS];
-        n_own = row < head.rows ? (int)(o.n_row & 0xffffu) : 0;
-        r_own = (int)(o.n_row >> 16);
+        const int live = row <= at ? row : 0x7fffffff;
+        n_own = live < head.rows ? min((int)(o.n_row & 0xffffu), N_WG) : 0;
+        r_own = (int)(o.n_row >> 16) % BLOCK_ROWS;
         own = o.slot;
         shared = s.slot;
         r_shared = at % BLOCK_ROWS;
-        shares = row < head.shared_rows;
-        n = n_own + (shares ? (int)s.n_row : 0);
+        shares = live < head.shared_rows;
+        n = n_own + (shares ? (int)min(s.n_row, (unsigned)N_WG) : 0);
+        last = a.n_records - 1;
     }
     // piece q's record, and the row's place in it
     template <int DV>
     __device__ __forceinline__ const char * at(const char * records, int q, int & r) const {
         const bool mine = q < n_own;
         r = mine ? r_own : r_shared;
-        const int of_own = own + q + (q > 0 && !shares ? N_WG : 0);
-        return records + (size_t)(mine ? of_own : shared + q - n_own) * record_bytes<DV>();
+        const unsigned of_own = (unsigned)own + (unsigned)(q + (q > 0 && !shares ? N_WG : 0));
+        return records + (size_t)min(mine ? of_own : (unsigned)shared + (unsigned)(q - n_own), (unsigned)last) * record_bytes<DV>();
     }
 };
 
@@ -605,12 +609,16 @@ __global__ __launch_bounds__(NTHR) void kqkv_paged_merge_kernel(AttnArgs a) {
 
 bool attn_supported(int dk, int dv) { return (dk == 576 && dv == 512) || (dk == 320 && dv == 256); }
 
-size_t attn_workspace_bytes(int dv, int n_seq, int n_head, int nt, bool prefix) {
+int attn_records(int n_seq, int n_head, int nt, bool prefix) {
     // the sharing rows' records: one per workgroup and group, shared blocks and own ones, of which each request with
     // tokens has at most one that is not full
     size_t n = SHARED_RECORDS;
     if (prefix) n += N_WG + 2 * shared_blocks(n_head, nt) + (size_t)(n_seq < nt ? n_seq : nt);
-    return records_off(n_head, nt) + n * (dv == 512 ? record_bytes<512>() : record_bytes<256>());
+    return (int)n;
+}
+
+size_t attn_workspace_bytes(int dv, int n_seq, int n_head, int nt, bool prefix) {
+    return records_off(n_head, nt) + (size_t)attn_records(n_seq, n_head, nt, prefix) * (dv == 512 ? record_bytes<512>() : record_bytes<256>());
 }
 
 template <int DK, int DV>

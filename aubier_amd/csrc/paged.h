@@ -67,8 +67,10 @@ struct AttnArgs {
     float scale_log2;
     int n_seq, max_pages, n_pages, page_shift, n_head, nt;
     int q_f16, dst_f16;
+    int n_records;          // what the workspace holds
 };
 bool attn_supported(int dk, int dv);
+int attn_records(int n_seq, int n_head, int nt, bool prefix);
 size_t attn_workspace_bytes(int dv, int n_seq, int n_head, int nt, bool prefix);
 // n_head^2 nt and the cells that a table lists: the line of work (kqkv_paged.hip), in units of a tenth of a tile's cost by
 // n_head, is at most 10 / 8192 of it long and 2^49 for the requests' last blocks, so it stays below 2^51

@@ -263,6 +263,7 @@ int mla_m4_kqkv_paged(const mla_m4_tensor * kcache, const mla_m4_tensor * q, con
     a.nt = (int)q->ne[2];
     a.q_f16 = q->type == MLA_M4_TYPE_F16;
     a.dst_f16 = dst->type == MLA_M4_TYPE_F16;
+    a.n_records = pg::attn_records(a.n_seq, a.n_head, a.nt, a.prefix != nullptr);
     return pg::launch_attn((int)kcache->ne[0], (int)dst->ne[0], kcache->type == MLA_M4_TYPE_Q8_0, a,
                            static_cast<hipStream_t>(stream)) == hipSuccess ? MLA_M4_OK : MLA_M4_ERR_LAUNCH;
 }

@@ -331,7 +331,7 @@ int mla_m4_kvrows(const mla_m4_tensor * x, const mla_m4_tensor * kv_norm, const 
  * computed as f16(q d).  Relative to exact arithmetic on the given values (2-norm) that is 1.0e-4 to 2.3e-4, with an F32
  * q 4e-4, beside an F16 dst's own 2.1e-4.
  * workspace: device memory, >= mla_m4_kqkv_paged_workspace_bytes(), 16-byte aligned, not shared by calls
- * that may overlap. */
+ * that may overlap (their results would be wrong; nothing outside the operands is touched). */
 int mla_m4_kqkv_paged(const mla_m4_tensor * kcache, const mla_m4_tensor * q, const mla_m4_tensor * past,
                       const mla_m4_tensor * n_new, const mla_m4_tensor * table, int32_t page_size,
                       const mla_m4_tensor * prefix, float kq_scale, const mla_m4_tensor * dst,
