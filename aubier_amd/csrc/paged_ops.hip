@@ -128,11 +128,14 @@ __global__ __launch_bounds__(NTHR) void kvrows_kernel(KvRowsArgs a) {
                 *reinterpret_cast<half4 *>(row + 2 * c) = h;
             }
         } else {
-            // ggml's f32 -> q8_0 rounding: d = max / 127, q = roundf(x * (1 / d)), d stored as f16
-            float m = fmaxf(fmaxf(fabsf(v[i][0]), fabsf(v[i][1])), fmaxf(fabsf(v[i][2]), fabsf(v[i][3])));
-            m = fmaxf(m, dpp_xor<1>(m));
-            m = fmaxf(m, dpp_xor<2>(m));
-            m = fmaxf(m, dpp_xor<4>(m));
+            // ggml's f32 -> q8_0 rounding: d = max / 127, q = roundf(x * (1 / d)), d stored as f16.  The maximum is taken of the
+            // bit patterns, which order magnitudes and put a NaN above them all: its block's d is NaN
+            auto size = [](float x) { return __float_as_uint(fabsf(x)); };
+            uint32_t top = max(max(size(v[i][0]), size(v[i][1])), max(size(v[i][2]), size(v[i][3])));
+            top = max(top, __float_as_uint(dpp_xor<1>(__uint_as_float(top))));
+            top = max(top, __float_as_uint(dpp_xor<2>(__uint_as_float(top))));
+            top = max(top, __float_as_uint(dpp_xor<4>(__uint_as_float(top))));
+            const float m = __uint_as_float(top);
             const float d = m / 127.0f, id = d != 0.0f ? 1.0f / d : 0.0f;
             uint32_t q[4];
 #pragma unroll

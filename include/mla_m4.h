@@ -300,9 +300,10 @@ int mla_m4_pages(const mla_m4_tensor * past, const mla_m4_tensor * n_new, const 
  *   dst      F32 ne [d_lat + n_dims, n_rows]      Kcur, 16-byte aligned rows; or NULL
  * Columns [0, d_lat): x / sqrt(mean of squares + eps) * kv_norm; [d_lat, d_lat + n_dims): rope, NORMAL
  * mode with YaRN, as phase 0, the angles taken in 64 bits.  The row goes to cache row slot, rounded as
- * phase 0 does (f16, or ggml's f32 -> q8_0); a slot outside [0, n_cells) stores nothing.  Kcur is
- * written for every row.  Slots are distinct: of two rows with one slot, either's values may end up
- * there.  d_lat and n_dims multiples of 32, n_dims <= 256, d_lat + n_dims <= 1024, n_rows <= 2^24. */
+ * phase 0 does (f16, or ggml's f32 -> q8_0; a block of 32 values that holds a NaN gets a NaN scale); a slot
+ * outside [0, n_cells) stores nothing.  Kcur is written for every row.  Slots are distinct: of two rows with
+ * one slot, either's values may end up there.  d_lat and n_dims multiples of 32, n_dims <= 256,
+ * d_lat + n_dims <= 1024, n_rows <= 2^24. */
 int mla_m4_kvrows(const mla_m4_tensor * x, const mla_m4_tensor * kv_norm, const mla_m4_tensor * kcache,
                   const mla_m4_tensor * slot, const mla_m4_tensor * pos, const mla_m4_rope_params * rope,
                   const mla_m4_tensor * dst, void * stream);
