@@ -520,6 +520,11 @@ def supports_phase_kvwrite(cur, wkv_a, kv_norm, kcache, kidx, pos, rope: RopePar
 
 
 # ------------------------------------------------------------------------------------ paged batches
+def _page_size(n: int) -> int:
+    """The page size for a call, 0 (which is refused) for what is no int32: ctypes would take its lower 32 bits."""
+    return int(n) if -2 ** 31 <= n < 2 ** 31 else 0
+
+
 def ggml_m4_pages(past: torch.Tensor, n_new: torch.Tensor, free: torch.Tensor, table: torch.Tensor, page_size: int, n_rows: int,
                   slot: Optional[torch.Tensor] = None, pos: Optional[torch.Tensor] = None, used: Optional[torch.Tensor] = None):
     """Block tables and slot maps from request lengths (include/mla_m4.h mla_m4_pages): past, n_new int32 [n_seq];
@@ -535,7 +540,7 @@ def ggml_m4_pages(past: torch.Tensor, n_new: torch.Tensor, free: torch.Tensor, t
     pos = torch.empty(n_rows, dtype=torch.int32, device=dev) if pos is None else pos
     used = torch.empty(2, dtype=torch.int32, device=dev) if used is None else used
     (p, n, f, t, s, o, u), gpu = _descriptors("ggml_m4_pages", (past, n_new, free, table, slot, pos, used))
-    _run_on("ggml_m4_pages", gpu, lib.mla_m4_pages, p, n, f, t, page_size, s, o, u)
+    _run_on("ggml_m4_pages", gpu, lib.mla_m4_pages, p, n, f, t, _page_size(page_size), s, o, u)
     return slot, pos, used
 
 
@@ -586,13 +591,13 @@ def ggml_m4_kqkv_paged(kcache, q: torch.Tensor, past: torch.Tensor, n_new: torch
     elif workspace.get_device() != gpu or not workspace.is_contiguous():
         raise MlaM4Error("ggml_m4_kqkv_paged", -5)
     ws_ptr, ws_bytes = (workspace.data_ptr(), workspace.numel() * workspace.element_size()) if workspace is not None else (None, 0)
-    _run_on("ggml_m4_kqkv_paged", gpu, lib.mla_m4_kqkv_paged, vk, vq, vp, vn, vt, page_size, vf, kq_scale, vo, ws_ptr, ws_bytes)
+    _run_on("ggml_m4_kqkv_paged", gpu, lib.mla_m4_kqkv_paged, vk, vq, vp, vn, vt, _page_size(page_size), vf, kq_scale, vo, ws_ptr, ws_bytes)
     return out
 
 
 def supports_pages(past, n_new, free, table, page_size: int, slot, pos, used) -> bool:
     return bool(load_library().mla_m4_supports_pages(_ptr(view(past)), _ptr(view(n_new)), _ptr(view(free)), _ptr(view(table)),
-                                                     int(page_size), _ptr(view(slot)), _ptr(view(pos)), _ptr(view(used))))
+                                                     _page_size(page_size), _ptr(view(slot)), _ptr(view(pos)), _ptr(view(used))))
 
 
 def supports_kvrows(x, kv_norm, kcache, slot, pos, rope: RopeParams, out) -> bool:
@@ -602,4 +607,4 @@ def supports_kvrows(x, kv_norm, kcache, slot, pos, rope: RopeParams, out) -> boo
 
 def supports_kqkv_paged(kcache, q, past, n_new, table, page_size: int, prefix, out) -> bool:
     return bool(load_library().mla_m4_supports_kqkv_paged(_ptr(view(kcache)), _ptr(view(q)), _ptr(view(past)), _ptr(view(n_new)),
-                                                          _ptr(view(table)), int(page_size), _ptr(view(prefix)), _ptr(view(out))))
+                                                          _ptr(view(table)), _page_size(page_size), _ptr(view(prefix)), _ptr(view(out))))

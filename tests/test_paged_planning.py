@@ -36,3 +36,12 @@ def test_the_rows_of_one_head_end_inside_their_span():
     assert 127 * 16909296 + 1152 <= 2 ** 31 < 127 * 16909312 + 1152
     for head_bytes in (16, 1152):
         assert fits(16909296, head_bytes) and not fits(16909312, head_bytes)
+
+
+def test_page_sizes_past_32_bits():
+    """Refused, not taken for their lower 32 bits."""
+    i32 = lambda *n: torch.zeros(n, dtype=torch.int32)  # noqa: E731
+    for more in (0, 1 << 32, -(1 << 32), 1 << 40):
+        assert (more == 0) == A.supports_pages(i32(4), i32(4), i32(9), i32(4, 8), 64 + more, torch.zeros(10, dtype=torch.int64), i32(10), i32(2))
+        assert (more == 0) == A.supports_kqkv_paged(torch.zeros((640, 320), dtype=torch.float16), torch.zeros(3, 8, 320), i32(2), i32(2), i32(2, 9), 64 + more,
+                                                    None, torch.zeros(8, 3, 256))
