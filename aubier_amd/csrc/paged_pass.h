@@ -218,7 +218,8 @@ __device__ __forceinline__ void clear_nonfinite(char * sb, int lane, uint64_t & 
 // the piece's results have been stored (all waves).  By the definition, of a seen cell whose score is NaN or +inf the
 // whole row is NaN (inf - inf); one of score -inf has weight 0, and the columns in which it is not finite are NaN (0
 // times infinity).  The score's class comes from the cell's non-finite values alone.  The cells are read again, a wavefront
-// per cell, as this hardly ever runs.
+// per cell, as this hardly ever runs; a row that is NaN is not looked at any more, so that a cache full of them takes
+// little longer.
 template <int DK, int DV, bool Q8, bool QF16>
 __device__ __forceinline__ void seen_nonfinite(const AttnArgs & a, const PieceLds<DK, DV, Q8> & sh, char * rec) {
     static_assert(DK % 64 == 0 && DV % 64 == 0, "64 columns at a time");
@@ -236,44 +237,48 @@ __device__ __forceinline__ void seen_nonfinite(const AttnArgs & a, const PieceLd
         }
     };
     const int ka = p.key0 + TK * p.ta, kb = min(p.key1, p.key0 + TK * p.tb);
-    // from the first tile that not all rows see
-    for (int j = max(ka, p.key0 + max(p.lim_min - p.key0, 0) / TK * TK) + w; j < kb; j += NWAVE) {
-        const int id = __builtin_amdgcn_readfirstlane(p.table[j >> a.page_shift]);
-        if (id < 0 || id >= a.n_pages) continue;
-        const char * cell = a.kc + (((int64_t)id << a.page_shift) + (j & ((1 << a.page_shift) - 1))) * a.kc_nb1;
-        float score[2] = {0.0f, 0.0f};                      // of rows lane and 64 + lane
-        bool any = false;
-        for (int d0 = 0; d0 < DK; d0 += 64) {
-            half_t v;
-            if constexpr (Q8) {
-                const char * blk = cell + (d0 + lane) / 32 * 34;
-                v = to_half((float)*reinterpret_cast<const half_t *>(blk) * (float)*reinterpret_cast<const int8_t *>(blk + 2 + (lane & 31)));
-            } else {
-                v = *reinterpret_cast<const half_t *>(cell + 2 * (d0 + lane));
-            }
-            const int bits = __builtin_bit_cast(uint16_t, v);
-            for (uint64_t bad = __builtin_amdgcn_ballot_w64((bits & 0x7c00) == 0x7c00); bad != 0; bad &= bad - 1) {
-                const int at = __builtin_ctzll(bad), d = d0 + at;
-                const float x = (float)__builtin_bit_cast(half_t, (uint16_t)__builtin_amdgcn_readlane(bits, at));
-                any = true;
-#pragma unroll
-                for (int n = 0; n < 2; ++n) {
-                    const int r = lane + 64 * n;
-                    if (j >= sh.lim[r]) continue;           // (0 for a row that is not there)
-                    const char * qd = q + sh.qoff[r];
-                    const half_t qv = QF16 ? reinterpret_cast<const half_t *>(qd)[d] : to_half(reinterpret_cast<const float *>(qd)[d]);
-                    score[n] += (float)qv * x;
+    // two halves of the rows one after the other, row r0 + lane a lane
+#pragma unroll 1
+    for (int r0 = 0; r0 < p.rows; r0 += 64) {
+        const int r = r0 + lane, lim = sh.lim[r];           // (0 for a row that is not there)
+        bool nan = false;
+        // from the first tile that not all rows see
+        for (int j = max(ka, p.key0 + max(p.lim_min - p.key0, 0) / TK * TK) + w; j < kb; j += NWAVE) {
+            bool open = j < lim && !nan;                    // sees the cell, and is not NaN yet
+            if (__builtin_amdgcn_ballot_w64(open) == 0) continue;
+            const int id = __builtin_amdgcn_readfirstlane(p.table[j >> a.page_shift]);
+            if (id < 0 || id >= a.n_pages) continue;
+            const char * cell = a.kc + (((int64_t)id << a.page_shift) + (j & ((1 << a.page_shift) - 1))) * a.kc_nb1;
+            float score = 0.0f;
+#pragma unroll 1
+            for (int d0 = 0; d0 < DK; d0 += 64) {
+                half_t v;
+                if constexpr (Q8) {
+                    const char * blk = cell + (d0 + lane) / 32 * 34;
+                    v = to_half((float)*reinterpret_cast<const half_t *>(blk) * (float)*reinterpret_cast<const int8_t *>(blk + 2 + (lane & 31)));
+                } else {
+                    v = *reinterpret_cast<const half_t *>(cell + 2 * (d0 + lane));
+                }
+                const int bits = __builtin_bit_cast(uint16_t, v);
+                for (uint64_t bad = __builtin_amdgcn_ballot_w64((bits & 0x7c00) == 0x7c00);
+                     bad != 0 && __builtin_amdgcn_ballot_w64(open) != 0; bad &= bad - 1) {
+                    const int at = __builtin_ctzll(bad), d = d0 + at;
+                    const float x = (float)__builtin_bit_cast(half_t, (uint16_t)__builtin_amdgcn_readlane(bits, at));
+                    if (!open) continue;
+                    const half_t qv = QF16 ? reinterpret_cast<const half_t *>(q + sh.qoff[r])[d] : to_half(reinterpret_cast<const float *>(q + sh.qoff[r])[d]);
+                    score += (float)qv * x;
+                    open = score == score;
+                    nan |= !open;
                     if (d < DV) put_nan(r, d);
                 }
             }
+            const float s = score * a.scale_log2;
+            nan |= open && score != 0.0f && !(s < INFINITY);        // (0: the cell holds none)
         }
-        if (!any) continue;
-#pragma unroll
-        for (int n = 0; n < 2; ++n) {
-            const int r = lane + 64 * n;
-            const float s = score[n] * a.scale_log2;
-            if (j >= sh.lim[r] || (s == s && s != INFINITY)) continue;
+        // (the narrow form took the scores before it cleared the cells)
+        if (p.rows > HG && nan) {
             if (p.slot >= 0) reinterpret_cast<f32x2 *>(rec)[r][1] = __builtin_nanf("");
+#pragma unroll 1
             for (int c = 0; c < DV; ++c) put_nan(r, c);
         }
     }

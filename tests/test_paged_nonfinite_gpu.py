@@ -208,3 +208,20 @@ def test_without_a_score_and_without_a_page(dev, absent):
     else:
         assert torch.isnan(got[:, :3]).all()
     assert torch.isfinite(got[:, 3]).all() and (got[:, 4] == 7.0).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("what", ["nan", "inf", "column"])
+@pytest.mark.parametrize("past,new,H", [([0, 30], [300, 2], 32), ([9000, 10], [9, 3], 40), ([5, 40], [90, 1], 1)])
+def test_a_request_full_of_them(dev, what, past, new, H):
+    """Every cell of a request NaN, infinite throughout, or infinite in one column."""
+    b = Batch(dev, past, new, 16, dk=320, H=H, seed=H, pad=1, poison=1.0)
+    j = torch.arange(past[0] + new[0], device=dev)
+    cells = b.table[0, j // 16].long() * 16 + j % 16
+    if what == "nan":
+        b.kc[cells] = NAN
+    elif what == "inf":
+        b.kc[cells] = torch.where(b.kc[cells] > 0, INF, -INF).half()
+    else:
+        b.kc[cells, 7] = INF
+    check(b, b.run(), what)
