@@ -22,8 +22,8 @@
 //
 // What it comes to (device times in a graph, both launches; narrow pieces read at 6.3 TB/s, wide ones run at 1.08
 // PFLOP/s, where a large copy moves 5.2 and a large f16 matrix product 1.18): 4 requests of 90,000 to 131,000 cells, 16
-// heads, 82 us; 48 of 300 to 9,000, 32 heads, 43.8; 64 of 150 to 250 15.9; 64 behind 32,768 shared cells 166; 9 requests
-// and a chunk of 700 tokens, 40 heads, 126; one of 200 cells 11.9.  Around the tiles a call spends 2.5 us on the places,
+// heads, 82 us; 48 of 300 to 9,000, 32 heads, 44.1; 64 of 150 to 250 15.9; 64 behind 32,768 shared cells 166; 9 requests
+// and a chunk of 700 tokens, 40 heads, 127; one of 200 cells 11.9.  Around the tiles a call spends 2.5 us on the places,
 // 0.8 on a piece's setup, 2 (narrow) to 4 (wide, f16) or 7 (wide, f32) on its q, 1 to 2 on its results, and 4 to 22 on the
 // second launch, whose bytes are the records'.  Requests without tokens cost a workgroup that passes them between two
 // groups 0.09 us each: 5 live ones of 9,000 cells among 5, 256, 1,024 and 4,096 slots 22, 26, 44 and 119 us.
