@@ -45,9 +45,9 @@ struct Piece {
 };
 
 // Records: (m, l) of the block's 128 rows, m in log2 units (a reference for the scores, at most 15 below their
-// maximum; M_NONE: keys were seen, but no score is above -inf; -inf: no key was seen, and o need not be there), then o / l in f16 as the accumulators' lanes hold it, so that neither side needs LDS: for every
-// 32 rows D_v / 16 slabs of 1 KB, slab s holding columns 16 s .. + 15, lane l's 8 of them (of row l & 31, the upper 8 in
-// the upper half) at 16 l.
+// maximum; M_NONE: keys were seen, but no score is above -inf; -inf: no key was seen, and o need not be there), then
+// o / l in f16 as the accumulators' lanes hold it, so that neither side needs LDS: for every 32 rows D_v / 16 slabs of 1 KB,
+// slab s holding columns 16 s .. + 15, lane l's 8 of them (of row l & 31, the upper 8 in the upper half) at 16 l.
 // Why f16: |o / l| <= max |V| cannot overflow, and records are half the bytes; in f32 the calls whose groups are cut took 7
 // to 15% longer.  The rounding moves a result by 2.0e-4 (relative 2-norm), as much as storing the result in f16 does; a
 // group in one piece has none.
@@ -342,13 +342,13 @@ __device__ __forceinline__ void scale_acc(f32x16 (&o)[N], float f) {
 // ---------------------------------------------------------------- up to 32 rows
 // Over an f16 cache bound by the memory: 480 MB of four long contexts in 76 us, 6.3 TB/s (counters: 1.002 of the bytes read,
 // matrix pipes busy in 14% of the cycles), a tile of 72 KB per workgroup in 2.75 us; the next tile's DMA is spread through
-// this one's Q.K^T.  Over an 8-bit cache by the conversion's instructions and the waits at four phases' barriers: 48 requests of
-// 300 to 9,000 cells at (320, 256) run at 1.9 TB/s, 53 MB in 28 us, where reading alone takes 10.  A tile's latency, 2 us where a workgroup has the card to itself, is why
-// small batches are cut into single tiles.
+// this one's Q.K^T.  Over an 8-bit cache by the conversion's instructions and the waits at four phases' barriers: 48 requests
+// of 300 to 9,000 cells at (320, 256) run at 1.9 TB/s, 53 MB in 28 us, where reading alone takes 10.  A tile's latency, 2 us
+// where a workgroup has the card to itself, is why small batches are cut into single tiles.
 // Rows of q are reached by 32-bit offsets from the first token's (Q_SPAN, which the host checks); a 64-bit address per
 // lane (global_load_lds) takes 1 to 2 us more a piece.
-// q enters Q.K^T as f16, the weights P.V as f16: the matrix instructions for f32 operands have an eighth of their rate.  A weight's
-// rounding moves a result by 1.0e-4 (relative 2-norm; 200 cells, 32 heads), an f32 q's by 3.4e-4.
+// q enters Q.K^T as f16, the weights P.V as f16: the matrix instructions for f32 operands have an eighth of their rate.  The
+// weights' rounding moves a result by 1.0e-4 (relative 2-norm; 200 cells, 32 heads), an f32 q's by 3.4e-4.
 // Eight rows of f32 q into LDS by a wavefront: DMA instruction i brings chunks 8 i .. 8 i + 7 (16 bytes) of every row, lane
 // l's to 1 KB block i at 16 l.  squeeze() then turns them into f16 in place, row r's 16-byte chunk c at
 // 1024 (c >> 3) + 128 r + 16 ((c & 7) ^ r) of the first half: the fragments' reads find no bank twice.
