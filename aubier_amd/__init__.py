@@ -13,6 +13,14 @@ from .ops import (  # noqa: F401
     ggml_m4_pages,
     kqkv_paged_workspace_bytes,
     supports_kqkv_paged,
+    ggml_m4_mul_i8,
+    ggml_m4_norm,
+    ggml_m4_qrope,
+    ggml_m4_rows_i8,
+    supports_mul_i8,
+    supports_norm,
+    supports_qrope,
+    supports_rows_i8,
     supports_kvrows,
     supports_pages,
     ggml_m4_phase_kvwrite,

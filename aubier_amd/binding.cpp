@@ -1,4 +1,4 @@
-// binding.cpp -- the paged operators' calls from Python, compiled (aubier_amd/_binding.so).
+// binding.cpp -- the calls of a paged batch's operators from Python, compiled (aubier_amd/_binding.so).
 //
 // A paged batch's calls run once per step or layer on a handful of small tensors, and the device's time is 3 to 12 us
 // each, so what the host adds counts: descriptors straight from the tensors instead of by Python and ctypes, and outputs
@@ -21,6 +21,10 @@ struct {
     decltype(&mla_m4_kvrows) kvrows;
     decltype(&mla_m4_kqkv_paged) kqkv_paged;
     decltype(&mla_m4_kqkv_paged_workspace_bytes) workspace_bytes;
+    decltype(&mla_m4_norm) norm;
+    decltype(&mla_m4_rows_i8) rows_i8;
+    decltype(&mla_m4_mul_i8) mul_i8;
+    decltype(&mla_m4_qrope) qrope;
 } lib;
 
 // The descriptors of a call's tensors, all on one GPU
@@ -35,6 +39,7 @@ struct Call {
         switch (t.scalar_type()) {
             case at::kFloat: type = MLA_M4_TYPE_F32; break;
             case at::kHalf: type = MLA_M4_TYPE_F16; break;
+            case at::kChar: type = MLA_M4_TYPE_I8; break;
             case at::kInt: type = MLA_M4_TYPE_I32; break;
             case at::kLong: type = MLA_M4_TYPE_I64; break;
             default: status = MLA_M4_ERR_TYPE; return nullptr;
@@ -99,13 +104,14 @@ at::Tensor given_or_new(PyObject * o, at::IntArrayRef size, at::ScalarType type,
 
 c10::Device gpu(int i) { return c10::Device(c10::DeviceType::CUDA, (c10::DeviceIndex)i); }
 
-// bind(pages, kvrows, kqkv_paged, workspace_bytes): addresses
+// bind(pages, kvrows, kqkv_paged, workspace_bytes, norm, rows_i8, mul_i8, qrope): addresses
 PyObject * bind(PyObject *, PyObject * const * args, Py_ssize_t n) {
-    if (n != 4) return PyErr_Format(PyExc_TypeError, "four addresses");
-    void * p[4];
-    for (int i = 0; i < 4; ++i) p[i] = PyLong_AsVoidPtr(args[i]);
+    if (n != 8) return PyErr_Format(PyExc_TypeError, "eight addresses");
+    void * p[8];
+    for (int i = 0; i < 8; ++i) p[i] = PyLong_AsVoidPtr(args[i]);
     if (PyErr_Occurred()) return nullptr;
-    lib = {(decltype(lib.pages))p[0], (decltype(lib.kvrows))p[1], (decltype(lib.kqkv_paged))p[2], (decltype(lib.workspace_bytes))p[3]};
+    lib = {(decltype(lib.pages))p[0], (decltype(lib.kvrows))p[1], (decltype(lib.kqkv_paged))p[2], (decltype(lib.workspace_bytes))p[3],
+           (decltype(lib.norm))p[4], (decltype(lib.rows_i8))p[5], (decltype(lib.mul_i8))p[6], (decltype(lib.qrope))p[7]};
     Py_RETURN_NONE;
 }
 
@@ -189,11 +195,124 @@ PyObject * kqkv_paged(PyObject *, PyObject * const * a, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
+// the type of a float or int8 result by its number, MLA_M4_TYPE_*
+at::ScalarType float_or_i8(long type) { return type == MLA_M4_TYPE_F16 ? at::kHalf : type == MLA_M4_TYPE_I8 ? at::kChar : at::kFloat; }
+
+// the results of a call, None for a tensor that is not there
+PyObject * results(std::initializer_list<at::Tensor> ts) {
+    PyObject * r = PyTuple_New((Py_ssize_t)ts.size());
+    if (r == nullptr) return nullptr;
+    Py_ssize_t i = 0;
+    for (const at::Tensor & t : ts) {
+        PyObject * o = Py_None;
+        if (t.defined()) o = THPVariable_Wrap(t);
+        else Py_INCREF(o);
+        PyTuple_SET_ITEM(r, i++, o);
+    }
+    return r;
+}
+
+// norm(x, post, gate, res, scale, pre, eps, res_out, out, out_scale, type, stream) -> (res_out, out, out_scale)
+PyObject * norm(PyObject *, PyObject * const * a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    if (n != 12) return PyErr_Format(PyExc_TypeError, "twelve arguments");
+    if (!tensors(a, 1) || !tensors(a + 1, 3, true) || !tensors(a + 5, 1, true) || !tensors(a + 7, 3, true)) return nullptr;
+    const double scale = PyFloat_AsDouble(a[4]), eps = PyFloat_AsDouble(a[6]);
+    const long type = PyLong_AsLong(a[10]);
+    void * stream = PyLong_AsVoidPtr(a[11]);
+    if (PyErr_Occurred()) return nullptr;
+    const at::Tensor & x = THPVariable_Unpack(a[0]);
+    if (x.dim() != 2) return PyLong_FromLong(MLA_M4_ERR_SHAPE);
+    at::Tensor res_out, out, out_scale;
+    if (a[7] != Py_None) res_out = THPVariable_Unpack(a[7]);
+    else if (a[3] != Py_None) res_out = at::empty(x.sizes(), at::TensorOptions().dtype(THPVariable_Unpack(a[3]).scalar_type()).device(x.device()));
+    if (type >= 0 || a[8] != Py_None) out = given_or_new(a[8], x.sizes(), float_or_i8(type), x);
+    if (a[9] != Py_None) out_scale = THPVariable_Unpack(a[9]);
+    else if (out.defined() && out.scalar_type() == at::kChar) out_scale = at::empty({x.size(0)}, at::TensorOptions().dtype(at::kFloat).device(x.device()));
+    Call c;
+    const mla_m4_tensor *vx = c.add(x), *vp = c.add(a[1]), *vg = c.add(a[2]), *vr = c.add(a[3]), *vw = c.add(a[5]);
+    const mla_m4_tensor *vo = res_out.defined() ? c.add(res_out) : nullptr, *vd = out.defined() ? c.add(out) : nullptr;
+    const mla_m4_tensor * vs = out_scale.defined() ? c.add(out_scale) : nullptr;
+    if (c.status == 0) {
+        const c10::DeviceGuard guard(gpu(c.device));
+        c.status = lib.norm(vx, vp, vg, vr, (float)scale, vw, (float)eps, vo, vd, vs, stream);
+    }
+    return c.status != 0 ? PyLong_FromLong(c.status) : results({res_out, out, out_scale});
+    END_HANDLE_TH_ERRORS
+}
+
+// rows_i8(x, out, scale, stream) -> (out, scale)
+PyObject * rows_i8(PyObject *, PyObject * const * a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    if (n != 4) return PyErr_Format(PyExc_TypeError, "four arguments");
+    if (!tensors(a, 1) || !tensors(a + 1, 2, true)) return nullptr;
+    void * stream = PyLong_AsVoidPtr(a[3]);
+    if (PyErr_Occurred()) return nullptr;
+    const at::Tensor & x = THPVariable_Unpack(a[0]);
+    if (x.dim() != 2 && x.dim() != 3) return PyLong_FromLong(MLA_M4_ERR_SHAPE);
+    const at::Tensor out = given_or_new(a[1], {x.size(0), x.dim() == 3 ? x.size(1) * x.size(2) : x.size(1)}, at::kChar, x);
+    const at::Tensor scale = given_or_new(a[2], {x.size(0)}, at::kFloat, x);
+    Call c;
+    const mla_m4_tensor *vx = c.add(x), *vd = c.add(out), *vs = c.add(scale);
+    if (c.status == 0) {
+        const c10::DeviceGuard guard(gpu(c.device));
+        c.status = lib.rows_i8(vx, vd, vs, stream);
+    }
+    return c.status != 0 ? PyLong_FromLong(c.status) : results({out, scale});
+    END_HANDLE_TH_ERRORS
+}
+
+// mul_i8(w, w_scale, x, x_scale, out, type, stream) -> out
+PyObject * mul_i8(PyObject *, PyObject * const * a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    if (n != 7) return PyErr_Format(PyExc_TypeError, "seven arguments");
+    if (!tensors(a, 4) || !tensors(a + 4, 1, true)) return nullptr;
+    const long type = PyLong_AsLong(a[5]);
+    void * stream = PyLong_AsVoidPtr(a[6]);
+    if (PyErr_Occurred()) return nullptr;
+    const at::Tensor & w = THPVariable_Unpack(a[0]);
+    const at::Tensor & x = THPVariable_Unpack(a[2]);
+    if (w.dim() != 2 || x.dim() != 2) return PyLong_FromLong(MLA_M4_ERR_SHAPE);
+    const at::Tensor out = given_or_new(a[4], {x.size(0), w.size(0)}, float_or_i8(type), x);
+    Call c;
+    const mla_m4_tensor *vw = c.add(w), *vs = c.add(a[1]), *vx = c.add(x), *vt = c.add(a[3]), *vd = c.add(out);
+    if (c.status == 0) {
+        const c10::DeviceGuard guard(gpu(c.device));
+        c.status = lib.mul_i8(vw, vs, vx, vt, vd, stream);
+    }
+    return c.status != 0 ? PyLong_FromLong(c.status) : THPVariable_Wrap(out);
+    END_HANDLE_TH_ERRORS
+}
+
+// qrope(q, pos, rope, out, stream) -> out; rope: the address of the parameters
+PyObject * qrope(PyObject *, PyObject * const * a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    if (n != 5) return PyErr_Format(PyExc_TypeError, "five arguments");
+    if (!tensors(a, 2) || !tensors(a + 3, 1, true)) return nullptr;
+    const auto * rope = static_cast<const mla_m4_rope_params *>(PyLong_AsVoidPtr(a[2]));
+    void * stream = PyLong_AsVoidPtr(a[4]);
+    if (PyErr_Occurred()) return nullptr;
+    const at::Tensor & q = THPVariable_Unpack(a[0]);
+    const at::Tensor out = given_or_new(a[3], q.sizes(), at::kFloat, q);
+    Call c;
+    const mla_m4_tensor *vq = c.add(q), *vp = c.add(a[1]), *vd = c.add(out);
+    if (c.status == 0) {
+        const c10::DeviceGuard guard(gpu(c.device));
+        c.status = lib.qrope(vq, vp, rope, vd, stream);
+    }
+    return c.status != 0 ? PyLong_FromLong(c.status) : THPVariable_Wrap(out);
+    END_HANDLE_TH_ERRORS
+}
+
 PyMethodDef methods[] = {
     {"bind", (PyCFunction)(void *)bind, METH_FASTCALL, nullptr},
     {"pages", (PyCFunction)(void *)pages, METH_FASTCALL, nullptr},
     {"kvrows", (PyCFunction)(void *)kvrows, METH_FASTCALL, nullptr},
     {"kqkv_paged", (PyCFunction)(void *)kqkv_paged, METH_FASTCALL, nullptr},
+    {"norm", (PyCFunction)(void *)norm, METH_FASTCALL, nullptr},
+    {"rows_i8", (PyCFunction)(void *)rows_i8, METH_FASTCALL, nullptr},
+    {"mul_i8", (PyCFunction)(void *)mul_i8, METH_FASTCALL, nullptr},
+    {"qrope", (PyCFunction)(void *)qrope, METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr},
 };
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_binding", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

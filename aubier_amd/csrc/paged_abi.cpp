@@ -11,15 +11,6 @@ namespace {
 using namespace mla::abi;
 namespace pg = mla::paged;
 
-// a vector: ne [n], packed
-int check_vec(const mla_m4_tensor * t, int32_t type, size_t es, int64_t n, bool plan) {
-    if (!has_data(t, plan)) return MLA_M4_ERR_NULL;
-    if (t->type != type) return MLA_M4_ERR_TYPE;
-    if (t->ne[0] != n || t->ne[1] != 1 || t->ne[2] != 1 || t->ne[3] != 1) return MLA_M4_ERR_SHAPE;
-    if ((n != 1 && t->nb[0] != es) || (reinterpret_cast<uintptr_t>(t->data) & (es - 1))) return MLA_M4_ERR_STRIDE;
-    return MLA_M4_OK;
-}
-
 // the lengths of a batch, its block tables and page size
 int check_batch(const mla_m4_tensor * past, const mla_m4_tensor * n_new, const mla_m4_tensor * table, int32_t page_size,
                 bool plan) {
@@ -95,27 +86,9 @@ int check_kvrows(const mla_m4_tensor * x, const mla_m4_tensor * nw, const mla_m4
         if (dst->nb[0] != 4 || (dst->nb[1] & 15u) || (n_rows > 1 && dst->nb[1] < (size_t)n_out * 4) || !al16(dst->data, plan))
             return MLA_M4_ERR_STRIDE;
     }
-    if (!(rp->freq_base > 0.0f) || !(rp->freq_scale > 0.0f) || !(rp->eps >= 0.0f) || rp->n_ctx_orig < 1 ||
-        !std::isfinite(rp->freq_base) || !std::isfinite(rp->freq_scale) || !std::isfinite(rp->eps) ||
-        !std::isfinite(rp->ext_factor) || !std::isfinite(rp->attn_factor) || !(rp->beta_fast > 0.0f) || !(rp->beta_slow > 0.0f))
-        return MLA_M4_ERR_ARG;
+    if (!rope_in_range(rp)) return MLA_M4_ERR_ARG;
     if (n_out > 1024 || n_dims > pg::MAX_ROPE || n_rows > pg::MAX_KV_ROWS) return MLA_M4_ERR_UNSUPPORTED;
     return MLA_M4_OK;
-}
-
-// Turns (of 2 pi) per position of every rope pair, taken in 64 bits: the frequency
-// freq_base^(-2 p / n_dims) times freq_scale (1 - mix) + mix (YaRN's ramp, which is linear in the angle).
-void rope_turns(const mla_m4_rope_params * rp, double * turns) {
-    float corr[2] = {0.0f, 0.0f};
-    if (rp->ext_factor != 0.0f) rope_yarn_corr_dims(rp->n_dims, rp->n_ctx_orig, rp->freq_base, rp->beta_fast, rp->beta_slow, corr);
-    const double width = (double)corr[1] - (double)corr[0];
-    const double step = -2.0 / (double)rp->n_dims * std::log((double)rp->freq_base);
-    for (int p = 0; 2 * p < rp->n_dims; ++p) {
-        double y = ((double)p - (double)corr[0]) / (width > 0.001 ? width : 0.001);
-        y = y < 0.0 ? 0.0 : y > 1.0 ? 1.0 : y;
-        const double mix = (1.0 - y) * (double)rp->ext_factor;
-        turns[p] = std::exp(step * p) * ((double)rp->freq_scale * (1.0 - mix) + mix) / 6.283185307179586476925;
-    }
 }
 
 // ---------------------------------------------------------------- attention over pages
@@ -209,8 +182,7 @@ int mla_m4_kvrows(const mla_m4_tensor * x, const mla_m4_tensor * kv_norm, const 
     a.n_rope = rope->n_dims;
     a.d_lat = (int)x->ne[0] - rope->n_dims;
     a.eps = rope->eps;
-    a.mscale = rope->attn_factor;
-    if (rope->ext_factor != 0.0f) a.mscale *= 1.0f + 0.1f * logf(1.0f / rope->freq_scale);
+    a.mscale = rope_mscale(rope);
     rope_turns(rope, a.turns);
     return pg::launch_kvrows(a, static_cast<hipStream_t>(stream)) == hipSuccess ? MLA_M4_OK : MLA_M4_ERR_LAUNCH;
 }

@@ -112,6 +112,15 @@ _EXPORTS = {
                                                                  ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]),
     "mla_m4_kqkv_paged_workspace_bytes": (ctypes.c_size_t, [ctypes.c_void_p] * 5),
     "mla_m4_supports_kqkv_paged": (ctypes.c_int, [ctypes.c_void_p] * 5 + [ctypes.c_int32] + [ctypes.c_void_p] * 2),
+    # (and those around its attention)
+    "mla_m4_norm": (ctypes.c_int, [ctypes.c_void_p] * 4 + [ctypes.c_float, ctypes.c_void_p, ctypes.c_float] + [ctypes.c_void_p] * 4),
+    "mla_m4_supports_norm": (ctypes.c_int, [ctypes.c_void_p] * 5 + [ctypes.c_float] + [ctypes.c_void_p] * 3),
+    "mla_m4_rows_i8": (ctypes.c_int, [ctypes.c_void_p] * 4),
+    "mla_m4_supports_rows_i8": (ctypes.c_int, [ctypes.c_void_p] * 3),
+    "mla_m4_mul_i8": (ctypes.c_int, [ctypes.c_void_p] * 6),
+    "mla_m4_supports_mul_i8": (ctypes.c_int, [ctypes.c_void_p] * 5),
+    "mla_m4_qrope": (ctypes.c_int, [ctypes.c_void_p] * 5),
+    "mla_m4_supports_qrope": (ctypes.c_int, [ctypes.c_void_p] * 4),
 }
 
 
@@ -136,8 +145,8 @@ def exported_symbols() -> list[str]:
 
 
 # ------------------------------------------------------------------------------------ views
-TYPE_Q8_0, TYPE_I32, TYPE_I64 = 8, 26, 27
-_DT = {torch.float32: (TYPE_F32, 4), torch.float16: (TYPE_F16, 2), torch.int32: (TYPE_I32, 4),
+TYPE_Q8_0, TYPE_I8, TYPE_I32, TYPE_I64 = 8, 24, 26, 27
+_DT = {torch.float32: (TYPE_F32, 4), torch.float16: (TYPE_F16, 2), torch.int8: (TYPE_I8, 1), torch.int32: (TYPE_I32, 4),
        torch.int64: (TYPE_I64, 8)}
 
 
@@ -307,7 +316,8 @@ def _calls():
             _native = False
         else:
             _binding.bind(*(ctypes.cast(getattr(lib, f), ctypes.c_void_p).value for f in (
-                "mla_m4_pages", "mla_m4_kvrows", "mla_m4_kqkv_paged", "mla_m4_kqkv_paged_workspace_bytes")))
+                "mla_m4_pages", "mla_m4_kvrows", "mla_m4_kqkv_paged", "mla_m4_kqkv_paged_workspace_bytes",
+                "mla_m4_norm", "mla_m4_rows_i8", "mla_m4_mul_i8", "mla_m4_qrope")))
             _native = _binding
     return _native
 
@@ -608,3 +618,113 @@ def supports_kvrows(x, kv_norm, kcache, slot, pos, rope: RopeParams, out) -> boo
 def supports_kqkv_paged(kcache, q, past, n_new, table, page_size: int, prefix, out) -> bool:
     return bool(load_library().mla_m4_supports_kqkv_paged(_ptr(view(kcache)), _ptr(view(q)), _ptr(view(past)), _ptr(view(n_new)),
                                                           _ptr(view(table)), _page_size(page_size), _ptr(view(prefix)), _ptr(view(out))))
+
+
+# ------------------------------------------------------------------------------------ around a batch's attention
+_FLOAT_OR_I8 = {torch.float32: TYPE_F32, torch.float16: TYPE_F16, torch.int8: TYPE_I8}
+_FLOAT = {torch.float32: TYPE_F32, torch.float16: TYPE_F16}
+
+
+def _type_for(op: str, dtype, types) -> int:
+    """The type's number; MlaM4Error where a result cannot have it."""
+    try:
+        return types[dtype]
+    except KeyError:
+        raise MlaM4Error(op, -2) from None
+
+
+def ggml_m4_norm(x: torch.Tensor, pre: Optional[torch.Tensor], eps: float, post: Optional[torch.Tensor] = None,
+                 gate: Optional[torch.Tensor] = None, res: Optional[torch.Tensor] = None, scale: float = 1.0,
+                 dtype: Optional[torch.dtype] = torch.float32, res_out: Optional[torch.Tensor] = None,
+                 out: Optional[torch.Tensor] = None, out_scale: Optional[torch.Tensor] = None):
+    """The norms before and after a block with the gate and the residual between them (include/mla_m4.h mla_m4_norm):
+    y = rms(x) * post, r = res + scale * gate * y, h = rms(r) * pre; post, gate, res, pre None: that part is left out (res
+    None: r = gate * y).  x f32 or f16 [rows, n], a block's output; post, pre f32 [n]; gate f32 [n], [rows, 1], [rows, n]
+    or [1]; res f32 or f16 [rows, n].  Returns (r, h, h's scale): r of res's type, None without a res or res_out; h of
+    `dtype` (None: no h), int8 with a scale f32 [rows], else None.  res_out may be res."""
+    ty = -1 if dtype is None else _type_for("ggml_m4_norm", dtype, _FLOAT_OR_I8)
+    calls = _native or _calls()
+    if calls:
+        return _done("ggml_m4_norm", calls.norm(x, post, gate, res, scale, pre, eps, res_out, out, out_scale, ty, _stream_of("ggml_m4_norm", x)))
+    if x.dim() != 2:
+        raise MlaM4Error("ggml_m4_norm", -3)
+    lib = load_library()
+    dev = x.device
+    if res_out is None and res is not None:
+        res_out = torch.empty(x.shape, dtype=res.dtype, device=dev)
+    if out is None and dtype is not None:
+        out = torch.empty(x.shape, dtype=dtype, device=dev)
+    if out_scale is None and out is not None and out.dtype == torch.int8:
+        out_scale = torch.empty(x.shape[0], dtype=torch.float32, device=dev)
+    (vx, p, g, r, w, o, d, s), gpu = _descriptors("ggml_m4_norm", (x, post, gate, res, pre, res_out, out, out_scale))
+    _run_on("ggml_m4_norm", gpu, lib.mla_m4_norm, vx, p, g, r, scale, w, eps, o, d, s)
+    return res_out, out, out_scale
+
+
+def ggml_m4_rows_i8(x: torch.Tensor, out: Optional[torch.Tensor] = None, scale: Optional[torch.Tensor] = None):
+    """Rows in int8 with a scale each (include/mla_m4.h mla_m4_rows_i8): x f32 or f16 [rows, n], or [rows, H, d] of any strides
+    between pieces and rows (wv_b's result [H, rows, d], permuted) -> int8 [rows, n] or [rows, H d], f32 [rows].  Weights,
+    whose rows are channels, are brought into this form by the same call."""
+    calls = _native or _calls()
+    if calls:
+        return _done("ggml_m4_rows_i8", calls.rows_i8(x, out, scale, _stream_of("ggml_m4_rows_i8", x)))
+    if x.dim() not in (2, 3):
+        raise MlaM4Error("ggml_m4_rows_i8", -3)
+    lib = load_library()
+    if out is None:
+        out = torch.empty((x.shape[0], x.shape[1] if x.dim() == 2 else x.shape[1] * x.shape[2]), dtype=torch.int8, device=x.device)
+    if scale is None:
+        scale = torch.empty(x.shape[0], dtype=torch.float32, device=x.device)
+    (vx, d, s), gpu = _descriptors("ggml_m4_rows_i8", (x, out, scale))
+    _run_on("ggml_m4_rows_i8", gpu, lib.mla_m4_rows_i8, vx, d, s)
+    return out, scale
+
+
+def ggml_m4_mul_i8(w: torch.Tensor, w_scale: torch.Tensor, x: torch.Tensor, x_scale: torch.Tensor,
+                   dtype: torch.dtype = torch.float32, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """The product of int8 rows and weights (include/mla_m4.h mla_m4_mul_i8): out[t, c] = x_scale[t] w_scale[c] sum_k w[c, k]
+    x[t, k].  w int8 [N, K], w_scale f32 [N], x int8 [rows, K], x_scale f32 [rows] -> [rows, N] of `dtype` (f32 or f16) or in
+    out."""
+    ty = _type_for("ggml_m4_mul_i8", dtype, _FLOAT)
+    calls = _native or _calls()
+    if calls:
+        return _done("ggml_m4_mul_i8", calls.mul_i8(w, w_scale, x, x_scale, out, ty, _stream_of("ggml_m4_mul_i8", x)))
+    if w.dim() != 2 or x.dim() != 2:
+        raise MlaM4Error("ggml_m4_mul_i8", -3)
+    lib = load_library()
+    if out is None:
+        out = torch.empty((x.shape[0], w.shape[0]), dtype=dtype, device=x.device)
+    (vw, s, vx, t, d), gpu = _descriptors("ggml_m4_mul_i8", (w, w_scale, x, x_scale, out))
+    _run_on("ggml_m4_mul_i8", gpu, lib.mla_m4_mul_i8, vw, s, vx, t, d)
+    return out
+
+
+def ggml_m4_qrope(q: torch.Tensor, pos: torch.Tensor, rope: RopeParams, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """The rope parts of q (include/mla_m4.h mla_m4_qrope): q f32 or f16 [rows, H, n_dims], a view of a product's rows; pos int32
+    [rows] -> [rows, H, n_dims], in out (a view into Qcur, or q itself) or a new f32 tensor."""
+    calls = _native or _calls()
+    if calls:
+        return _done("ggml_m4_qrope", calls.qrope(q, pos, ctypes.addressof(rope), out, _stream_of("ggml_m4_qrope", q)))
+    lib = load_library()
+    if out is None:
+        out = torch.empty(q.shape, dtype=torch.float32, device=q.device)
+    (vq, p, d), gpu = _descriptors("ggml_m4_qrope", (q, pos, out))
+    _run_on("ggml_m4_qrope", gpu, lib.mla_m4_qrope, vq, p, ctypes.addressof(rope), d)
+    return out
+
+
+def supports_norm(x, pre, eps: float, post=None, gate=None, res=None, res_out=None, out=None, out_scale=None) -> bool:
+    v = [_ptr(view(t)) for t in (x, post, gate, res, pre, res_out, out, out_scale)]
+    return bool(load_library().mla_m4_supports_norm(*v[:5], eps, *v[5:]))
+
+
+def supports_rows_i8(x, out, scale) -> bool:
+    return bool(load_library().mla_m4_supports_rows_i8(*(_ptr(view(t)) for t in (x, out, scale))))
+
+
+def supports_mul_i8(w, w_scale, x, x_scale, out) -> bool:
+    return bool(load_library().mla_m4_supports_mul_i8(*(_ptr(view(t)) for t in (w, w_scale, x, x_scale, out))))
+
+
+def supports_qrope(q, pos, rope: RopeParams, out) -> bool:
+    return bool(load_library().mla_m4_supports_qrope(_ptr(view(q)), _ptr(view(pos)), ctypes.byref(rope), _ptr(view(out))))

@@ -33,6 +33,7 @@ enum {
     MLA_M4_TYPE_F32  = 0,
     MLA_M4_TYPE_F16  = 1,
     MLA_M4_TYPE_Q8_0 = 8,
+    MLA_M4_TYPE_I8   = 24,
     MLA_M4_TYPE_I32  = 26,
     MLA_M4_TYPE_I64  = 27
 };
@@ -353,6 +354,82 @@ int mla_m4_supports_kvrows(const mla_m4_tensor * x, const mla_m4_tensor * kv_nor
 int mla_m4_supports_kqkv_paged(const mla_m4_tensor * kcache, const mla_m4_tensor * q, const mla_m4_tensor * past,
                                const mla_m4_tensor * n_new, const mla_m4_tensor * table, int32_t page_size,
                                const mla_m4_tensor * prefix, const mla_m4_tensor * dst);
+
+/* -------------------------------------------------------------------------------------------
+ * Around a batch's attention -- no counterpart in the reference, whose layers take one token through
+ * ggml's own operators: the norms and the residual between two blocks, rows in 8-bit integers with a
+ * scale each, their products with 8-bit weights, and the rope of q.  With them a layer of a batch runs
+ * without any other operator:
+ *   mla_m4_norm (residual, int8 rows), mla_m4_mul_i8 (the latents of q and of the cache), mla_m4_norm
+ *   (q's latents), mla_m4_mul_i8 (q), mla_m4_qrope, mla_m4_wkb, mla_m4_kvrows, mla_m4_kqkv_paged,
+ *   mla_m4_phase_wvb, mla_m4_rows_i8, mla_m4_mul_i8 (the output projection), mla_m4_norm.
+ * A row is a token.  Every row is worked on by itself: what rows of a padded batch hold matters to them
+ * alone.  Where operands may share memory it is said so; otherwise they do not overlap.
+ *
+ * int8 rows.  A row v of finite values is held as integers q in [-127, 127] and one f32 scale:
+ *   top = max |v|,  scale = top / 127,  q = 127 v / top rounded to the nearest, half away from zero
+ * (all zeros: scale 0, q 0).  The integers are exactly these: the rounding is decided in 64 bits.  A row
+ * that holds a NaN or an infinity gets scale NaN and q 0, so its products are NaN.  Where top < 2^-119 the
+ * scale itself is a subnormal f32 and rounds coarser.
+ * ------------------------------------------------------------------------------------------- */
+
+/* The norms before and after a block, with the gate and the residual between them:
+ *   y = x / sqrt(mean(x^2) + eps) * post        (post NULL: y = x)
+ *   r = res + scale * gate * y                  (gate NULL: 1; res NULL: r = gate * y)
+ *   h = r / sqrt(mean(r^2) + eps) * pre         (pre NULL: h = r)
+ *   x       F32|F16 ne [n, rows]       a block's output
+ *   post, pre  F32 ne [n], or NULL     16-byte aligned
+ *   gate    F32 ne [n or 1, rows or 1], or NULL: one for each channel, each row, each value, or one;
+ *           ne[0] = n: rows 16-byte aligned
+ *   res     F32|F16 ne [n, rows], or NULL
+ *   res_out F32|F16 ne [n, rows], or NULL: r, rounded to its type; may be res itself
+ *   dst     F32|F16|I8 ne [n, rows], or NULL (not both NULL): h of the r that is stored (of r in f32 where none is);
+ *           I8: int8 rows as above, of v = r * pre and its root
+ *   dst_scale  F32 ne [rows]           with an I8 dst, else NULL
+ * n a multiple of 4, at most 32768; rows at most 2^24; rows of x, res, res_out and dst aligned to 4 elements.
+ * Computed in 64 bits and rounded once where it is stored (f16 by way of f32). */
+int mla_m4_norm(const mla_m4_tensor * x, const mla_m4_tensor * post, const mla_m4_tensor * gate,
+                const mla_m4_tensor * res, float scale, const mla_m4_tensor * pre, float eps,
+                const mla_m4_tensor * res_out, const mla_m4_tensor * dst, const mla_m4_tensor * dst_scale,
+                void * stream);
+
+/* Rows in int8, as above.
+ *   x      F32|F16 ne [d, H, rows]   a row is H pieces of d values, wherever they lie (wv_b's result is
+ *                                    [d, rows, H] in memory); of a matrix ne [d, rows], H = 1
+ *   dst    I8 ne [H d, rows]
+ *   scale  F32 ne [rows]
+ * d a multiple of 4, H d at most 32768, rows at most 2^24; pieces and rows aligned to 4 elements. */
+int mla_m4_rows_i8(const mla_m4_tensor * x, const mla_m4_tensor * dst, const mla_m4_tensor * scale, void * stream);
+
+/* The product of int8 rows and int8 weights with a scale for each row and each channel:
+ *   dst[t][c] = x_scale[t] * w_scale[c] * sum_k w[c][k] x[t][k]
+ *   w        I8 ne [K, N]       w_scale  F32 ne [N]
+ *   x        I8 ne [K, rows]    x_scale  F32 ne [rows]
+ *   dst      F32|F16 ne [N, rows]
+ * K a multiple of 16, at most 131056: the sum is exact in 32 bits, -128 included; then two f32 products and
+ * for F16 one more rounding.  w and x rows 16-byte aligned, at most 4 MiB apart; dst rows at any distance.
+ * N at most 2^22, rows at most 2^22. */
+int mla_m4_mul_i8(const mla_m4_tensor * w, const mla_m4_tensor * w_scale, const mla_m4_tensor * x,
+                  const mla_m4_tensor * x_scale, const mla_m4_tensor * dst, void * stream);
+
+/* The rope parts of q, NORMAL mode with YaRN as mla_m4_kvrows, the angles taken in 64 bits.
+ *   q    F32|F16 ne [n_dims, H, rows]   strided: the rope parts of a product's rows
+ *   pos  I32 ne [rows]
+ *   dst  F32|F16 ne [n_dims, H, rows]   strided: into Qcur; may be q itself
+ * n_dims a multiple of 32, at most 256 (rope->n_dims); pieces and rows aligned to 4 elements; H at most 1024,
+ * rows at most 2^22. */
+int mla_m4_qrope(const mla_m4_tensor * q, const mla_m4_tensor * pos, const mla_m4_rope_params * rope,
+                 const mla_m4_tensor * dst, void * stream);
+
+/* their supports_op mirrors, as below */
+int mla_m4_supports_norm(const mla_m4_tensor * x, const mla_m4_tensor * post, const mla_m4_tensor * gate,
+                         const mla_m4_tensor * res, const mla_m4_tensor * pre, float eps,
+                         const mla_m4_tensor * res_out, const mla_m4_tensor * dst, const mla_m4_tensor * dst_scale);
+int mla_m4_supports_rows_i8(const mla_m4_tensor * x, const mla_m4_tensor * dst, const mla_m4_tensor * scale);
+int mla_m4_supports_mul_i8(const mla_m4_tensor * w, const mla_m4_tensor * w_scale, const mla_m4_tensor * x,
+                           const mla_m4_tensor * x_scale, const mla_m4_tensor * dst);
+int mla_m4_supports_qrope(const mla_m4_tensor * q, const mla_m4_tensor * pos, const mla_m4_rope_params * rope,
+                          const mla_m4_tensor * dst);
 
 /* -------------------------------------------------------------------------------------------
  * supports_op mirrors (ggml-cuda.cu:5848-5885): 1 if the entry point above accepts these
