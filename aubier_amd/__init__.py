@@ -17,6 +17,7 @@ from .ops import (  # noqa: F401
     ggml_m4_norm,
     ggml_m4_qrope,
     ggml_m4_rows_i8,
+    mul_i8_workspace_bytes,
     supports_mul_i8,
     supports_norm,
     supports_qrope,

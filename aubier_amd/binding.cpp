@@ -25,6 +25,7 @@ struct {
     decltype(&mla_m4_rows_i8) rows_i8;
     decltype(&mla_m4_mul_i8) mul_i8;
     decltype(&mla_m4_qrope) qrope;
+    decltype(&mla_m4_mul_i8_workspace_bytes) mul_workspace_bytes;
 } lib;
 
 // The descriptors of a call's tensors, all on one GPU
@@ -104,14 +105,15 @@ at::Tensor given_or_new(PyObject * o, at::IntArrayRef size, at::ScalarType type,
 
 c10::Device gpu(int i) { return c10::Device(c10::DeviceType::CUDA, (c10::DeviceIndex)i); }
 
-// bind(pages, kvrows, kqkv_paged, workspace_bytes, norm, rows_i8, mul_i8, qrope): addresses
+// bind(pages, kvrows, kqkv_paged, workspace_bytes, norm, rows_i8, mul_i8, qrope, mul_workspace_bytes): addresses
 PyObject * bind(PyObject *, PyObject * const * args, Py_ssize_t n) {
-    if (n != 8) return PyErr_Format(PyExc_TypeError, "eight addresses");
-    void * p[8];
-    for (int i = 0; i < 8; ++i) p[i] = PyLong_AsVoidPtr(args[i]);
+    if (n != 9) return PyErr_Format(PyExc_TypeError, "nine addresses");
+    void * p[9];
+    for (int i = 0; i < 9; ++i) p[i] = PyLong_AsVoidPtr(args[i]);
     if (PyErr_Occurred()) return nullptr;
     lib = {(decltype(lib.pages))p[0], (decltype(lib.kvrows))p[1], (decltype(lib.kqkv_paged))p[2], (decltype(lib.workspace_bytes))p[3],
-           (decltype(lib.norm))p[4], (decltype(lib.rows_i8))p[5], (decltype(lib.mul_i8))p[6], (decltype(lib.qrope))p[7]};
+           (decltype(lib.norm))p[4], (decltype(lib.rows_i8))p[5], (decltype(lib.mul_i8))p[6], (decltype(lib.qrope))p[7],
+           (decltype(lib.mul_workspace_bytes))p[8]};
     Py_RETURN_NONE;
 }
 
@@ -262,13 +264,13 @@ PyObject * rows_i8(PyObject *, PyObject * const * a, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
-// mul_i8(w, w_scale, x, x_scale, out, type, stream) -> out
+// mul_i8(w, w_scale, x, x_scale, out, type, workspace, stream) -> out
 PyObject * mul_i8(PyObject *, PyObject * const * a, Py_ssize_t n) {
     HANDLE_TH_ERRORS
-    if (n != 7) return PyErr_Format(PyExc_TypeError, "seven arguments");
-    if (!tensors(a, 4) || !tensors(a + 4, 1, true)) return nullptr;
+    if (n != 8) return PyErr_Format(PyExc_TypeError, "eight arguments");
+    if (!tensors(a, 4) || !tensors(a + 4, 1, true) || !tensors(a + 6, 1, true)) return nullptr;
     const long type = PyLong_AsLong(a[5]);
-    void * stream = PyLong_AsVoidPtr(a[6]);
+    void * stream = PyLong_AsVoidPtr(a[7]);
     if (PyErr_Occurred()) return nullptr;
     const at::Tensor & w = THPVariable_Unpack(a[0]);
     const at::Tensor & x = THPVariable_Unpack(a[2]);
@@ -276,10 +278,17 @@ PyObject * mul_i8(PyObject *, PyObject * const * a, Py_ssize_t n) {
     const at::Tensor out = given_or_new(a[4], {x.size(0), w.size(0)}, float_or_i8(type), x);
     Call c;
     const mla_m4_tensor *vw = c.add(w), *vs = c.add(a[1]), *vx = c.add(x), *vt = c.add(a[3]), *vd = c.add(out);
-    if (c.status == 0) {
-        const c10::DeviceGuard guard(gpu(c.device));
-        c.status = lib.mul_i8(vw, vs, vx, vt, vd, stream);
+    if (c.status != 0) return PyLong_FromLong(c.status);
+    const c10::DeviceGuard guard(gpu(c.device));
+    at::Tensor work;
+    if (a[6] != Py_None) {
+        work = THPVariable_Unpack(a[6]);
+        if (!work.is_cuda() || (int)work.get_device() != c.device || !work.is_contiguous()) return PyLong_FromLong(MLA_M4_ERR_WORKSPACE);
+    } else {
+        const size_t need = lib.mul_workspace_bytes(vw, vx);
+        if (need > 0) work = at::empty({(int64_t)need}, at::TensorOptions().dtype(at::kByte).device(x.device()));
     }
+    c.status = lib.mul_i8(vw, vs, vx, vt, vd, work.defined() ? work.data_ptr() : nullptr, work.defined() ? (size_t)work.nbytes() : 0, stream);
     return c.status != 0 ? PyLong_FromLong(c.status) : THPVariable_Wrap(out);
     END_HANDLE_TH_ERRORS
 }

@@ -55,7 +55,9 @@ struct MulArgs {
     int64_t dst_nb1;
     int dst_f16;
     int n, k, n_rows;
+    char * work;            // mul_workspace_bytes, or null: k is not cut
 };
+size_t mul_workspace_bytes(int n, int k, int n_rows);
 hipError_t launch_mul_i8(const MulArgs & a, hipStream_t stream);
 
 struct QropeArgs {

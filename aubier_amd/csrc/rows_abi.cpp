@@ -225,11 +225,18 @@ int mla_m4_supports_rows_i8(const mla_m4_tensor * x, const mla_m4_tensor * dst, 
     return check_rows_i8(x, dst, scale, true) == MLA_M4_OK;
 }
 
+size_t mla_m4_mul_i8_workspace_bytes(const mla_m4_tensor * w, const mla_m4_tensor * x) {
+    if (!w || !x || w->ne[0] < 16 || w->ne[0] > rw::MAX_K || w->ne[1] < 1 || w->ne[1] > rw::MAX_MUL || x->ne[1] < 1 || x->ne[1] > rw::MAX_MUL) return 0;
+    return rw::mul_workspace_bytes((int)w->ne[1], (int)w->ne[0], (int)x->ne[1]);
+}
+
 int mla_m4_mul_i8(const mla_m4_tensor * w, const mla_m4_tensor * w_scale, const mla_m4_tensor * x, const mla_m4_tensor * x_scale,
-                  const mla_m4_tensor * dst, void * stream) {
+                  const mla_m4_tensor * dst, void * workspace, size_t workspace_bytes, void * stream) {
     const int rc = check_mul(w, w_scale, x, x_scale, dst);
     if (rc != MLA_M4_OK) return rc;
+    if (workspace && (!aligned16(workspace) || workspace_bytes < mla_m4_mul_i8_workspace_bytes(w, x))) return MLA_M4_ERR_WORKSPACE;
     rw::MulArgs a{};
+    a.work = static_cast<char *>(workspace);
     a.w = static_cast<const char *>(w->data);
     a.w_nb1 = w->ne[1] > 1 ? (int64_t)w->nb[1] : 0;
     a.w_scale = static_cast<const float *>(w_scale->data);

@@ -117,7 +117,8 @@ _EXPORTS = {
     "mla_m4_supports_norm": (ctypes.c_int, [ctypes.c_void_p] * 5 + [ctypes.c_float] + [ctypes.c_void_p] * 3),
     "mla_m4_rows_i8": (ctypes.c_int, [ctypes.c_void_p] * 4),
     "mla_m4_supports_rows_i8": (ctypes.c_int, [ctypes.c_void_p] * 3),
-    "mla_m4_mul_i8": (ctypes.c_int, [ctypes.c_void_p] * 6),
+    "mla_m4_mul_i8": (ctypes.c_int, [ctypes.c_void_p] * 6 + [ctypes.c_size_t, ctypes.c_void_p]),
+    "mla_m4_mul_i8_workspace_bytes": (ctypes.c_size_t, [ctypes.c_void_p] * 2),
     "mla_m4_supports_mul_i8": (ctypes.c_int, [ctypes.c_void_p] * 5),
     "mla_m4_qrope": (ctypes.c_int, [ctypes.c_void_p] * 5),
     "mla_m4_supports_qrope": (ctypes.c_int, [ctypes.c_void_p] * 4),
@@ -317,7 +318,7 @@ def _calls():
         else:
             _binding.bind(*(ctypes.cast(getattr(lib, f), ctypes.c_void_p).value for f in (
                 "mla_m4_pages", "mla_m4_kvrows", "mla_m4_kqkv_paged", "mla_m4_kqkv_paged_workspace_bytes",
-                "mla_m4_norm", "mla_m4_rows_i8", "mla_m4_mul_i8", "mla_m4_qrope")))
+                "mla_m4_norm", "mla_m4_rows_i8", "mla_m4_mul_i8", "mla_m4_qrope", "mla_m4_mul_i8_workspace_bytes")))
             _native = _binding
     return _native
 
@@ -680,22 +681,33 @@ def ggml_m4_rows_i8(x: torch.Tensor, out: Optional[torch.Tensor] = None, scale: 
     return out, scale
 
 
+def mul_i8_workspace_bytes(w: torch.Tensor, x: torch.Tensor) -> int:
+    return int(load_library().mla_m4_mul_i8_workspace_bytes(_ptr(view(w)), _ptr(view(x))))
+
+
 def ggml_m4_mul_i8(w: torch.Tensor, w_scale: torch.Tensor, x: torch.Tensor, x_scale: torch.Tensor,
-                   dtype: torch.dtype = torch.float32, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+                   dtype: torch.dtype = torch.float32, out: Optional[torch.Tensor] = None,
+                   workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
     """The product of int8 rows and weights (include/mla_m4.h mla_m4_mul_i8): out[t, c] = x_scale[t] w_scale[c] sum_k w[c, k]
     x[t, k].  w int8 [N, K], w_scale f32 [N], x int8 [rows, K], x_scale f32 [rows] -> [rows, N] of `dtype` (f32 or f16) or in
-    out."""
+    out.  workspace: optional uint8 device buffer (allocated here when None and the shape has a use for one)."""
     ty = _type_for("ggml_m4_mul_i8", dtype, _FLOAT)
     calls = _native or _calls()
     if calls:
-        return _done("ggml_m4_mul_i8", calls.mul_i8(w, w_scale, x, x_scale, out, ty, _stream_of("ggml_m4_mul_i8", x)))
+        return _done("ggml_m4_mul_i8", calls.mul_i8(w, w_scale, x, x_scale, out, ty, workspace, _stream_of("ggml_m4_mul_i8", x)))
     if w.dim() != 2 or x.dim() != 2:
         raise MlaM4Error("ggml_m4_mul_i8", -3)
     lib = load_library()
     if out is None:
         out = torch.empty((x.shape[0], w.shape[0]), dtype=dtype, device=x.device)
     (vw, s, vx, t, d), gpu = _descriptors("ggml_m4_mul_i8", (w, w_scale, x, x_scale, out))
-    _run_on("ggml_m4_mul_i8", gpu, lib.mla_m4_mul_i8, vw, s, vx, t, d)
+    if workspace is None:
+        need = lib.mla_m4_mul_i8_workspace_bytes(vw, vx)
+        workspace = torch.empty(need, dtype=torch.uint8, device=x.device) if need > 0 else None
+    elif workspace.get_device() != gpu or not workspace.is_contiguous():
+        raise MlaM4Error("ggml_m4_mul_i8", -5)
+    ws_ptr, ws_bytes = (workspace.data_ptr(), workspace.numel() * workspace.element_size()) if workspace is not None else (None, 0)
+    _run_on("ggml_m4_mul_i8", gpu, lib.mla_m4_mul_i8, vw, s, vx, t, d, ws_ptr, ws_bytes)
     return out
 
 

@@ -1,4 +1,5 @@
 """The product of int8 rows and weights (mla_m4_mul_i8) against exact integer sums."""
+import ctypes
 import math
 
 import pytest
@@ -56,6 +57,39 @@ def test_large(dev, rows, n, k):
     a = make(dev, rows, n, k, 2)
     for dtype in (F32, F16):
         check(a, A.ggml_m4_mul_i8(*a, dtype=dtype), dtype)
+
+
+@pytest.mark.parametrize("rows,n,k", [
+    (1, 24577, 1552), (31, 24570, 1536), (32, 576, 7184), (48, 2112, 7168), (64, 2100, 7152), (100, 570, 7168), (64, 7168, 4096), (61, 7150, 4112),
+    (128, 7168, 4096), (125, 7100, 4080), (60, 24576, 1536), (64, 7168, 16384), (300, 7168, 4096), (290, 7101, 4112), (130, 7168, 16384),
+    (200, 24576, 1536), (1000, 7168, 4096), (1030, 4100, 4112), (3000, 4096, 528), (4001, 2112, 1040)])
+def test_forms(dev, rows, n, k):
+    """Shapes that the forms of the product share out among them, with and without a workspace, into rows at odd places."""
+    a = make(dev, rows, n, k, 3)
+    got = A.ggml_m4_mul_i8(*a)
+    check(a, got)
+    need = A.mul_i8_workspace_bytes(a[0], a[2])
+    assert need <= 1 << 24
+    work = torch.full((need + 16,), 99, dtype=torch.uint8, device=dev)
+    buf = torch.full((rows, n + 3), 7.0, device=dev)
+    assert torch.equal(A.ggml_m4_mul_i8(*a, out=buf[:, 1:n + 1], workspace=work[:max(need, 16)]), got)
+    assert (buf[:, 0] == 7).all() and (buf[:, n + 1:] == 7).all() and (work[max(need, 16):] == 99).all()
+    check(a, A.ggml_m4_mul_i8(*a, dtype=F16))
+
+
+def test_without_a_workspace(dev):
+    """The C entry point given none: the same bits; one that is too small is refused."""
+    a = make(dev, 64, 576, 7168)
+    want = A.ggml_m4_mul_i8(*a)
+    need = A.mul_i8_workspace_bytes(a[0], a[2])
+    assert need > 0
+    with pytest.raises(A.MlaM4Error) as e:
+        A.ggml_m4_mul_i8(*a, workspace=torch.empty(need - 1, dtype=torch.uint8, device=dev))
+    assert e.value.status == -5
+    out = torch.empty_like(want)
+    v = [A.view(t) for t in (*a, out)]
+    assert A.load_library().mla_m4_mul_i8(*(ctypes.byref(t) for t in v), None, 0, torch.cuda.current_stream().cuda_stream) == 0
+    assert torch.equal(out, want)
 
 
 @pytest.mark.parametrize("rows", [1, 40, 300])

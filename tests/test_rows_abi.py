@@ -74,7 +74,8 @@ def test_rows_i8(status, args):
 def mul(**kw):
     d = dict(w=z(5, 64, dtype=I8), ws=z(5), x=z(3, 64, dtype=I8), xs=z(3), out=z(3, 5))
     d.update(kw)
-    return refused("mla_m4_mul_i8", list(d.values()))
+    v = [A.view(t) if isinstance(t, torch.Tensor) else t for t in d.values()]
+    return A.load_library().mla_m4_mul_i8(*(ctypes.byref(t) if t is not None else None for t in v), None, 0, None)
 
 
 @pytest.mark.parametrize("status,bad", [
@@ -147,7 +148,7 @@ def test_supports():
     for t in v:
         t.data = None
     assert A.load_library().mla_m4_supports_mul_i8(*(ctypes.byref(t) for t in v))
-    assert A.load_library().mla_m4_mul_i8(*(ctypes.byref(t) for t in v), None) == -1
+    assert A.load_library().mla_m4_mul_i8(*(ctypes.byref(t) for t in v), None, 0, None) == -1
 
 
 def test_python_refuses():
