@@ -2,13 +2,15 @@
 // rope parts of q (qrope_kernel).
 //
 // norm_kernel: a workgroup per row, the row in registers, so x and the residual are read once and r and h written once.
-// Everything is taken in 64 bits and rounded where it is stored.  That makes the int8 rows what their definition says
-// (a value next to a border between two integers falls on its side) and costs little, as the card's rate for 64-bit
-// vector instructions is that of 32-bit ones and the kernel waits for memory.
+// Everything is taken in 64 bits and rounded where it is stored, or as if it were (int8).  That makes the int8 rows what their
+// definition says (a value next to a border between two integers falls on its side) and costs little, as the card's rate for
+// 64-bit vector instructions is that of 32-bit ones and the kernel waits for memory.
 //
 // qrope_kernel: a wavefront per token; a lane turns the same pairs of several heads, so an angle is taken once for them.
 #include "mla_common.h"
 #include "rows.h"
+
+#include <type_traits>
 
 namespace mla {
 namespace rows {
@@ -17,77 +19,73 @@ namespace {
 
 // v of another lane, 64 bits wide, by DPP
 template <int CTRL>
-__device__ __forceinline__ uint64_t dpp64(uint64_t v) {
-    const uint32_t lo = (uint32_t)__builtin_amdgcn_mov_dpp((int)(uint32_t)v, CTRL, 0xf, 0xf, false);
-    const uint32_t hi = (uint32_t)__builtin_amdgcn_mov_dpp((int)(uint32_t)(v >> 32), CTRL, 0xf, 0xf, false);
-    return (uint64_t)hi << 32 | lo;
+__device__ __forceinline__ double dpp64(double v) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_mov_dpp((int)(uint32_t)u, CTRL, 0xf, 0xf, false);
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_mov_dpp((int)(uint32_t)(u >> 32), CTRL, 0xf, 0xf, false);
+    return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
 }
 struct Sum {
-    __device__ __forceinline__ uint64_t operator()(uint64_t a, uint64_t b) const {
-        return __builtin_bit_cast(uint64_t, __builtin_bit_cast(double, a) + __builtin_bit_cast(double, b));
-    }
+    __device__ __forceinline__ double operator()(double a, double b) const { return a + b; }
 };
 struct Max {
-    __device__ __forceinline__ uint64_t operator()(uint64_t a, uint64_t b) const { return a > b ? a : b; }
+    __device__ __forceinline__ double operator()(double a, double b) const { return fmax(a, b); }
 };
-// v of all lanes of the wavefront combined, at every lane
+// v of a row of 16 lanes combined, at each of them
 template <typename Op>
-__device__ __forceinline__ uint64_t wave_all(uint64_t v, Op op) {
+__device__ __forceinline__ double row_all(double v, Op op) {
     v = op(v, dpp64<0xB1>(v));                  // lane ^ 1, ^ 2
     v = op(v, dpp64<0x4E>(v));
     v = op(v, dpp64<0x1B>(dpp64<0x141>(v)));    // ^ 4
-    v = op(v, dpp64<0x128>(v));                 // ^ 8
-    auto pair = [&](bool rows16) {
-        const uint32_t lo = (uint32_t)v, hi = (uint32_t)(v >> 32);
-        if (rows16) {
-            const auto a = __builtin_amdgcn_permlane16_swap(lo, lo, false, false);
-            const auto b = __builtin_amdgcn_permlane16_swap(hi, hi, false, false);
-            return op((uint64_t)b[0] << 32 | a[0], (uint64_t)b[1] << 32 | a[1]);
-        }
-        const auto a = __builtin_amdgcn_permlane32_swap(lo, lo, false, false);
-        const auto b = __builtin_amdgcn_permlane32_swap(hi, hi, false, false);
-        return op((uint64_t)b[0] << 32 | a[0], (uint64_t)b[1] << 32 | a[1]);
+    return op(v, dpp64<0x128>(v));              // ^ 8
+}
+// v of all lanes of the wavefront combined, at every lane
+template <typename Op>
+__device__ __forceinline__ double wave_all(double v, Op op) {
+    v = row_all(v, op);
+    auto pair = [&](auto swap) {
+        const uint64_t u = __builtin_bit_cast(uint64_t, v);
+        const auto a = swap((uint32_t)u), b = swap((uint32_t)(u >> 32));
+        return op(__builtin_bit_cast(double, (uint64_t)b[0] << 32 | a[0]), __builtin_bit_cast(double, (uint64_t)b[1] << 32 | a[1]));
     };
-    v = pair(true);
-    return pair(false);
+    v = pair([](uint32_t x) { return __builtin_amdgcn_permlane16_swap(x, x, false, false); });
+    return pair([](uint32_t x) { return __builtin_amdgcn_permlane32_swap(x, x, false, false); });
 }
 
-// the workgroup's sum and largest of a value each per thread; red: NT / 64 pairs of LDS that no other reduction uses
-template <int NT>
-__device__ __forceinline__ void block_all(double & sum, uint64_t & top, uint64_t * red) {
+// the workgroup's sum and largest of a value each per thread (either may be left out); red: NT / 64 pairs of LDS that no other
+// reduction uses.  A lane takes one wave's, and a row of 16 lanes puts them together.
+template <int NT, bool SUM, bool MAX>
+__device__ __forceinline__ void block_all(double & sum, double & top, double (&red)[NT / 64][2]) {
     constexpr int NW = NT / 64;
-    uint64_t s = wave_all(__builtin_bit_cast(uint64_t, sum), Sum{}), t = wave_all(top, Max{});
-    if constexpr (NW > 1) {
-        const int w = threadIdx.x >> 6;
-        if ((threadIdx.x & 63) == 0) {
-            red[2 * w] = s;
-            red[2 * w + 1] = t;
-        }
-        __syncthreads();
-        s = red[0];
-        t = red[1];
-#pragma unroll
-        for (int i = 1; i < NW; ++i) {
-            s = Sum{}(s, red[2 * i]);
-            t = Max{}(t, red[2 * i + 1]);
-        }
+    if constexpr (SUM) sum = wave_all(sum, Sum{});
+    if constexpr (MAX) top = wave_all(top, Max{});
+    if constexpr (NW == 1) return;
+    if ((threadIdx.x & 63) == 0) {
+        if constexpr (SUM) red[threadIdx.x >> 6][0] = sum;
+        if constexpr (MAX) red[threadIdx.x >> 6][1] = top;
     }
-    sum = __builtin_bit_cast(double, s);
-    top = t;
+    __syncthreads();
+    const int l = threadIdx.x & 15;
+    if constexpr (SUM) sum = row_all(l < NW ? red[l % NW][0] : 0.0, Sum{});
+    if constexpr (MAX) top = row_all(l < NW ? red[l % NW][1] : 0.0, Max{});
 }
 
-__device__ __forceinline__ uint64_t magnitude(double v) { return __builtin_bit_cast(uint64_t, v) & 0x7fffffffffffffffull; }
-constexpr uint64_t INF64 = 0x7ff0000000000000ull;
+// 1 / sqrt(x): the hardware's estimate and two steps of Newton's method (to 2^-52 or so)
+__device__ __forceinline__ double inverse_root(double x) {
+    const double r = __builtin_amdgcn_rsq(x);
+    double y = r * fma(-0.5 * x * r, r, 1.5);
+    y = y * fma(-0.5 * x * y, y, 1.5);
+    return x > 0.0 && x < __builtin_inf() ? y : r;
+}
 
+// four neighbouring values as they lie in memory: turned into f32 where they are used, so that loads do not wait for one another
 template <bool F16>
-__device__ __forceinline__ f32x4 load4(const char * row, int c) {
-    if constexpr (F16) {
-        const half4 h = *reinterpret_cast<const half4 *>(row + 2 * c);
-        return f32x4{(float)h[0], (float)h[1], (float)h[2], (float)h[3]};
-    } else {
-        return *reinterpret_cast<const f32x4 *>(row + 4 * c);
-    }
-}
+struct Four {
+    typedef _Float16 h4 __attribute__((ext_vector_type(4)));
+    typename std::conditional<F16, h4, f32x4>::type v;
+    __device__ __forceinline__ void load(const char * row, int c) { v = __builtin_nontemporal_load(reinterpret_cast<const decltype(v) *>(row + (F16 ? 2 : 4) * (int64_t)c)); }
+    __device__ __forceinline__ f32x4 get() const { return f32x4{(float)v[0], (float)v[1], (float)v[2], (float)v[3]}; }
+};
 __device__ __forceinline__ void store4(char * row, int type, int c, f32x4 v) {
     if (type == OUT_F32) {
         *reinterpret_cast<f32x4 *>(row + 4 * c) = v;
@@ -99,108 +97,208 @@ __device__ __forceinline__ void store4(char * row, int type, int c, f32x4 v) {
     }
 }
 
-// The integer of v = |value| in a row whose largest magnitude is top: 127 v / top, half away from zero.  `per` is
-// 127 / top in 64 bits, so the quotient is off by 2^-51 of itself at most; within 2^-40 of a border it is taken by division.
-__device__ __forceinline__ int steps_of(double v, double top, double per) {
-    double u = v * per + 0.5, k = floor(u);
-    const double past = u - k;
-    if (past < 0x1p-40 || past > 1.0 - 0x1p-40) k = floor(v * 127.0 / top + 0.5);
-    return (int)k;
+__device__ __forceinline__ uint32_t pack4(int q0, int q1, int q2, int q3) {
+    const uint32_t lo = __builtin_amdgcn_perm((uint32_t)q1, (uint32_t)q0, 0x0c0c0400u), hi = __builtin_amdgcn_perm((uint32_t)q3, (uint32_t)q2, 0x0c0c0400u);
+    return hi << 16 | lo;
+}
+// the values, as far as the compiler knows others: so that it does not keep their 64-bit forms from one pass for the next (a row
+// would not fit in the registers with them: spills, or half as many rows on a CU at a time)
+template <int N>
+__device__ __forceinline__ void again(f32x4 (&v)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) asm volatile("" : "+v"(v[i]));
 }
 
-// NT threads, C groups of four values a thread.  RES: 0 none, 1 f32, 2 f16.
+constexpr int PIECES = 3;
+
+// NT threads, C groups of four values a thread.  RES: no residual, one of f32 (1) or f16 (2), or PIECES: int8 rows of x as it is, in
+// pieces, without any norm.
+//
+// int8.  The row's largest |r pre| is found in 64 bits, where such products are exact.  127 |r pre| / top is then taken in f32, off
+// by less than 4 * 2^-24 * 127 < 2^-15 (from a quotient in 64 bits where the row is near the ends of f32's range), and compared with
+// the border in 64 bits where it lies within 2^-14 of one between two integers (a value in 8,000).
 template <int NT, int C, bool XH, int RES>
-__global__ __launch_bounds__(NT) void norm_kernel(NormArgs a) {
+__global__ __launch_bounds__(NT, 4) void norm_kernel(NormArgs a) {
     // by turns, so that a row's reductions need not wait for the row before to have read its own
-    __shared__ uint64_t reds[2][2][2 * (NT / 64)];
+    __shared__ double reds[2][2][NT / 64][2];
     const int tid = threadIdx.x;
+    constexpr bool PLAIN = RES == PIECES;
+    const bool i8 = PLAIN || a.dst_type == OUT_I8;
     int turn = 0;
-    for (int row = blockIdx.x; row < a.n_rows; row += gridDim.x, turn ^= 1) {
-        auto & red = reds[turn];
+    // A row's values are on their way while the row before is worked on.  (Places past the row's end read its first values;
+    // what is made of them is not stored, and adds nothing.)
+    Four<XH> raw[C];
+    Four<RES == 2> rs[RES == 1 || RES == 2 ? C : 1];
+    auto load_x = [&](int row) {
         const char * xr = a.x + (int64_t)row * a.x_nb1;
-        f32x4 v[C], rs[RES ? C : 1];
+#pragma unroll
+        for (int i = 0; i < C; ++i) {
+            const int c = 4 * (NT * i + tid), at = c < a.n ? c : 0;
+            if constexpr (RES == PIECES) {
+                const int piece = a.d_shift >= 0 ? at >> a.d_shift : at / a.d;      // (one piece: a shift that leaves 0)
+                raw[i].load(xr + (int64_t)piece * a.x_nbh, at - piece * a.d);
+            } else {
+                raw[i].load(xr, at);
+            }
+        }
+    };
+    auto load_res = [&](int row) {
+        if constexpr (RES == 1 || RES == 2) {
+#pragma unroll
+            for (int i = 0; i < C; ++i) {
+                const int c = 4 * (NT * i + tid);
+                rs[i].load(a.res + (int64_t)row * a.res_nb1, c < a.n ? c : 0);
+            }
+        }
+    };
+    // weights of the thread's channels, or ones
+    auto weights = [&](f32x4 (&w)[C], const void * from) {
 #pragma unroll
         for (int i = 0; i < C; ++i) {
             const int c = 4 * (NT * i + tid);
-            v[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-            if (c < a.n) {
-                const int piece = c / a.d;
-                v[i] = load4<XH>(xr + (int64_t)piece * a.x_nbh, c - piece * a.d);
-                if constexpr (RES != 0) rs[i] = load4<RES == 2>(a.res + (int64_t)row * a.res_nb1, c);
-            }
+            w[i] = f32x4{1.f, 1.f, 1.f, 1.f};
+            if (!PLAIN && from != nullptr) w[i] = *reinterpret_cast<const f32x4 *>(static_cast<const char *>(from) + 4 * (int64_t)(c < a.n ? c : 0));
         }
+    };
+    load_x(blockIdx.x);
+    load_res(blockIdx.x);
+    for (int row = blockIdx.x; row < a.n_rows; row += gridDim.x, turn ^= 1) {
+        const int next = min(row + (int)gridDim.x, a.n_rows - 1);
+        f32x4 v[C], pw[C], gw[C], hw[C];
+#pragma unroll
+        for (int i = 0; i < C; ++i) v[i] = 4 * (NT * i + tid) < a.n ? raw[i].get() : f32x4{0.f, 0.f, 0.f, 0.f};
+        const char * gate = a.gate != nullptr ? a.gate + (int64_t)row * a.gate_nb1 : nullptr;
+        weights(pw, a.post);
+        weights(gw, a.gate_wide ? gate : nullptr);
+        if constexpr (C <= 2) weights(hw, a.pre);
+        load_x(next);
         double factor = 1.0;
-        if (a.post != nullptr) {
-            double s = 0.0;
-            uint64_t none = 0;
+        if (gate != nullptr && !a.gate_wide) factor = (double)*reinterpret_cast<const float *>(gate);
+        if constexpr (RES == 1 || RES == 2) factor *= (double)a.scale;
+        double sum = 0.0, top = 0.0;
+        if (!PLAIN && a.post != nullptr) {
 #pragma unroll
             for (int i = 0; i < C; ++i)
 #pragma unroll
-                for (int k = 0; k < 4; ++k) s += (double)v[i][k] * (double)v[i][k];
-            block_all<NT>(s, none, red[0]);
-            factor = 1.0 / sqrt(s / (double)a.n + (double)a.eps);
+                for (int k = 0; k < 4; ++k) sum = fma((double)v[i][k], (double)v[i][k], sum);
+            again(v);
+            block_all<NT, true, false>(sum, top, reds[turn][0]);
+            factor *= inverse_root(fma(sum, a.per_n, (double)a.eps));
         }
-        const char * gate = a.gate != nullptr ? a.gate + (int64_t)row * a.gate_nb1 : nullptr;
-        if (gate != nullptr && !a.gate_wide) factor *= (double)*reinterpret_cast<const float *>(gate);
-        if constexpr (RES != 0) factor *= (double)a.scale;
         // r, as it is stored
-        double sum = 0.0;
-        uint64_t top = 0;
+        if (!PLAIN && (RES == 1 || RES == 2 || a.post != nullptr || gate != nullptr)) {
 #pragma unroll
-        for (int i = 0; i < C; ++i) {
-            const int c = 4 * (NT * i + tid);
-            if (c >= a.n) continue;
-            f32x4 pw = {1.f, 1.f, 1.f, 1.f}, gw = pw, hw = pw;
-            if (a.post != nullptr) pw = *reinterpret_cast<const f32x4 *>(a.post + c);
-            if (gate != nullptr && a.gate_wide) gw = *reinterpret_cast<const f32x4 *>(gate + 4 * (int64_t)c);
-            if (a.pre != nullptr) hw = *reinterpret_cast<const f32x4 *>(a.pre + c);
+            for (int i = 0; i < C; ++i) {
+                const int c = 4 * (NT * i + tid);
+                const f32x4 before = RES == 1 || RES == 2 ? rs[i].get() : f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                double y = (double)v[i][k] * factor * (double)pw[k] * (double)gw[k];
-                if constexpr (RES != 0) y += (double)rs[i][k];
-                v[i][k] = (float)y;
-                if (a.res_out_type == OUT_F16) v[i][k] = (float)to_half(v[i][k]);
-                sum += (double)v[i][k] * (double)v[i][k];
-                const uint64_t m = magnitude((double)v[i][k] * (double)hw[k]);
-                top = m > top ? m : top;
-            }
-            if (a.res_out_type != OUT_NONE) store4(a.res_out + (int64_t)row * a.res_out_nb1, a.res_out_type, c, v[i]);
-        }
-        if (a.dst_type == OUT_NONE) continue;
-        double inv = 1.0;
-        if (a.rms || a.dst_type == OUT_I8) {
-            block_all<NT>(sum, top, red[1]);
-            if (a.rms) inv = 1.0 / sqrt(sum / (double)a.n + (double)a.eps);
-        }
-        const double most = __builtin_bit_cast(double, top);
-        const bool finite = top < INF64;
-        const double per = finite && top != 0 ? 127.0 / most : 0.0;
-        char * out = a.dst + (int64_t)row * a.dst_nb1;
-#pragma unroll
-        for (int i = 0; i < C; ++i) {
-            const int c = 4 * (NT * i + tid);
-            if (c >= a.n) continue;
-            f32x4 hw = {1.f, 1.f, 1.f, 1.f};
-            if (a.pre != nullptr) hw = *reinterpret_cast<const f32x4 *>(a.pre + c);
-            if (a.dst_type == OUT_I8) {
-                uint32_t q = 0;
-                if (per != 0.0) {
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        const double h = (double)v[i][k] * (double)hw[k];
-                        const int steps = steps_of(fabs(h), most, per);
-                        q |= (uint32_t)((h < 0.0 ? -steps : steps) & 0xff) << (8 * k);
-                    }
+                for (int k = 0; k < 4; ++k) {
+                    double y = (double)v[i][k] * factor;
+                    const double w = (double)pw[i][k] * (double)gw[i][k];
+                    if constexpr (RES == 1 || RES == 2) y = fma(y, w, (double)before[k]);
+                    else y *= w;
+                    v[i][k] = c < a.n ? (float)y : 0.0f;
                 }
-                *reinterpret_cast<uint32_t *>(out + c) = q;
-            } else {
+            }
+        }
+        load_res(next);
+        if (!PLAIN && a.res_out_type != OUT_NONE) {
+#pragma unroll
+            for (int i = 0; i < C; ++i) {
+                const int c = 4 * (NT * i + tid);
+                if (c >= a.n) continue;
+                if (a.res_out_type == OUT_F16) {
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) v[i][k] = (float)to_half(v[i][k]);
+                }
+                store4(a.res_out + (int64_t)row * a.res_out_nb1, a.res_out_type, c, v[i]);
+            }
+        }
+        if (!PLAIN && a.dst_type == OUT_NONE) continue;
+        char * out = a.dst + (int64_t)row * a.dst_nb1;
+        if constexpr (C > 2) weights(hw, a.pre);
+        sum = 0.0;
+        if (!i8) {
+            double inv = 1.0;
+            if (a.rms) {
+#pragma unroll
+                for (int i = 0; i < C; ++i)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) sum = fma((double)v[i][k], (double)v[i][k], sum);
+                again(v);
+                block_all<NT, true, false>(sum, top, reds[turn][1]);
+                inv = inverse_root(fma(sum, a.per_n, (double)a.eps));
+            }
+#pragma unroll
+            for (int i = 0; i < C; ++i) {
+                const int c = 4 * (NT * i + tid);
+                if (c >= a.n) continue;
                 f32x4 h;
 #pragma unroll
-                for (int k = 0; k < 4; ++k) h[k] = (float)((double)v[i][k] * inv * (double)hw[k]);
+                for (int k = 0; k < 4; ++k) h[k] = (float)((double)v[i][k] * inv * (double)hw[i][k]);
                 store4(out, a.dst_type, c, h);
             }
+            continue;
         }
-        if (a.dst_type == OUT_I8 && tid == 0) a.dst_scale[row] = finite ? (float)(most * inv / 127.0) : __builtin_nanf("");
+        if constexpr (PLAIN) {
+            // of the bits, which order magnitudes and put infinities and NaN above them all
+            uint32_t u = 0;
+#pragma unroll
+            for (int i = 0; i < C; ++i)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) u = max(u, __float_as_uint(v[i][k]) & 0x7fffffffu);
+            top = u < 0x7f800000u ? (double)__uint_as_float(u) : __builtin_inf();
+            block_all<NT, false, true>(sum, top, reds[turn][1]);
+        } else {
+            float finite = 0.0f;                        // NaN where a value is none or an infinity
+#pragma unroll
+            for (int i = 0; i < C; ++i)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const double r = (double)v[i][k];
+                    sum = fma(r, r, sum);
+                    top = fmax(top, fabs(r * (double)hw[i][k]));
+                    finite = fmaf(v[i][k], 0.0f, fmaf(hw[i][k], 0.0f, finite));
+                }
+            if (finite != 0.0f) top = __builtin_inf();
+            again(v);
+            again(hw);
+            block_all<NT, true, true>(sum, top, reds[turn][1]);
+        }
+        const bool there = top > 0.0 && top < __builtin_inf();
+        const double per64 = there ? 127.0 / top : 0.0;
+        const bool mid = top >= 0x1p-90 && top < 0x1p120;       // products and quotients are normal f32
+        const float per = mid ? (float)per64 : 0.0f;
+#pragma unroll
+        for (int i = 0; i < C; ++i) {
+            const int c = 4 * (NT * i + tid);
+            if (c >= a.n) continue;
+            int q[4];
+            float t[4], off = 0.0f;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                if (mid) t[k] = v[i][k] * hw[i][k] * per;
+                else t[k] = there ? (float)((double)v[i][k] * (double)hw[i][k] * per64) : 0.0f;
+                const float n = rintf(t[k]);
+                q[k] = (int)n;
+                off = fmaxf(off, fabsf(t[k] - n));
+            }
+            if (off > 0.5f - 0x1p-14f) {
+                // 127 |r pre| against (the integer below + 1 / 2) top
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const float below = floorf(fabsf(t[k]));
+                    const double h = fabs((double)v[i][k] * (double)hw[i][k]);
+                    const int n = (int)below + (h * 127.0 >= ((double)below + 0.5) * top ? 1 : 0);
+                    q[k] = t[k] < 0.0f ? -n : n;
+                }
+            }
+            *reinterpret_cast<uint32_t *>(out + c) = pack4(q[0], q[1], q[2], q[3]);
+        }
+        if (tid == 0) {
+            const double inv = !PLAIN && a.rms ? inverse_root(fma(sum, a.per_n, (double)a.eps)) : 1.0;
+            a.dst_scale[row] = there ? (float)(top * inv / 127.0) : top == 0.0 ? 0.0f : __builtin_nanf("");
+        }
     }
 }
 
@@ -224,7 +322,9 @@ __global__ __launch_bounds__(256) void qrope_kernel(QropeArgs a) {
         co[k] *= a.mscale;
     }
     for (int h = h0; h < a.n_head; h += per) {
-        f32x4 v = load4<QH>(a.q + (int64_t)row * a.q_nb2 + (int64_t)h * a.q_nb1, 4 * g);
+        Four<QH> q;
+        q.load(a.q + (int64_t)row * a.q_nb2 + (int64_t)h * a.q_nb1, 4 * g);
+        f32x4 v = q.get();
 #pragma unroll
         for (int k = 0; k < 4; k += 2) {
             const float x0 = v[k], x1 = v[k + 1];
@@ -235,26 +335,44 @@ __global__ __launch_bounds__(256) void qrope_kernel(QropeArgs a) {
     }
 }
 
-constexpr int MAX_GRID = 1 << 20;       // the grid's threads stay below 2^32
+constexpr int FEW = 256;                // rows, one a CU: as many threads as a row has use for
 
 template <int NT, int C>
 hipError_t norm(const NormArgs & a, hipStream_t stream) {
-    const dim3 grid(a.n_rows < MAX_GRID ? a.n_rows : MAX_GRID), block(NT);
-    auto go = [&](auto kernel) {
-        hipLaunchKernelGGL(kernel, grid, block, 0, stream, a);
+    auto go = [&](auto kernel, int waves) {
+        const int at_once = 256 * (64 * waves / NT);    // workgroups that the card holds
+        hipLaunchKernelGGL(kernel, dim3(a.n_rows < at_once ? a.n_rows : at_once), dim3(NT), 0, stream, a);
         return hipGetLastError();
     };
-    const int res = a.res == nullptr ? 0 : a.res_f16 ? 2 : 1;
-    if (a.x_f16) return res == 0 ? go(norm_kernel<NT, C, true, 0>) : res == 1 ? go(norm_kernel<NT, C, true, 1>) : go(norm_kernel<NT, C, true, 2>);
-    return res == 0 ? go(norm_kernel<NT, C, false, 0>) : res == 1 ? go(norm_kernel<NT, C, false, 1>) : go(norm_kernel<NT, C, false, 2>);
+    const int res = a.d != 0 ? PIECES : a.res == nullptr ? 0 : a.res_f16 ? 2 : 1;
+    switch (res + (a.x_f16 ? 4 : 0)) {
+        case 0: return go(norm_kernel<NT, C, false, 0>, 16);
+        case 1: return go(norm_kernel<NT, C, false, 1>, 16);
+        case 2: return go(norm_kernel<NT, C, false, 2>, 16);
+        case 3: return go(norm_kernel<NT, C, false, PIECES>, C <= 3 ? 32 : 16);
+        case 4: return go(norm_kernel<NT, C, true, 0>, 16);
+        case 5: return go(norm_kernel<NT, C, true, 1>, 16);
+        case 6: return go(norm_kernel<NT, C, true, 2>, 16);
+        default: return go(norm_kernel<NT, C, true, PIECES>, C <= 3 ? 32 : 16);
+    }
 }
 
 }  // namespace
 
 hipError_t launch_norm(const NormArgs & a, hipStream_t stream) {
-    if (a.n <= 1024) return norm<256, 1>(a, stream);
-    if (a.n <= 4096) return norm<256, 4>(a, stream);
-    if (a.n <= 8192) return norm<256, 8>(a, stream);
+    // Many rows: as few threads a row as keep its values in registers, so that a CU has several rows at different places of their
+    // way (8,000 rows of 1,536: 25 us by 256 threads, 35 by 512).  Few rows: more threads (one of 4,096: 4.1 us by 512, 5.8 by 256).
+    const bool few = a.n_rows <= FEW;
+    const int fours = (a.n + 255) / 256;                // groups of a thread, of a wavefront
+    if (!few && fours == 1) return norm<64, 1>(a, stream);
+    if (!few && fours == 2) return norm<64, 2>(a, stream);
+    if (fours <= 4) return norm<256, 1>(a, stream);
+    if (fours <= 8) return few ? norm<512, 1>(a, stream) : norm<256, 2>(a, stream);
+    if (fours <= 16) return norm<512, 2>(a, stream);
+    if (fours <= 24) return norm<512, 3>(a, stream);
+    if (fours <= 32) return norm<1024, 2>(a, stream);
+    if (fours <= 48) return norm<1024, 3>(a, stream);
+    if (fours <= 64) return norm<1024, 4>(a, stream);
     if (a.n <= MAX_N) return norm<1024, 8>(a, stream);
     return hipErrorInvalidValue;
 }

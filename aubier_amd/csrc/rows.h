@@ -21,7 +21,7 @@ enum { OUT_NONE = 0, OUT_F32 = 1, OUT_F16 = 2, OUT_I8 = 3 };
 struct NormArgs {
     const char * x;         // row r's value c: x + r x_nb1 + (c / d) x_nbh + (c % d) elements
     int64_t x_nb1, x_nbh;
-    int d;                  // values in a piece; n where a row is one piece
+    int d, d_shift;         // values in a piece, and its binary logarithm or -1; d 0: rows of norm, in one piece
     int x_f16;
     const float * post;     // [n] or null
     const char * gate;      // one value for every channel (gate_wide), or one; rows gate_nb1 bytes apart (0: the same); or null
@@ -33,6 +33,7 @@ struct NormArgs {
     const float * pre;      // [n] or null
     int rms;                // the second norm (0: h = r, as rows_i8)
     float scale, eps;
+    double per_n;           // 1 / n
     char * res_out;
     int64_t res_out_nb1;
     int res_out_type;       // OUT_*

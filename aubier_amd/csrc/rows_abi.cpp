@@ -163,7 +163,6 @@ int mla_m4_norm(const mla_m4_tensor * x, const mla_m4_tensor * post, const mla_m
     rw::NormArgs a{};
     a.x = static_cast<const char *>(x->data);
     a.x_nb1 = (int64_t)x->nb[1];
-    a.d = (int)x->ne[0];
     a.x_f16 = x->type == MLA_M4_TYPE_F16;
     a.post = post ? static_cast<const float *>(post->data) : nullptr;
     if (gate) {
@@ -192,6 +191,7 @@ int mla_m4_norm(const mla_m4_tensor * x, const mla_m4_tensor * post, const mla_m
     a.dst_type = out_type(dst);
     a.dst_scale = dst_scale ? static_cast<float *>(dst_scale->data) : nullptr;
     a.n = (int)x->ne[0];
+    a.per_n = 1.0 / (double)a.n;
     a.n_rows = (int)x->ne[1];
     return launched(rw::launch_norm(a, static_cast<hipStream_t>(stream)));
 }
@@ -209,8 +209,12 @@ int mla_m4_rows_i8(const mla_m4_tensor * x, const mla_m4_tensor * dst, const mla
     rw::NormArgs a{};
     a.x = static_cast<const char *>(p.data);
     a.x_nb1 = (int64_t)p.nb[2];
-    a.x_nbh = (int64_t)p.nb[1];
+    a.x_nbh = p.ne[1] > 1 ? (int64_t)p.nb[1] : 0;
     a.d = (int)p.ne[0];
+    a.d_shift = -1;
+    for (int i = 2; i < 16; ++i)
+        if (p.ne[0] == (int64_t)1 << i) a.d_shift = i;
+    if (p.ne[1] == 1) a.d_shift = 31;                   // one piece
     a.x_f16 = p.type == MLA_M4_TYPE_F16;
     a.dst = static_cast<char *>(dst->data);
     a.dst_nb1 = (int64_t)dst->nb[1];
