@@ -79,6 +79,35 @@ def test_norm_rows(dev, pre, rows):
         check_norm(i, dtype=dtype)
 
 
+@pytest.mark.parametrize("n,rows", [(4, 20000), (256, 9000), (260, 9000), (512, 6001), (516, 5000), (1024, 5000), (1536, 4500), (2048, 4400), (2052, 2100), (4096, 2100),
+                                    (5120, 1100), (6144, 1100), (7168, 1030), (8192, 600), (12288, 600), (12292, 600), (16384, 530), (32768, 530)])
+@pytest.mark.parametrize("x,res", [(F32, F32), (F16, F16), (F32, None)])
+def test_norm_many_rows(dev, n, rows, x, res):
+    """More rows than workgroups at once, at each width's split; the residual's place taken by r."""
+    i = inputs(dev, rows, n, x, res, "row")
+    check_norm(i, dtype=I8)
+    if res is not None:
+        want, mine = A.ggml_m4_norm(i["x"], i["pre"], EPS, post=i["post"], gate=i["gate"], res=i["res"], dtype=F16), i["res"].clone()
+        got = A.ggml_m4_norm(i["x"], i["pre"], EPS, post=i["post"], gate=i["gate"], res=mine, res_out=mine, dtype=F16)
+        assert got[0] is mine and all(torch.equal(a, b) for a, b in zip(got[:2], want[:2]))
+
+
+@pytest.mark.parametrize("n", [128, 1536, 4096, 7168, 16384])
+@pytest.mark.parametrize("rows", [64, 3000])
+def test_norm_bad_rows_beside(dev, n, rows):
+    """Rows behind a batch hold anything: NaN and infinities in every third row change no other row."""
+    i = inputs(dev, rows, n)
+    want = A.ggml_m4_norm(i["x"], i["pre"], EPS, post=i["post"], gate=i["gate"], res=i["res"], dtype=I8), A.ggml_m4_rows_i8(i["x"])
+    for k, v in enumerate((math.nan, math.inf, -math.inf)):
+        i["x"][k::9] = v
+    good = torch.ones(rows, dtype=torch.bool, device=dev)
+    for k in range(3):
+        good[k::9] = False
+    got = A.ggml_m4_norm(i["x"], i["pre"], EPS, post=i["post"], gate=i["gate"], res=i["res"], dtype=I8), A.ggml_m4_rows_i8(i["x"])
+    for g, w in zip(got, want):
+        assert all(torch.equal(a[good], b[good]) for a, b in zip(g, w)) and torch.isnan(g[-1][~good]).all() and (g[-2][~good] == 0).all()
+
+
 def test_norm_into_given(dev):
     """Outputs of other types than the default, into views whose padding stays, and r in the place of the residual."""
     i = inputs(dev, 33, 260)
@@ -146,7 +175,7 @@ def check_i8(x, got):
     near(s, ws, 2.0 ** -24, 2.0 ** -150)
 
 
-@pytest.mark.parametrize("shape", [(1, 4), (5, 256), (3, 1028), (64, 7168), (2, 32768), (300, 4096), (2, 1, 128), (7, 3, 4), (48, 32, 128), (9, 40, 128), (130, 128, 256)])
+@pytest.mark.parametrize("shape", [(1, 4), (5, 256), (3, 1028), (64, 7168), (2, 32768), (300, 4096), (2, 1, 128), (7, 3, 4), (48, 32, 128), (9, 40, 128), (130, 128, 256), (9000, 256), (4500, 3, 512), (1100, 6144), (600, 100, 128), (530, 32768)])
 @pytest.mark.parametrize("x", [F32, F16])
 def test_rows_i8(dev, shape, x):
     g = torch.Generator().manual_seed(len(shape) + shape[0])
@@ -209,7 +238,7 @@ def rope_bound(x, dtype):
     return pair * (math.pi + 8) * 2.0 ** -24 + (0 if dtype == F32 else pair * 2.0 ** -11 + 2.0 ** -25)
 
 
-@pytest.mark.parametrize("rows,heads,n", [(1, 1, 32), (1, 32, 64), (3, 5, 64), (64, 32, 64), (65, 40, 64), (7, 128, 64), (5, 3, 96), (5, 9, 256), (2, 1024, 32), (1001, 16, 64)])
+@pytest.mark.parametrize("rows,heads,n", [(1, 1, 32), (1, 32, 64), (3, 5, 64), (64, 32, 64), (65, 40, 64), (7, 128, 64), (5, 3, 96), (5, 9, 256), (2, 1024, 32), (1001, 16, 64), (20000, 3, 64)])
 @pytest.mark.parametrize("x", [F32, F16])
 @pytest.mark.parametrize("out", [F32, F16])
 @pytest.mark.parametrize("rp", [YARN, PLAIN])
