@@ -1,6 +1,10 @@
 // mul_i8.hip -- the product of int8 rows and int8 weights with a scale for each row and each channel
-// (mla_m4_mul_i8): y[t][c] = xs[t] ws[c] sum_k w[c][k] x[t][k], the sum exact in 32 bits.
+// (mla_m4_mul_i8): y[t][c] = xs[t] ws[c] sum_k w[c][k] x[t][k], the sum exact in 32 bits (k <= 131,056), then two f32 products and,
+// for an f16 result, one rounding more.  Integer sums have no order, so however a form cuts k the result is the same bit for bit.
 //
+// Three kernels, as three things bound it.  One to 32 rows: reading the weights once, and latency (direct_kernel).  Tens to hundreds
+// of rows: what a CU can fetch and how many CUs the shape keeps busy (split_kernel, and sum_kernel where k is cut).  More: the matrix
+// instructions (tile_kernel).  choose() below estimates each form's time.
 #include "mla_common.h"
 #include "rows.h"
 #include <type_traits>
@@ -10,34 +14,36 @@ namespace rows {
 
 namespace {
 
-// N neighbouring channels of a row of the result: one store where they are all there and aligned (whole), else the first `left`
-template <int N>
-__device__ __forceinline__ void put(char * p, bool f16, bool whole, int left, const float (&y)[N]) {
-    if (f16) {
-        typedef _Float16 halfn __attribute__((ext_vector_type(N)));
-        halfn v;
+// N neighbouring channels of a row of the result: one store where they are all there and aligned (whole; three need no more than a
+// value's alignment), else the first `left`
+template <int N, typename T>
+__device__ __forceinline__ void put_as(char * p, bool whole, int left, const float (&y)[N]) {
+    T v[N];
 #pragma unroll
-        for (int k = 0; k < N; ++k) v[k] = to_half(y[k]);
-        if (whole) {
-            *reinterpret_cast<halfn *>(p) = v;
+    for (int k = 0; k < N; ++k) {
+        if constexpr (sizeof(T) == 2) v[k] = to_half(y[k]);
+        else v[k] = y[k];
+    }
+    if (whole) {
+        if constexpr (N == 3) {         // (a vector of three would be stored as four)
+            __builtin_memcpy(__builtin_assume_aligned(p, sizeof(T)), v, 3 * sizeof(T));
         } else {
+            typedef T vec __attribute__((ext_vector_type(N)));
+            vec q;
 #pragma unroll
-            for (int k = 0; k < N; ++k)
-                if (k < left) reinterpret_cast<half_t *>(p)[k] = v[k];
+            for (int k = 0; k < N; ++k) q[k] = v[k];
+            *reinterpret_cast<vec *>(p) = q;
         }
     } else {
-        typedef float floatn __attribute__((ext_vector_type(N)));
-        floatn v;
 #pragma unroll
-        for (int k = 0; k < N; ++k) v[k] = y[k];
-        if (whole) {
-            *reinterpret_cast<floatn *>(p) = v;
-        } else {
-#pragma unroll
-            for (int k = 0; k < N; ++k)
-                if (k < left) reinterpret_cast<float *>(p)[k] = v[k];
-        }
+        for (int k = 0; k < N; ++k)
+            if (k < left) reinterpret_cast<T *>(p)[k] = v[k];
     }
+}
+template <int N>
+__device__ __forceinline__ void put(char * p, bool f16, bool whole, int left, const float (&y)[N]) {
+    if (f16) put_as<N, _Float16>(p, whole, left, y);
+    else put_as<N, float>(p, whole, left, y);
 }
 
 // direct_kernel: few rows.  A workgroup of NW waves takes 16 TN channels and 16 rows; wave w takes the 256-byte runs
@@ -120,7 +126,7 @@ constexpr uint32_t PAST = 0xfffffff0u;      // an offset past any resource's end
 template <int WN, int WM, int TN, int TM, int LATE>
 struct Tile {
     static constexpr int NW = WN * WM, NT = 64 * NW, BN = 32 * TN * WN, BM = 32 * TM * WM, BK = 128;
-    static constexpr int STAGE = (BN + BM) * BK, ST = 2;
+    static constexpr int STAGE = (BN + BM) * BK;
     static constexpr int DW = BN / 8 / NW, DX = BM / 8 / NW;           // DMA instructions of a wave and step
     static_assert(BN % (8 * NW) == 0 && BM % (8 * NW) == 0, "whole DMA instructions a wave");
 };
@@ -245,7 +251,7 @@ __global__ __launch_bounds__(64 * WN * WM) void tile_kernel(MulArgs a, int n_ct,
     __syncthreads();
     const int es = a.dst_f16 ? 2 : 4;
     // whole groups of TN channels at aligned places go out in one store
-    const bool whole = c + TN <= a.n && a.dst_nb1 % (TN * es) == 0 && (reinterpret_cast<uintptr_t>(a.dst) & (TN * es - 1)) == 0;
+    const bool whole = c + TN <= a.n && (TN == 3 || (a.dst_nb1 % (TN * es) == 0 && (reinterpret_cast<uintptr_t>(a.dst) & (TN * es - 1)) == 0));
 #pragma unroll
     for (int u = 0; u < TM; ++u)
 #pragma unroll
@@ -291,12 +297,21 @@ struct Split {
 };
 
 template <typename G>
-__global__ __launch_bounds__(G::NT, 2) void split_kernel(MulArgs a, int n_ct, int n_split, i32x4 * work) {
+__global__ __launch_bounds__(G::NT, 2) void split_kernel(MulArgs a, int n_ct, int n_tt, int n_split, i32x4 * work) {
     constexpr int TN = G::TN, TM = G::TM;
     __shared__ __attribute__((aligned(1024))) char lds[G::ST * G::STAGE];
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int tile = blockIdx.x, part = blockIdx.y;
-    const int tt = __builtin_amdgcn_readfirstlane(tile / n_ct), ct = tile - tt * n_ct;
+    // A compute die's workgroups (every eighth) take a run of neighbouring tiles, the rows inside, so that the rows' tiles that read the
+    // same weights share them in the die's L2
+    int tt, ct, part;
+    {
+        const int x = blockIdx.x & 7, groups = gridDim.x;
+        const int i = x * (groups >> 3) + min(x, groups & 7) + (blockIdx.x >> 3);
+        const int at = __builtin_amdgcn_readfirstlane(i / n_tt);
+        tt = i - at * n_tt;
+        part = __builtin_amdgcn_readfirstlane(at / n_ct);
+        ct = at - part * n_ct;
+    }
     const int c0 = ct * G::BN, t0 = tt * G::BM;
     const int all = (a.k + 127) >> 7;
     const int base = __builtin_amdgcn_readfirstlane(all / n_split), rem = all - base * n_split;
@@ -384,7 +399,7 @@ __global__ __launch_bounds__(G::NT, 2) void split_kernel(MulArgs a, int n_ct, in
 #pragma unroll
                 for (int i = 1; i < G::WK; ++i) s += from[64 * i];
                 if (n_split > 1) {
-                    const int64_t quad = ((int64_t)part * gridDim.x + tile) * (G::WN * G::WM * G::F * 4) + (pos * G::F + f0 + f) * 4 + q;
+                    const int64_t quad = ((int64_t)(part * n_tt + tt) * n_ct + ct) * (G::WN * G::WM * G::F * 4) + (pos * G::F + f0 + f) * 4 + q;
                     work[quad * 64 + lane] = s;
                     continue;
                 }
@@ -429,7 +444,7 @@ template <typename G>
 hipError_t split(const MulArgs & a, int n_split, hipStream_t stream) {
     const int n_ct = (a.n + G::BN - 1) / G::BN, n_tt = (a.n_rows + G::BM - 1) / G::BM;
     if ((int64_t)n_ct * n_tt * n_split * G::NT >= (1ll << 32)) return hipErrorInvalidValue;
-    hipLaunchKernelGGL((split_kernel<G>), dim3(n_ct * n_tt, n_split), dim3(G::NT), 0, stream, a, n_ct, n_split, reinterpret_cast<i32x4 *>(a.work));
+    hipLaunchKernelGGL((split_kernel<G>), dim3(n_ct * n_tt * n_split), dim3(G::NT), 0, stream, a, n_ct, n_tt, n_split, reinterpret_cast<i32x4 *>(a.work));
     if (n_split > 1)
         hipLaunchKernelGGL((sum_kernel<G>), dim3(n_ct * n_tt * G::WN * G::WM * G::F), dim3(256), 0, stream, a, n_ct, n_ct * n_tt, n_split,
                            reinterpret_cast<const i32x4 *>(a.work));
@@ -446,29 +461,30 @@ hipError_t direct(const MulArgs & a, hipStream_t stream) {
 // Which kernel takes a product, and in how many parts of k.  Each form's time (us) is estimated as
 //   fixed + step * (steps of 128 bytes a CU runs) + group * (workgroups a CU runs) + mb * (operands and result, MB)
 // and, where k is cut, the sums' launch and their traffic; of direct_kernel as fixed + mb * MB + what a CU fetches.  The constants
-// are fitted to 1,900 times of 120 shapes (1 to 4,001 rows, 576 to 24,576 channels, k 512 to 16,384, cold operands); the form they
-// choose takes 1.03 times the best form's time in the mean, 1.25 at most (512 rows of 576 channels).  What they weigh, in numbers:
-// 64 rows x 7168 x 4096 takes 10.0 us in tiles of 32 x 64 and 12.0 in 64 x 64 (112 workgroups leave half of the CUs idle), 64 x 576 x
-// 7168 takes 7.8 us with k in 4 parts and 10.8 in one, 4,001 x 4096 x 4096 71 us in tiles of 256 and 87 in tiles of 128, 200 x
-// 24,576 x 1536 32 and 23.
+// are fitted to 3,000 times of 225 shapes (1 to 8,000 rows, 576 to 24,576 channels, k 512 to 16,384, cold operands); the form they
+// choose takes 1.01 times the best form's time in the mean, 1.19 at most (150 rows x 24,576 x 1536).  What they weigh, in numbers:
+// 64 rows x 7168 x 4096 takes 9.7 us in tiles of 32 x 64 and 11.5 in 64 x 64 (112 workgroups leave half of the CUs idle), 64 x 576 x
+// 7168 takes 7.5 us with k in 4 parts and 11.1 in one, 4,001 x 4096 x 4096 71 us in tiles of 256 and 86 in tiles of 128, 200 x
+// 24,576 x 1536 32 and 23, and 1,500 x 7168 x 4096 takes 54 us in 192 x 256 (228 workgroups, one round), 64 in 256 x 256 and 76 in 128.
 struct Form {
     int kind, bn, bm;
-    float fixed, step, group, mb, pair, cut, cut_mb;   // pair: per step of two workgroups on a CU at once; direct_kernel: us per 100 KB
+    float fixed, step, group, mb, pair, cut, cut_mb;   // pair: per step of two workgroups at once on a CU; direct_kernel: us per 100 KB
 };
-enum { DIRECT8, DIRECT16, DIRECT8_2, SPLIT11, SPLIT12, SPLIT22, SPLIT32, SPLIT128, TILE128, TILE256 };
+enum { DIRECT8, DIRECT16, DIRECT8_2, SPLIT11, SPLIT12, SPLIT22, SPLIT32, SPLIT128, TILE128, TILE192, TILE256 };
 constexpr Form FORMS[] = {
-    {DIRECT8, 16, 16, 2.2f, 0.f, 0.f, 0.088f, 2.6f, 0.f, 0.f},
-    {DIRECT16, 16, 16, 2.4f, 0.f, 0.f, 0.095f, 2.6f, 0.f, 0.f},
-    {DIRECT8_2, 32, 16, 2.1f, 0.f, 0.f, 0.062f, 2.7f, 0.f, 0.f},
-    {SPLIT11, 32, 32, 2.7f, 0.11f, 0.47f, 0.065f, 0.f, 2.4f, 0.12f},
-    {SPLIT12, 32, 64, 2.4f, 0.15f, 1.1f, 0.036f, 0.f, 2.4f, 0.18f},
-    {SPLIT22, 64, 64, 2.2f, 0.20f, 1.8f, 0.056f, 0.f, 2.4f, 0.18f},
-    {SPLIT32, 96, 64, 2.5f, 0.24f, 2.5f, 0.082f, 0.f, 1.9f, 0.13f},
-    {SPLIT128, 128, 128, 6.2f, 0.33f, 0.f, 0.094f, 0.f, 1.6f, 0.24f},
-    {TILE128, 128, 128, 2.5f, 0.22f, 2.3f, 0.15f, 0.41f, 0.f, 0.f},
-    {TILE256, 256, 256, 0.f, 1.1f, 8.4f, 0.19f, 0.f, 0.f, 0.f},
+    {DIRECT8, 16, 16, 2.2f, 0.f, 0.f, 0.095f, 2.6f, 0.f, 0.f},
+    {DIRECT16, 16, 16, 2.4f, 0.f, 0.f, 0.10f, 2.7f, 0.f, 0.f},
+    {DIRECT8_2, 32, 16, 2.1f, 0.f, 0.f, 0.062f, 2.8f, 0.f, 0.f},
+    {SPLIT11, 32, 32, 2.5f, 0.058f, 0.73f, 0.066f, 0.063f, 2.3f, 0.19f},
+    {SPLIT12, 32, 64, 2.2f, 0.11f, 1.3f, 0.042f, 0.044f, 2.2f, 0.17f},
+    {SPLIT22, 64, 64, 2.4f, 0.16f, 1.9f, 0.075f, 0.027f, 2.0f, 0.16f},
+    {SPLIT32, 96, 64, 3.0f, 0.20f, 2.2f, 0.098f, 0.011f, 1.7f, 0.14f},
+    {SPLIT128, 128, 128, 6.7f, 0.33f, 0.f, 0.11f, 0.f, 0.8f, 0.25f},
+    {TILE128, 128, 128, 2.9f, 0.20f, 1.8f, 0.15f, 0.44f, 0.f, 0.f},
+    {TILE192, 192, 256, 0.f, 0.91f, 5.5f, 0.18f, 0.f, 0.f, 0.f},
+    {TILE256, 256, 256, 0.f, 1.1f, 8.2f, 0.19f, 0.f, 0.f, 0.f},
 };
-constexpr int CUS = 256, MOST_PARTS = 12, FEW_ROWS = 32, MANY_ROWS = 100, MOST_CUT = 512;
+constexpr int CUS = 256, MOST_PARTS = 12, FEW_ROWS = 48, MANY_ROWS = 100, MOST_CUT = 512;
 
 struct Choice {
     int kind, n_split;
@@ -526,6 +542,7 @@ hipError_t launch_mul_i8(const MulArgs & a, hipStream_t stream) {
         case SPLIT32: return split<Split<1, 1, 4, 3, 2>>(a, c.n_split, stream);
         case SPLIT128: return split<Split<2, 2, 2, 2, 2>>(a, c.n_split, stream);
         case TILE128: return tile<2, 2, 2, 2, 4>(a, stream);
+        case TILE192: return tile<2, 4, 3, 2, 5>(a, stream);
         default: return tile<2, 4, 4, 2, 6>(a, stream);
     }
 }

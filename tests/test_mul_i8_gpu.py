@@ -62,7 +62,8 @@ def test_large(dev, rows, n, k):
 @pytest.mark.parametrize("rows,n,k", [
     (1, 24577, 1552), (31, 24570, 1536), (32, 576, 7184), (48, 2112, 7168), (64, 2100, 7152), (100, 570, 7168), (64, 7168, 4096), (61, 7150, 4112),
     (128, 7168, 4096), (125, 7100, 4080), (60, 24576, 1536), (64, 7168, 16384), (300, 7168, 4096), (290, 7101, 4112), (130, 7168, 16384),
-    (200, 24576, 1536), (1000, 7168, 4096), (1030, 4100, 4112), (3000, 4096, 528), (4001, 2112, 1040)])
+    (200, 24576, 1536), (1000, 7168, 4096), (1030, 4100, 4112), (3000, 4096, 528), (4001, 2112, 1040),
+    (300, 24576, 1536), (389, 24570, 1552), (1401, 7100, 2064), (515, 24007, 528)])
 def test_forms(dev, rows, n, k):
     """Shapes that the forms of the product share out among them, with and without a workspace, into rows at odd places."""
     a = make(dev, rows, n, k, 3)
