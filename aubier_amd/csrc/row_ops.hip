@@ -1,12 +1,17 @@
 // row_ops.hip -- rows around a batch's attention: the norms with gate and residual and the int8 rows (norm_kernel), the
 // rope parts of q (qrope_kernel).
 //
-// norm_kernel: a workgroup per row, the row in registers, so x and the residual are read once and r and h written once.
+// norm_kernel: a workgroup per row, the row in registers, so x and the residual are read once and r and h written once; of many rows
+// the next one's values are on their way meanwhile.  Bound by memory where there are many rows (8,000 of 4096, f16 to int8 over an f32
+// residual: 78 us, 4.6 TB/s; of 7168, f32: 163 us, 4.6; int8 rows of 5,000 x 40 x 128: 25 us, 5.1, where a large copy makes 5.0), by
+// the launch and a row's latency where there are few (64 of 7168 6.2 us, 48 int8 rows of 4096 2.7).
 // Everything is taken in 64 bits and rounded where it is stored, or as if it were (int8).  That makes the int8 rows what their
 // definition says (a value next to a border between two integers falls on its side) and costs little, as the card's rate for
 // 64-bit vector instructions is that of 32-bit ones and the kernel waits for memory.
 //
-// qrope_kernel: a wavefront per token; a lane turns the same pairs of several heads, so an angle is taken once for them.
+// qrope_kernel: a wavefront per token; a lane turns the same pairs of several heads, so an angle is taken once for them.  5,000 x 40
+// heads of f16: 16.3 us (4.7 TB/s); 64 x 32: 3.7 us, of which the launch takes 2.2, the position, the angle in 64 bits and a head's
+// values behind one another the rest.
 #include "mla_common.h"
 #include "rows.h"
 
@@ -111,20 +116,27 @@ __device__ __forceinline__ void again(f32x4 (&v)[N]) {
 
 constexpr int PIECES = 3;
 
-// NT threads, C groups of four values a thread.  RES: no residual, one of f32 (1) or f16 (2), or PIECES: int8 rows of x as it is, in
+// NT threads, C groups of four values a thread.  ONE: a row a workgroup, and no row behind it to load.  RES: no residual, one of f32 (1) or f16 (2), or PIECES: int8 rows of x as it is, in
 // pieces, without any norm.
 //
 // int8.  The row's largest |r pre| is found in 64 bits, where such products are exact.  127 |r pre| / top is then taken in f32, off
 // by less than 4 * 2^-24 * 127 < 2^-15 (from a quotient in 64 bits where the row is near the ends of f32's range), and compared with
 // the border in 64 bits where it lies within 2^-14 of one between two integers (a value in 8,000).
-template <int NT, int C, bool XH, int RES>
-__global__ __launch_bounds__(NT, 4) void norm_kernel(NormArgs a) {
+template <int NT, int C, bool XH, int RES, bool ONE>
+__global__ __launch_bounds__(NT, C > 3 && NT <= 512 ? 2 : 4) void norm_kernel(NormArgs a) {
     // by turns, so that a row's reductions need not wait for the row before to have read its own
     __shared__ double reds[2][2][NT / 64][2];
     const int tid = threadIdx.x;
     constexpr bool PLAIN = RES == PIECES;
     const bool i8 = PLAIN || a.dst_type == OUT_I8;
+    // Where the registers hold them, weights are loaded ahead of the reductions, and the next row's values ahead of this one's end.
+    constexpr bool EARLY = C <= (NT > 512 ? 3 : 6), AHEAD = EARLY && !ONE;
     int turn = 0;
+    auto me = [&]() {                                       // (a wide row's places are worked out anew, not held from use to use)
+        int t = tid;
+        if constexpr (!EARLY) asm volatile("" : "+v"(t));
+        return t;
+    };
     // A row's values are on their way while the row before is worked on.  (Places past the row's end read its first values;
     // what is made of them is not stored, and adds nothing.)
     Four<XH> raw[C];
@@ -133,7 +145,7 @@ __global__ __launch_bounds__(NT, 4) void norm_kernel(NormArgs a) {
         const char * xr = a.x + (int64_t)row * a.x_nb1;
 #pragma unroll
         for (int i = 0; i < C; ++i) {
-            const int c = 4 * (NT * i + tid), at = c < a.n ? c : 0;
+            const int c = 4 * (NT * i + me()), at = c < a.n ? c : 0;
             if constexpr (RES == PIECES) {
                 const int piece = a.d_shift >= 0 ? at >> a.d_shift : at / a.d;      // (one piece: a shift that leaves 0)
                 raw[i].load(xr + (int64_t)piece * a.x_nbh, at - piece * a.d);
@@ -146,66 +158,88 @@ __global__ __launch_bounds__(NT, 4) void norm_kernel(NormArgs a) {
         if constexpr (RES == 1 || RES == 2) {
 #pragma unroll
             for (int i = 0; i < C; ++i) {
-                const int c = 4 * (NT * i + tid);
+                const int c = 4 * (NT * i + me());
                 rs[i].load(a.res + (int64_t)row * a.res_nb1, c < a.n ? c : 0);
             }
         }
     };
     // weights of the thread's channels, or ones
+    auto weight = [&](int i, const void * from) {
+        const int c = 4 * (NT * i + me());
+        if (PLAIN || from == nullptr) return f32x4{1.f, 1.f, 1.f, 1.f};
+        return *reinterpret_cast<const f32x4 *>(static_cast<const char *>(from) + 4 * (int64_t)(c < a.n ? c : 0));
+    };
     auto weights = [&](f32x4 (&w)[C], const void * from) {
 #pragma unroll
-        for (int i = 0; i < C; ++i) {
-            const int c = 4 * (NT * i + tid);
-            w[i] = f32x4{1.f, 1.f, 1.f, 1.f};
-            if (!PLAIN && from != nullptr) w[i] = *reinterpret_cast<const f32x4 *>(static_cast<const char *>(from) + 4 * (int64_t)(c < a.n ? c : 0));
+        for (int i = 0; i < C; ++i) w[i] = weight(i, from);
+    };
+    // A wide row's groups are taken two after two, as the 64-bit forms of all of them at once, and the places that me() hides, do not fit
+    // in the registers (64 rows of 16,384: 10.9 us; 18.0 where they spill, and of 24,576 20 and 55)
+    auto two = [&](int i) {
+        if constexpr (!EARLY) {
+            if (i & 1) __builtin_amdgcn_sched_barrier(0);
         }
     };
-    load_x(blockIdx.x);
-    load_res(blockIdx.x);
+    if constexpr (EARLY) {
+        load_x(blockIdx.x);
+        load_res(blockIdx.x);
+    }
     for (int row = blockIdx.x; row < a.n_rows; row += gridDim.x, turn ^= 1) {
-        const int next = min(row + (int)gridDim.x, a.n_rows - 1);
+        const int next = AHEAD ? min(row + (int)gridDim.x, a.n_rows - 1) : 0;
+        if constexpr (!EARLY) {
+            load_x(row);
+            load_res(row);
+        }
         f32x4 v[C], pw[C], gw[C], hw[C];
 #pragma unroll
-        for (int i = 0; i < C; ++i) v[i] = 4 * (NT * i + tid) < a.n ? raw[i].get() : f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int i = 0; i < C; ++i) v[i] = 4 * (NT * i + me()) < a.n ? raw[i].get() : f32x4{0.f, 0.f, 0.f, 0.f};
         const char * gate = a.gate != nullptr ? a.gate + (int64_t)row * a.gate_nb1 : nullptr;
-        weights(pw, a.post);
-        weights(gw, a.gate_wide ? gate : nullptr);
+        const char * wide = a.gate_wide ? gate : nullptr;
+        if constexpr (EARLY) {
+            weights(pw, a.post);
+            weights(gw, wide);
+        }
         if constexpr (C <= 2) weights(hw, a.pre);
-        load_x(next);
+        if constexpr (AHEAD) load_x(next);
         double factor = 1.0;
         if (gate != nullptr && !a.gate_wide) factor = (double)*reinterpret_cast<const float *>(gate);
         if constexpr (RES == 1 || RES == 2) factor *= (double)a.scale;
         double sum = 0.0, top = 0.0;
         if (!PLAIN && a.post != nullptr) {
 #pragma unroll
-            for (int i = 0; i < C; ++i)
+            for (int i = 0; i < C; ++i) {
 #pragma unroll
                 for (int k = 0; k < 4; ++k) sum = fma((double)v[i][k], (double)v[i][k], sum);
+                two(i);
+            }
             again(v);
             block_all<NT, true, false>(sum, top, reds[turn][0]);
             factor *= inverse_root(fma(sum, a.per_n, (double)a.eps));
         }
+        if constexpr (!EARLY) weights(pw, a.post);
         // r, as it is stored
         if (!PLAIN && (RES == 1 || RES == 2 || a.post != nullptr || gate != nullptr)) {
 #pragma unroll
             for (int i = 0; i < C; ++i) {
-                const int c = 4 * (NT * i + tid);
+                const int c = 4 * (NT * i + me());
                 const f32x4 before = RES == 1 || RES == 2 ? rs[i].get() : f32x4{0.f, 0.f, 0.f, 0.f};
+                const f32x4 p = pw[i], g = EARLY ? gw[i] : weight(i, wide);
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
                     double y = (double)v[i][k] * factor;
-                    const double w = (double)pw[i][k] * (double)gw[i][k];
+                    const double w = (double)p[k] * (double)g[k];
                     if constexpr (RES == 1 || RES == 2) y = fma(y, w, (double)before[k]);
                     else y *= w;
                     v[i][k] = c < a.n ? (float)y : 0.0f;
                 }
+                two(i);
             }
         }
-        load_res(next);
+        if constexpr (AHEAD) load_res(next);
         if (!PLAIN && a.res_out_type != OUT_NONE) {
 #pragma unroll
             for (int i = 0; i < C; ++i) {
-                const int c = 4 * (NT * i + tid);
+                const int c = 4 * (NT * i + me());
                 if (c >= a.n) continue;
                 if (a.res_out_type == OUT_F16) {
 #pragma unroll
@@ -222,21 +256,25 @@ __global__ __launch_bounds__(NT, 4) void norm_kernel(NormArgs a) {
             double inv = 1.0;
             if (a.rms) {
 #pragma unroll
-                for (int i = 0; i < C; ++i)
+                for (int i = 0; i < C; ++i) {
 #pragma unroll
                     for (int k = 0; k < 4; ++k) sum = fma((double)v[i][k], (double)v[i][k], sum);
+                    two(i);
+                }
                 again(v);
                 block_all<NT, true, false>(sum, top, reds[turn][1]);
                 inv = inverse_root(fma(sum, a.per_n, (double)a.eps));
             }
 #pragma unroll
             for (int i = 0; i < C; ++i) {
-                const int c = 4 * (NT * i + tid);
+                const int c = 4 * (NT * i + me());
                 if (c >= a.n) continue;
+                const f32x4 w = hw[i];
                 f32x4 h;
 #pragma unroll
-                for (int k = 0; k < 4; ++k) h[k] = (float)((double)v[i][k] * inv * (double)hw[i][k]);
+                for (int k = 0; k < 4; ++k) h[k] = (float)((double)v[i][k] * inv * (double)w[k]);
                 store4(out, a.dst_type, c, h);
+                two(i);
             }
             continue;
         }
@@ -252,14 +290,17 @@ __global__ __launch_bounds__(NT, 4) void norm_kernel(NormArgs a) {
         } else {
             float finite = 0.0f;                        // NaN where a value is none or an infinity
 #pragma unroll
-            for (int i = 0; i < C; ++i)
+            for (int i = 0; i < C; ++i) {
+                const f32x4 w = hw[i];
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
                     const double r = (double)v[i][k];
                     sum = fma(r, r, sum);
-                    top = fmax(top, fabs(r * (double)hw[i][k]));
-                    finite = fmaf(v[i][k], 0.0f, fmaf(hw[i][k], 0.0f, finite));
+                    top = fmax(top, fabs(r * (double)w[k]));
+                    finite = fmaf(v[i][k], 0.0f, fmaf(w[k], 0.0f, finite));
                 }
+                two(i);
+            }
             if (finite != 0.0f) top = __builtin_inf();
             again(v);
             again(hw);
@@ -271,14 +312,15 @@ __global__ __launch_bounds__(NT, 4) void norm_kernel(NormArgs a) {
         const float per = mid ? (float)per64 : 0.0f;
 #pragma unroll
         for (int i = 0; i < C; ++i) {
-            const int c = 4 * (NT * i + tid);
+            const int c = 4 * (NT * i + me());
             if (c >= a.n) continue;
+            const f32x4 w = hw[i];
             int q[4];
             float t[4], off = 0.0f;
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-                if (mid) t[k] = v[i][k] * hw[i][k] * per;
-                else t[k] = there ? (float)((double)v[i][k] * (double)hw[i][k] * per64) : 0.0f;
+                if (mid) t[k] = v[i][k] * w[k] * per;
+                else t[k] = there ? (float)((double)v[i][k] * (double)w[k] * per64) : 0.0f;
                 const float n = rintf(t[k]);
                 q[k] = (int)n;
                 off = fmaxf(off, fabsf(t[k] - n));
@@ -288,12 +330,13 @@ __global__ __launch_bounds__(NT, 4) void norm_kernel(NormArgs a) {
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
                     const float below = floorf(fabsf(t[k]));
-                    const double h = fabs((double)v[i][k] * (double)hw[i][k]);
+                    const double h = fabs((double)v[i][k] * (double)w[k]);
                     const int n = (int)below + (h * 127.0 >= ((double)below + 0.5) * top ? 1 : 0);
                     q[k] = t[k] < 0.0f ? -n : n;
                 }
             }
             *reinterpret_cast<uint32_t *>(out + c) = pack4(q[0], q[1], q[2], q[3]);
+            two(i);
         }
         if (tid == 0) {
             const double inv = !PLAIN && a.rms ? inverse_root(fma(sum, a.per_n, (double)a.eps)) : 1.0;
@@ -335,46 +378,57 @@ __global__ __launch_bounds__(256) void qrope_kernel(QropeArgs a) {
     }
 }
 
-constexpr int FEW = 256;                // rows, one a CU: as many threads as a row has use for
+constexpr int FEW = 256;                // rows, one a CU
 
-template <int NT, int C>
+template <int NT, int C, bool ONE>
 hipError_t norm(const NormArgs & a, hipStream_t stream) {
     auto go = [&](auto kernel, int waves) {
-        const int at_once = 256 * (64 * waves / NT);    // workgroups that the card holds
+        const int at_once = ONE ? FEW : 256 * (64 * waves / NT);        // workgroups that the card holds
         hipLaunchKernelGGL(kernel, dim3(a.n_rows < at_once ? a.n_rows : at_once), dim3(NT), 0, stream, a);
         return hipGetLastError();
     };
     const int res = a.d != 0 ? PIECES : a.res == nullptr ? 0 : a.res_f16 ? 2 : 1;
     switch (res + (a.x_f16 ? 4 : 0)) {
-        case 0: return go(norm_kernel<NT, C, false, 0>, 16);
-        case 1: return go(norm_kernel<NT, C, false, 1>, 16);
-        case 2: return go(norm_kernel<NT, C, false, 2>, 16);
-        case 3: return go(norm_kernel<NT, C, false, PIECES>, C <= 3 ? 32 : 16);
-        case 4: return go(norm_kernel<NT, C, true, 0>, 16);
-        case 5: return go(norm_kernel<NT, C, true, 1>, 16);
-        case 6: return go(norm_kernel<NT, C, true, 2>, 16);
-        default: return go(norm_kernel<NT, C, true, PIECES>, C <= 3 ? 32 : 16);
+        case 0: return go(norm_kernel<NT, C, false, 0, ONE>, 16);
+        case 1: return go(norm_kernel<NT, C, false, 1, ONE>, 16);
+        case 2: return go(norm_kernel<NT, C, false, 2, ONE>, 16);
+        case 3: return go(norm_kernel<NT, C, false, PIECES, ONE>, C <= 3 ? 32 : 16);
+        case 4: return go(norm_kernel<NT, C, true, 0, ONE>, 16);
+        case 5: return go(norm_kernel<NT, C, true, 1, ONE>, 16);
+        case 6: return go(norm_kernel<NT, C, true, 2, ONE>, 16);
+        default: return go(norm_kernel<NT, C, true, PIECES, ONE>, C <= 3 ? 32 : 16);
     }
 }
 
 }  // namespace
 
 hipError_t launch_norm(const NormArgs & a, hipStream_t stream) {
-    // Many rows: as few threads a row as keep its values in registers, so that a CU has several rows at different places of their
-    // way (8,000 rows of 1,536: 25 us by 256 threads, 35 by 512).  Few rows: more threads (one of 4,096: 4.1 us by 512, 5.8 by 256).
-    const bool few = a.n_rows <= FEW;
+    if (a.n > MAX_N) return hipErrorInvalidValue;
     const int fours = (a.n + 255) / 256;                // groups of a thread, of a wavefront
-    if (!few && fours == 1) return norm<64, 1>(a, stream);
-    if (!few && fours == 2) return norm<64, 2>(a, stream);
-    if (fours <= 4) return norm<256, 1>(a, stream);
-    if (fours <= 8) return few ? norm<512, 1>(a, stream) : norm<256, 2>(a, stream);
-    if (fours <= 16) return norm<512, 2>(a, stream);
-    if (fours <= 24) return norm<512, 3>(a, stream);
-    if (fours <= 32) return norm<1024, 2>(a, stream);
-    if (fours <= 48) return norm<1024, 3>(a, stream);
-    if (fours <= 64) return norm<1024, 4>(a, stream);
-    if (a.n <= MAX_N) return norm<1024, 8>(a, stream);
-    return hipErrorInvalidValue;
+    if (a.n_rows <= FEW) {
+        // A CU has one of them: threads that share its work, but not so many that starting and joining them costs more (one of 4,096: 4.0
+        // us by 512, 4.4 by 1,024, 4.8 by 256; 64 of 7168: 6.2 by 1,024 and by 512; 64 of 12,288: 9.0 by 512, 9.6 by 1,024)
+        if (fours <= 4) return norm<256, 1, true>(a, stream);
+        if (fours <= 8) return norm<512, 1, true>(a, stream);
+        if (fours <= 16) return norm<512, 2, true>(a, stream);
+        if (fours <= 24) return norm<512, 3, true>(a, stream);
+        if (fours <= 32) return norm<1024, 2, true>(a, stream);
+        if (fours <= 48) return norm<512, 6, true>(a, stream);
+        if (fours <= 64) return norm<1024, 4, true>(a, stream);
+        return norm<1024, 8, true>(a, stream);
+    }
+    // As few threads a row as keep its values in registers, so that a CU has several rows at different places of their way (8,000 rows
+    // of 1,536: 25 us by 256 threads, 35 by 512)
+    if (fours == 1) return norm<64, 1, false>(a, stream);
+    if (fours == 2) return norm<64, 2, false>(a, stream);
+    if (fours <= 4) return norm<256, 1, false>(a, stream);
+    if (fours <= 8) return norm<256, 2, false>(a, stream);
+    if (fours <= 16) return norm<512, 2, false>(a, stream);
+    if (fours <= 24) return norm<512, 3, false>(a, stream);
+    if (fours <= 32) return norm<1024, 2, false>(a, stream);
+    if (fours <= 48) return norm<1024, 3, false>(a, stream);
+    if (fours <= 64) return norm<1024, 4, false>(a, stream);
+    return norm<1024, 8, false>(a, stream);
 }
 
 hipError_t launch_qrope(const QropeArgs & a, hipStream_t stream) {
