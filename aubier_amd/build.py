@@ -1,4 +1,4 @@
-"""Build the gfx950 kernel library (aubier_amd/libmla_m4.so), the compiled calls of the paged operators
+"""Build the gfx950 kernel library (aubier_amd/libmla_m4.so), the compiled calls of a batch's operators
 (aubier_amd/_binding.so) and the CPU oracle (oracle/libmla_oracle.so), in-tree.
 
     python -m aubier_amd.build            # all

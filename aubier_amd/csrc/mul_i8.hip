@@ -50,7 +50,7 @@ __device__ __forceinline__ void put(char * p, bool f16, bool whole, int left, co
 // w, w + NW, ... of k, its operands straight from memory (lane l: row l % 16, 16 bytes at 16 (l / 16), as
 // v_mfma_i32_16x16x64_i8 takes both; a run is 4 of its steps), and the waves' integers are added in LDS.  Integer sums have
 // no order, so the result is the same however k is cut.  Bound by memory latency and by what a CU fetches (40 KB/us): 1 row x 576
-// x 7168 6.4 us, x 7168 x 4096 7.7 us (3.8 TB/s), x 24576 x 1536 8.2 us (4.6 TB/s).
+// x 7168 5.9 us, x 7168 x 4096 8.1 us (3.6 TB/s), x 24576 x 1536 8.3 us (4.6 TB/s).
 template <int NW, int TN>
 __global__ __launch_bounds__(64 * NW) void direct_kernel(MulArgs a) {
     constexpr int U = 4, RUN = 64 * U;
@@ -115,6 +115,10 @@ __global__ __launch_bounds__(64 * NW) void direct_kernel(MulArgs a) {
 //
 // One barrier a step, ahead of the last quarter's products, whose operands are in registers by then: behind it the next
 // step's first operands are read and the DMA of the step after the next is sent into the stage that all have read.
+//
+// Bound by power where the card is full: 8,000 rows x 7168 x 16,384 798 us on the best card (2.36 POP/s at 1.7 GHz, matrix instructions
+// busy 64% of the cycles; the library's int8 product alone 781).  8192 x 8192 x 4096: 291 us; without the DMA 257, without the operand
+// reads 263, without both 219, 212 without the barrier too.  300 x 24,576 x 1536 in 192 x 256: 22 us, a step 0.9, start and end 5.5.
 typedef int i32x16 __attribute__((ext_vector_type(16)));
 
 __device__ __forceinline__ void tile_dma16(i32x4 rsrc, uint32_t voff, uint32_t soff, uint32_t lds_base) {
@@ -282,7 +286,9 @@ hipError_t tile(const MulArgs & a, hipStream_t stream) {
 // split_kernel: what lies between.  WN x WM x WK waves take 32 TN WN channels and 32 TM WM rows of a part of k (one of n_split); of
 // every 128-byte step the WK waves of one place take 128 / WK bytes of each row, so operand bytes are read from LDS less often than by
 // waves that share k, and their integers are added in LDS at the end.  ST stages, filled by DMA ST - 1 steps ahead.  Where k is cut,
-// the sums of the parts go to the workspace as they lie in the lanes, and sum_kernel puts them together.
+// the sums of the parts go to the workspace as they lie in the lanes, and sum_kernel puts them together (2.3 us of the launch and its
+// reads).  Bound by the start of the stream and by what a CU fetches: 64 rows x 7168 x 4096 9.2 us (3.3 TB/s), 64 x 7168 x 16,384 33 us
+// (3.6 TB/s), 300 x 4096 x 4096 14.5 us.
 template <int WN_, int WM_, int WK_, int TN_, int TM_>
 struct Split {
     static constexpr int WN = WN_, WM = WM_, WK = WK_, TN = TN_, TM = TM_;

@@ -3,7 +3,7 @@
 //
 // norm_kernel: a workgroup per row, the row in registers, so x and the residual are read once and r and h written once; of many rows
 // the next one's values are on their way meanwhile.  Bound by memory where there are many rows (8,000 of 4096, f16 to int8 over an f32
-// residual: 78 us, 4.6 TB/s; of 7168, f32: 163 us, 4.6; int8 rows of 5,000 x 40 x 128: 25 us, 5.1, where a large copy makes 5.0), by
+// residual: 80 us, 4.5 TB/s; of 7168, f32: 163 us, 4.6; int8 rows of 5,000 x 40 x 128: 25 us, 5.1, where a large copy makes 5.0), by
 // the launch and a row's latency where there are few (64 of 7168 6.2 us, 48 int8 rows of 4096 2.7).
 // Everything is taken in 64 bits and rounded where it is stored, or as if it were (int8).  That makes the int8 rows what their
 // definition says (a value next to a border between two integers falls on its side) and costs little, as the card's rate for

@@ -306,7 +306,7 @@ _native = None
 
 
 def _calls():
-    """The paged operators' calls as compiled from binding.cpp (13 -> 6 us of host time each), or False where that module is
+    """A batch's operators' calls as compiled from binding.cpp (13 -> 6 us of host time each), or False where that module is
     not built or was built for another PyTorch: then they go through ctypes, with the same results."""
     global _native
     if _native is None:
