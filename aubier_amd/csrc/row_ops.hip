@@ -418,11 +418,12 @@ hipError_t launch_norm(const NormArgs & a, hipStream_t stream) {
         return norm<1024, 8, true>(a, stream);
     }
     // As few threads a row as keep its values in registers, so that a CU has several rows at different places of their way (8,000 rows
-    // of 1,536: 25 us by 256 threads, 35 by 512)
+    // of 1,536: 25 us by 256 threads, 35 by 512; 6,000 of 2,560: 53 by 256, 63 by 512)
     if (fours == 1) return norm<64, 1, false>(a, stream);
     if (fours == 2) return norm<64, 2, false>(a, stream);
     if (fours <= 4) return norm<256, 1, false>(a, stream);
     if (fours <= 8) return norm<256, 2, false>(a, stream);
+    if (fours <= 12) return norm<256, 3, false>(a, stream);
     if (fours <= 16) return norm<512, 2, false>(a, stream);
     if (fours <= 24) return norm<512, 3, false>(a, stream);
     if (fours <= 32) return norm<1024, 2, false>(a, stream);

@@ -79,7 +79,7 @@ def test_norm_rows(dev, pre, rows):
         check_norm(i, dtype=dtype)
 
 
-@pytest.mark.parametrize("n,rows", [(4, 20000), (256, 9000), (260, 9000), (512, 6001), (516, 5000), (1024, 5000), (1536, 4500), (2048, 4400), (2052, 2100), (4096, 2100),
+@pytest.mark.parametrize("n,rows", [(4, 20000), (256, 9000), (260, 9000), (512, 6001), (516, 5000), (1024, 5000), (1536, 4500), (2048, 4400), (2052, 2100), (2560, 2100), (4096, 2100),
                                     (5120, 1100), (6144, 1100), (7168, 1030), (8192, 600), (12288, 600), (12292, 600), (16384, 530), (32768, 530)])
 @pytest.mark.parametrize("x,res", [(F32, F32), (F16, F16), (F32, None)])
 def test_norm_many_rows(dev, n, rows, x, res):
