@@ -201,7 +201,7 @@ PyObject * kqkv_paged(PyObject *, PyObject * const * a, Py_ssize_t n) {
         if (!work.is_cuda() || (int)work.get_device() != c.device || !work.is_contiguous()) return PyLong_FromLong(MLA_M4_ERR_WORKSPACE);
     } else {
         const size_t need = lib.workspace_bytes(vk, vq, vp, vf, vo);
-        if (need > 0) work = at::empty({(int64_t)need}, at::TensorOptions().dtype(at::kByte).device(q.device()));
+        if (need > 0) work = fresh({(int64_t)need}, at::kByte, q);
     }
     c.status = page_size != (int32_t)page_size ? MLA_M4_ERR_ARG
         : lib.kqkv_paged(vk, vq, vp, vn, vt, (int32_t)page_size, vf, (float)scale, vo, work.defined() ? work.data_ptr() : nullptr,
@@ -299,7 +299,7 @@ PyObject * mul_i8(PyObject *, PyObject * const * a, Py_ssize_t n) {
         if (!work.is_cuda() || (int)work.get_device() != c.device || !work.is_contiguous()) return PyLong_FromLong(MLA_M4_ERR_WORKSPACE);
     } else {
         const size_t need = lib.mul_workspace_bytes(vw, vx);
-        if (need > 0) work = at::empty({(int64_t)need}, at::TensorOptions().dtype(at::kByte).device(x.device()));
+        if (need > 0) work = fresh({(int64_t)need}, at::kByte, x);
     }
     c.status = lib.mul_i8(vw, vs, vx, vt, vd, work.defined() ? work.data_ptr() : nullptr, work.defined() ? (size_t)work.nbytes() : 0, stream);
     return c.status != 0 ? PyLong_FromLong(c.status) : THPVariable_Wrap(out);
