@@ -121,7 +121,7 @@ constexpr int PIECES = 3;
 //
 // int8.  The row's largest |r pre| is found in 64 bits, where such products are exact.  127 |r pre| / top is then taken in f32, off
 // by less than 4 * 2^-24 * 127 < 2^-15 (from a quotient in 64 bits where the row is near the ends of f32's range), and compared with
-// the border in 64 bits where it lies within 2^-14 of one between two integers (a value in 8,000).
+// the border exactly where it lies within 2^-14 of one between two integers (a value in 8,000).
 template <int NT, int C, bool XH, int RES, bool ONE>
 __global__ __launch_bounds__(NT, C > 3 && NT <= 512 ? 2 : 4) void norm_kernel(NormArgs a) {
     // by turns, so that a row's reductions need not wait for the row before to have read its own
@@ -326,12 +326,13 @@ __global__ __launch_bounds__(NT, C > 3 && NT <= 512 ? 2 : 4) void norm_kernel(No
                 off = fmaxf(off, fabsf(t[k] - n));
             }
             if (off > 0.5f - 0x1p-14f) {
-                // 127 |r pre| against (the integer below + 1 / 2) top
+                // 127 |r pre| against (the integer below + 1 / 2) top, which take 55 and 56 bits.  Next to the border the latter's distance
+                // from 128 |r pre|, a multiple of 2^-48 of top's leading bit and less than twice top, is a double: compared with |r pre|.
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
                     const float below = floorf(fabsf(t[k]));
                     const double h = fabs((double)v[i][k] * (double)w[k]);
-                    const int n = (int)below + (h * 127.0 >= ((double)below + 0.5) * top ? 1 : 0);
+                    const int n = (int)below + (fma(-((double)below + 0.5), top, 128.0 * h) >= h ? 1 : 0);
                     q[k] = t[k] < 0.0f ? -n : n;
                 }
             }

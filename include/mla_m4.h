@@ -368,7 +368,7 @@ int mla_m4_supports_kqkv_paged(const mla_m4_tensor * kcache, const mla_m4_tensor
  *
  * int8 rows.  A row v of finite values is held as integers q in [-127, 127] and one f32 scale:
  *   top = max |v|,  scale = top / 127,  q = 127 v / top rounded to the nearest, half away from zero
- * (all zeros: scale 0, q 0).  The integers are exactly these: the rounding is decided in 64 bits.  A row
+ * (all zeros: scale 0, q 0).  The integers are exactly these, next to the borders between two too.  A row
  * that holds a NaN or an infinity gets scale NaN and q 0, so its products are NaN.  Where top < 2^-119 the
  * scale itself is a subnormal f32 and rounds coarser.
  * ------------------------------------------------------------------------------------------- */
