@@ -10,6 +10,7 @@
 #include <ATen/ATen.h>
 #include <ATen/EmptyTensor.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -99,12 +100,15 @@ bool tensors(PyObject * const * args, int n, bool or_none = false) {
     return true;
 }
 
-// A new tensor where `like` is, as at::empty's: the first by it, the rest straight from the allocator that it took (0.3 us less each)
+// A new tensor where `like` is, as at::empty's: the first by it, the rest straight from the allocator that it took (0.3 us less each,
+// without the fill of new memory that torch's deterministic mode may ask for; every call writes all of its results).  Under a dispatch
+// mode all come by at::empty: a mode sees them, and what it makes of one (a fake tensor's allocator gives no memory) is not kept.
 at::Tensor fresh(at::IntArrayRef size, at::ScalarType type, const at::Tensor & like) {
     static c10::Allocator * from = nullptr;             // (behind Python's lock)
-    if (from == nullptr || !like.is_cuda()) {
+    const bool modes = c10::impl::TorchDispatchModeTLS::any_modes_set();
+    if (from == nullptr || !like.is_cuda() || modes) {
         const at::Tensor t = at::empty(size, at::TensorOptions().dtype(type).device(like.device()));
-        if (like.is_cuda()) from = t.storage().allocator();
+        if (!modes && t.storage().device().is_cuda()) from = t.storage().allocator();
         return t;
     }
     const c10::DeviceGuard guard(like.device());
