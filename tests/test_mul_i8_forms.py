@@ -25,3 +25,12 @@ def test_every_form_is_chosen():
                 assert U.form_of(rows, n, k, False)[1:] == (1, 0)
                 seen |= {(name, parts > 1), (U.form_of(rows, n, k, False)[0], False)}
     assert seen == {(f, cut) for f, (_, _, cuts) in forms.items() for cut in ({False, cuts})}
+
+
+def test_shapes_of_every_form():
+    """The shapes that the GPU tests run are given to the forms that they are listed under: uncut without a workspace, cut with one."""
+    assert set(U.SHAPES) == {(f, cut) for f, (_, _, cuts) in U.forms().items() for cut in ({False, cuts})}
+    for (form, cut), shapes in U.SHAPES.items():
+        for s in shapes:
+            name, parts, _ = U.form_of(*s, cut)
+            assert (name, parts > 1) == (form, cut), (s, name, parts)
