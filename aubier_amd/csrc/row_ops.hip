@@ -415,8 +415,7 @@ hipError_t launch_norm(const NormArgs & a, hipStream_t stream) {
         if (fours <= 24) return norm<512, 3, true>(a, stream);
         if (fours <= 32) return norm<1024, 2, true>(a, stream);
         if (fours <= 48) return norm<512, 6, true>(a, stream);
-        if (fours <= 64) return norm<1024, 4, true>(a, stream);
-        return norm<1024, 8, true>(a, stream);
+        // (wider ones load no row ahead in any case: the kernels of many rows below)
     }
     // As few threads a row as keep its values in registers, so that a CU has several rows at different places of their way (8,000 rows
     // of 1,536: 25 us by 256 threads, 35 by 512; 6,000 of 2,560: 53 by 256, 63 by 512)
