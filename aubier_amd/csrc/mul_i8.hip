@@ -1,10 +1,12 @@
 // mul_i8.hip -- the product of int8 rows and int8 weights with a scale for each row and each channel
-// (mla_m4_mul_i8): y[t][c] = xs[t] ws[c] sum_k w[c][k] x[t][k], the sum exact in 32 bits (k <= 131,056), then two f32 products and,
-// for an f16 result, one rounding more.  Integer sums have no order, so however a form cuts k the result is the same bit for bit.
+// (mla_m4_mul_i8): y[t][c] = xs[t] ws[c] sum_k w[c][k] x[t][k], the sum exact in 32 bits (k <= 131,056), rounded to f32 (exactly
+// up to 2^24), then two f32 products and, for an f16 result, one rounding more.  Integer sums have no order, so however a form cuts k the
+// result is the same bit for bit.
 //
-// Three kernels, as three things bound it.  One to 32 rows: reading the weights once, and latency (direct_kernel).  Tens to hundreds
-// of rows: what a CU can fetch and how many CUs the shape keeps busy (split_kernel, and sum_kernel where k is cut).  More: the matrix
-// instructions (tile_kernel).  choose() (mul_i8_forms.h) estimates each form's time.
+// Three kernels, as three things bound it.  Few rows (48 at most, fewer of more weights: up to 32 with 2112 x 4096, 8 with 7168 x 7168, 1
+// with 24,576 x 7168): reading the weights once, and latency (direct_kernel).  From there to hundreds: what a CU can fetch and how many
+// CUs the shape keeps busy (split_kernel, and sum_kernel where k is cut).  More: the matrix instructions (tile_kernel).  choose()
+// (mul_i8_forms.h) estimates each form's time.
 #include "mla_common.h"
 #include "mul_i8_forms.h"
 #include "rows.h"
@@ -50,8 +52,8 @@ __device__ __forceinline__ void put(char * p, bool f16, bool whole, int left, co
 // direct_kernel: few rows.  A workgroup of NW waves takes 16 TN channels and 16 rows; wave w takes the 256-byte runs
 // w, w + NW, ... of k, its operands straight from memory (lane l: row l % 16, 16 bytes at 16 (l / 16), as
 // v_mfma_i32_16x16x64_i8 takes both; a run is 4 of its steps), and the waves' integers are added in LDS.  Integer sums have
-// no order, so the result is the same however k is cut.  Bound by memory latency and by what a CU fetches (40 KB/us): 1 row x 576
-// x 7168 5.9 us, x 7168 x 4096 8.1 us (3.6 TB/s), x 24576 x 1536 8.3 us (4.6 TB/s).
+// no order, so the result is the same however k is cut.  Bound by memory latency (a wave has one run's loads on their way, and sends
+// the next run's when they are here) and by what a CU fetches (40 KB/us): 1 row x 576 x 7168 5.9 us, x 7168 x 4096 8.1 us (3.6 TB/s), x 24576 x 1536 8.3 us (4.6 TB/s).
 template <int NW, int TN>
 __global__ __launch_bounds__(64 * NW) void direct_kernel(MulArgs a) {
     constexpr int U = 4, RUN = 64 * U;

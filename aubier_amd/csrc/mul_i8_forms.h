@@ -13,7 +13,7 @@ namespace rows {
 // the smaller ones in the card's 256 MB cache); the form they choose takes 1.01 times the best form's time in the mean, 1.19 at most
 // (150 rows x 24,576 x 1536), and with operands out of memory (1,500 times of 96 shapes) 1.02 and 1.22 (1 x 7168 x 16,384).  What they weigh:
 // 64 rows x 7168 x 4096 takes 9.7 us in tiles of 32 x 64 and 11.5 in 64 x 64 (112 workgroups leave half of the CUs idle), 64 x 576 x
-// 7168 takes 7.5 us with k in 4 parts and 11.1 in one, 4,001 x 4096 x 4096 71 us in tiles of 256 and 86 in tiles of 128, 200 x
+// 7168 takes 7.7 us with k in 7 parts and 10.9 in one, 32 x 2112 x 7168 9.0 in 3 and 15.1, 4,001 x 4096 x 4096 71 us in tiles of 256 and 86 in tiles of 128, 200 x
 // 24,576 x 1536 32 and 23, and 1,500 x 7168 x 4096 takes 54 us in 192 x 256 (228 workgroups, one round), 64 in 256 x 256 and 76 in 128.
 struct Form {
     int kind, bn, bm;

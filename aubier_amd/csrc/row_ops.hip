@@ -10,8 +10,8 @@
 // 64-bit vector instructions is that of 32-bit ones and the kernel waits for memory.
 //
 // qrope_kernel: a wavefront per token; a lane turns the same pairs of several heads, so an angle is taken once for them.  5,000 x 40
-// heads of f16: 16.3 us (4.7 TB/s); 64 x 32: 3.7 us, of which the launch takes 2.2, the position, the angle in 64 bits and a head's
-// values behind one another the rest.
+// heads of f16: 16.3 us (4.7 TB/s); 64 x 32: 3.7 us, of which the launch takes 2.2, the position, the angle in 64 bits and the heads the
+// rest: a lane's heads come one behind the other, as a load waits for the store before it (dst may be q).
 #include "mla_common.h"
 #include "rows.h"
 
@@ -129,7 +129,8 @@ __global__ __launch_bounds__(NT, C > 3 && NT <= 512 ? 2 : 4) void norm_kernel(No
     const int tid = threadIdx.x;
     constexpr bool PLAIN = RES == PIECES;
     const bool i8 = PLAIN || a.dst_type == OUT_I8;
-    // Where the registers hold them, weights are loaded ahead of the reductions, and the next row's values ahead of this one's end.
+    // Weights are loaded ahead of the reductions, and the next row's values ahead of this one's end, but not of rows over 12,288 values
+    // (of which those up to 16,384 use 44 to 92 of 128 registers without, and wider ones all)
     constexpr bool EARLY = C <= (NT > 512 ? 3 : 6), AHEAD = EARLY && !ONE;
     int turn = 0;
     auto me = [&]() {                                       // (a wide row's places are worked out anew, not held from use to use)
@@ -174,7 +175,8 @@ __global__ __launch_bounds__(NT, C > 3 && NT <= 512 ? 2 : 4) void norm_kernel(No
         for (int i = 0; i < C; ++i) w[i] = weight(i, from);
     };
     // A wide row's groups are taken two after two, as the 64-bit forms of all of them at once, and the places that me() hides, do not fit
-    // in the registers (64 rows of 16,384: 10.9 us; 18.0 where they spill, and of 24,576 20 and 55)
+    // in the registers (64 rows of 16,384: 10.9 us; 18.0 where they spill, and of 24,576 20 and 55).  With a residual rows over 16,384 values
+    // still spill 6 to 25 registers.
     auto two = [&](int i) {
         if constexpr (!EARLY) {
             if (i & 1) __builtin_amdgcn_sched_barrier(0);
